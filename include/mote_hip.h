@@ -1,6 +1,7 @@
 /*
  * mote_hip.h: C ABI of libmote_hip.so, the MI355X (gfx950) implementation of
- * Mote's Q4_0 quantized-linear path, RMSNorm and RoPE.
+ * Mote's Q4_0 quantized-linear path, RMSNorm and RoPE, and of the attention
+ * between them.
  *
  * Conventions (all of them those of the reference's Rust FFI,
  * crates/mote-backend-hip/src/ffi.rs:8-13): pointers are untyped device
@@ -284,6 +285,114 @@ int mote_hip_rope_qk_f16(const void* q_input, const void* k_input, const void* c
  * or theta <= 0. */
 int mote_hip_rope_tables_f32(const void* positions, void* cos_out, void* sin_out,
                              uint64_t tokens, uint64_t rotary_dim, double theta, void* stream);
+
+/* ---- Attention over packed prompts ----------------------------------------- */
+/* [new] No counterpart in the reference.  Sequences of different lengths lie one
+ * behind the other: sequence s has query rows query_offsets[s] up to
+ * query_offsets[s + 1] and key rows key_offsets[s] up to key_offsets[s + 1]
+ * (int32, sequences + 1 of each, on the device, ascending from 0 to query_tokens
+ * and key_tokens; key_offsets NULL: the query offsets).  q and output are f16
+ * rows of q_heads x head_dim, k and v of kv_heads x head_dim, a row `stride`
+ * elements after the one before; query head h reads key head
+ * h / (q_heads / kv_heads).  Query i of a sequence with n queries and t keys has
+ * position i + t - n: with causal = 1 it sees the keys up to its position, and
+ * with window > 0 only the last `window` of those; with causal = 0 all t keys
+ * (window must be 0).  output = softmax(scale q k^T) v over the keys seen, in f32
+ * with one f16 rounding (the weights of the second product are rounded to f16);
+ * a query that sees none gets zeros.  Keys and values that a query does not see
+ * do not touch its output, whatever they hold.  max_keys: at least the longest
+ * sequence's keys (it only chooses how the work is divided).
+ * Few rows over many keys are computed in parts that a second launch joins, in
+ * `workspace` (16-byte aligned, at least the bytes that
+ * mote_hip_prompt_attention_workspace says for the same sizes, which may be 0);
+ * it holds nothing between calls.  The output may be q itself (same stride), and
+ * must not overlap k or v.  Offsets that run past the rows there are cut to them.
+ * Nothing is allocated, and a call can be captured.
+ * Status: 0; -1 for a null pointer (key_offsets, and a workspace of which 0 bytes
+ * are needed, excepted), an odd f16 or misaligned offsets address, head_dim not a
+ * multiple of 8 or above 256, q_heads not a multiple of kv_heads or above 65535,
+ * an output stride below q_heads x head_dim, a scale that is not finite and
+ * positive, causal other than 0 or 1, a window without causal, key_offsets NULL
+ * with key_tokens other than query_tokens, more than 2^30 rows, too small a
+ * workspace; the launch status.  No sequence, query, head or dimension: 0 without
+ * a launch. */
+int mote_hip_prompt_attention_workspace(uint64_t sequences, uint64_t query_tokens, uint64_t key_tokens,
+                                        uint64_t max_keys, uint64_t q_heads, uint64_t kv_heads,
+                                        uint64_t head_dim, size_t* bytes);
+int mote_hip_prompt_attention_f16(const void* q, const void* k, const void* v, void* output,
+                                  const void* query_offsets, const void* key_offsets, uint64_t sequences,
+                                  uint64_t query_tokens, uint64_t key_tokens, uint64_t max_keys,
+                                  uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim, uint64_t q_stride,
+                                  uint64_t k_stride, uint64_t v_stride, uint64_t output_stride, float scale,
+                                  int causal, uint64_t window, void* workspace, size_t workspace_bytes,
+                                  void* stream);
+
+/* ---- Keys and values in 8 bits ----------------------------------------------- */
+/* [new] No counterpart in the reference.  The cache is cache_blocks blocks of 32
+ * tokens; sequence s's tokens 32 b .. 32 b + 31 are in block
+ * block_table[s x table_blocks + b] (int32).  With P = head_dim rounded up to a
+ * multiple of 32, `cache` is uint8 [cache_blocks][kv_heads][2][32 P] (planes of
+ * keys and of values, 16-byte aligned) and `scales` float
+ * [cache_blocks][kv_heads][2]; byte u of a plane stands for (u - 128) x its scale.
+ * With c = d / 32, element (token t of the block, dimension d) is byte
+ *   keys:   [c][(d % 32) / 8][t % 16][t / 16][d % 8]                of [P/32][4][16][2][8]
+ *   values: [c][(t % 16) / 4][d % 16][(d % 32) / 16][4 (t/16) + t%4]  of the same.
+ *
+ * append: rows offsets[s] up to offsets[s + 1] of k and v (f16, kv_heads x
+ * head_dim, `stride` elements apart) become sequence s's tokens from
+ * positions[s] on (int32).  A plane's scale is the largest magnitude of its
+ * tokens over 127, a byte 128 + the rounded quotient (ties to even).  Tokens
+ * that join a block begun earlier (positions[s] not a multiple of 32) keep its
+ * scale unless one needs a larger one; the block's bytes are then rounded again
+ * to the larger scale.  A block written from its first token on starts anew,
+ * whatever it held, with bytes of 128 in the slots not written.  An infinity or NaN makes its plane's scale NaN, so that
+ * every read of the plane shows it, until the block starts anew.  Blocks shared
+ * by sequences must not be appended to.
+ *
+ * read: the same rows the other way: tokens of sequence s from positions[s] on,
+ * as many as its rows, to k and v, (u - 128) x scale rounded to f16.
+ *
+ * Tokens past the table, and those of blocks whose number is not below
+ * cache_blocks, are left out.  Nothing is allocated, and a call can be captured.
+ * Status: 0; -1 for a null pointer, an odd f16 address, int32 or float arrays off
+ * their alignment, a cache off the 16-byte grid, head_dim not a multiple of 8 or
+ * above 256, more than 65535 heads, 2^30 tokens or 2^25 blocks of a sequence (for
+ * read, a stride below kv_heads x head_dim); the launch status.  No sequence,
+ * token, head or dimension: 0 without a launch. */
+int mote_hip_kv_cache_append_q8(const void* k, const void* v, const void* offsets, const void* positions,
+                                const void* block_table, void* cache, void* scales, uint64_t sequences,
+                                uint64_t tokens, uint64_t kv_heads, uint64_t head_dim, uint64_t k_stride,
+                                uint64_t v_stride, uint64_t table_blocks, uint64_t cache_blocks, void* stream);
+int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* scales, const void* offsets,
+                                  const void* positions, const void* block_table, void* k, void* v,
+                                  uint64_t sequences, uint64_t tokens, uint64_t kv_heads, uint64_t head_dim,
+                                  uint64_t k_stride, uint64_t v_stride, uint64_t table_blocks,
+                                  uint64_t cache_blocks, void* stream);
+
+/* [new] Attention of the last tokens of each sequence over the cache: sequence s
+ * holds lengths[s] tokens (int32, its queries' own included), and its n query
+ * rows, query_offsets[s] up to query_offsets[s + 1] (NULL: row s alone), are the
+ * last n of them: query i has position lengths[s] - n + i and sees the tokens up
+ * to it, with window > 0 only the last `window` of those.  Formula, heads,
+ * strides, types, rows that see nothing, workspace and statuses as for the prompt
+ * attention above, with the cache's values (u - 128) x scale for k and v; the
+ * cache's own requirements as for append.  max_queries: at least the largest n
+ * (rows past it are not computed); max_context: at least the largest length (it
+ * only chooses how the work is divided).  query_offsets NULL needs query_tokens =
+ * sequences and max_queries = 1.  Blocks whose number is not below cache_blocks
+ * count as not there.  A plane whose scale is NaN makes every query NaN that
+ * sees one of its tokens.  Nothing is allocated, and a call can be captured. */
+int mote_hip_cache_attention_workspace(uint64_t sequences, uint64_t query_tokens, uint64_t max_queries,
+                                       uint64_t max_context, uint64_t q_heads, uint64_t kv_heads,
+                                       uint64_t head_dim, size_t* bytes);
+int mote_hip_cache_attention_q8_f16(const void* q, const void* cache, const void* scales,
+                                    const void* query_offsets, const void* lengths, const void* block_table,
+                                    void* output, uint64_t sequences, uint64_t query_tokens,
+                                    uint64_t max_queries, uint64_t max_context, uint64_t q_heads,
+                                    uint64_t kv_heads, uint64_t head_dim, uint64_t q_stride,
+                                    uint64_t output_stride, uint64_t table_blocks, uint64_t cache_blocks,
+                                    float scale, uint64_t window, void* workspace, size_t workspace_bytes,
+                                    void* stream);
 
 #ifdef __cplusplus
 }

@@ -86,6 +86,18 @@ SIGNATURES = {
         [_P, _P, _P, _P, _P, _P, _U64, _U64, _U64, _U64, _U64, ctypes.c_uint32, _P],
     ),
     "mote_hip_rope_tables_f32": (_I, [_P, _P, _P, _U64, _U64, ctypes.c_double, _P]),
+    "mote_hip_prompt_attention_workspace": (_I, [_U64] * 7 + [ctypes.POINTER(_SZ)]),
+    "mote_hip_prompt_attention_f16": (
+        _I,
+        [_P] * 6 + [_U64] * 11 + [ctypes.c_float, _I, _U64, _P, _SZ, _P],
+    ),
+    "mote_hip_kv_cache_append_q8": (_I, [_P] * 7 + [_U64] * 8 + [_P]),
+    "mote_hip_kv_cache_read_q8_f16": (_I, [_P] * 7 + [_U64] * 8 + [_P]),
+    "mote_hip_cache_attention_workspace": (_I, [_U64] * 7 + [ctypes.POINTER(_SZ)]),
+    "mote_hip_cache_attention_q8_f16": (
+        _I,
+        [_P] * 7 + [_U64] * 11 + [ctypes.c_float, _U64, _P, _SZ, _P],
+    ),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,379 @@
+// Attention over the 8-bit cache: the last n tokens of each sequence (one when
+// decoding, several for drafts or a chunk of a prompt) over all its cached
+// tokens, or the last `window` of them.
+//
+// The query heads of a key head and the sequence's query tokens are the rows of
+// one small matrix product, so each cached byte is read once for all of them:
+// S^T = K Q^T and O^T = V^T P^T on the 16 x 16 x 32 matrix instruction, 16 rows a
+// tile.  With keys as the instruction's rows, a lane ends with the scores of one
+// query row for tokens 4 g .. 4 g + 3 of each half block (g = lane / 16), which is
+// the operand that the second product wants of it: no score leaves its register.
+// Bytes become the exact binary16 integers u - 128; the planes' scales are
+// applied in 32 bits, to the scores and to each block's sums.
+//
+// One pass is bound by the cache's bytes.  A workgroup takes `chunk` blocks of
+// one (sequence, rows, key head), its four waves every fourth block each, and
+// joins the waves' sums through LDS; the chunks' sums join in a second launch.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "attention.hpp"
+
+namespace mote::attention {
+namespace {
+
+struct CacheAttentionArgs {
+    const _Float16* q;
+    const uint8_t* cache;
+    const float* scales;
+    const int32_t* offsets;  // null: one query of each sequence
+    const int32_t* lengths;
+    const int32_t* table;
+    _Float16* output;
+    float2* stats;  // null: one part, written to output
+    float* sums;
+    uint64_t q_stride, out_stride;
+    uint32_t sequences, tokens, row_tiles, heads, kv_heads, head_dim, table_blocks, cache_blocks, window, chunk, parts;
+    float exponent;  // scale log2(e)
+};
+
+__device__ __forceinline__ f32x4 mfma16(const f16x8& a, const f16x8& b, const f32x4& c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Eight bytes as the binary16 integers u - 128: a byte under 0x64 reads 1024 + u.
+__device__ __forceinline__ f16x8 values_of(uint32_t lo, uint32_t hi) {
+    const f16x2 bias = {static_cast<_Float16>(-1152.0f), static_cast<_Float16>(-1152.0f)};
+    const uint32_t top = 0x64646464u;
+    const f16x2 a = as_h2(__builtin_amdgcn_perm(top, lo, 0x04010400u)) + bias;
+    const f16x2 b = as_h2(__builtin_amdgcn_perm(top, lo, 0x04030402u)) + bias;
+    const f16x2 c = as_h2(__builtin_amdgcn_perm(top, hi, 0x04010400u)) + bias;
+    const f16x2 d = as_h2(__builtin_amdgcn_perm(top, hi, 0x04030402u)) + bias;
+    return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// C: 32-dimension groups of the padded head; NT: 16-row tiles of a workgroup.
+template <int C, int NT>
+__global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttentionArgs a) {
+    constexpr int kRows = 16 * NT;
+    constexpr int kJoin = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // dimension groups joined at a time: 256 pieces of 8
+    constexpr int kRowFloats = 32 * kJoin + 4;            // padded: rows start 4 banks apart
+    __shared__ __align__(16) float sums_of[4][kRows][kRowFloats];
+    __shared__ float2 stats_of[4][kRows];
+
+    uint32_t id = blockIdx.x;
+    const uint32_t part = id % a.parts;
+    id /= a.parts;
+    const uint32_t kv_head = id % a.kv_heads;
+    id /= a.kv_heads;
+    const uint32_t row_tile = id % a.row_tiles, seq = id / a.row_tiles;
+
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const uint32_t group = a.heads / a.kv_heads;
+    Span rows = {static_cast<int>(seq), 1};
+    if (a.offsets != nullptr) rows = span_of(a.offsets, seq, a.tokens);
+    const uint32_t row0 = row_tile * kRows, all_rows = static_cast<uint32_t>(rows.n) * group;
+    if (row0 >= all_rows) return;
+    const uint32_t here = min(all_rows - row0, static_cast<uint32_t>(kRows));
+    const int most_length = static_cast<int>(a.table_blocks * kBlockTokens);
+    const int length = min(max(a.lengths[seq], 0), most_length);
+    const int shift = length - rows.n;  // position of the first query; below 0: it sees nothing
+    const int first_token = static_cast<int>(row0 / group), last_token = static_cast<int>((row0 + here - 1) / group);
+    // Blocks that any of the rows sees: [b0, b1)
+    const int last_seen = shift + last_token;
+    const int first_seen = a.window ? max(0, shift + first_token - static_cast<int>(a.window) + 1) : 0;
+    const int start = first_seen / static_cast<int>(kBlockTokens);
+    const int b0 = start + static_cast<int>(part * a.chunk);
+    const int end = (last_seen + 1 + 31) / static_cast<int>(kBlockTokens);
+    const int b1 = part + 1 == a.parts ? end : min(b0 + static_cast<int>(a.chunk), end);  // the last part: all that is left
+
+    // Queries: the lane's row of each tile, and its position.
+    f16x8 qf[NT][C];
+    int pos[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const uint32_t r = min(row0 + 16 * t + n, all_rows - 1);  // rows past the last are not written
+        const uint32_t token = r / group, head = kv_head * group + r % group;
+        pos[t] = shift + static_cast<int>(token);
+        const _Float16* q = a.q + static_cast<uint64_t>(rows.at + token) * a.q_stride +
+                            static_cast<uint64_t>(head) * a.head_dim;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const uint32_t d = 32 * c + 8 * g;
+            u32x4 v = {0, 0, 0, 0};
+            if (d < a.head_dim) v = *reinterpret_cast<const u32x4_a2*>(q + d);
+            qf[t][c] = __builtin_bit_cast(f16x8, v);
+        }
+    }
+
+    f32x4 o[NT][2 * C];
+    float m[NT], l[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -infinity();
+        l[t] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * C; ++i) o[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const int32_t* table = a.table + static_cast<uint64_t>(seq) * a.table_blocks;
+    constexpr uint32_t kPlane = 1024 * C;
+    for (int b = b0 + static_cast<int>(wave); b < b1; b += 4) {
+        const int32_t block = table[b];
+        if (block < 0 || static_cast<uint32_t>(block) >= a.cache_blocks) continue;  // none there
+        const uint64_t at = static_cast<uint64_t>(block) * a.kv_heads + kv_head;
+        const uint8_t* planes = a.cache + at * (2 * kPlane) + lane * 16;
+        const float key_scale = a.scales[at * 2], value_scale = a.scales[at * 2 + 1];
+        u32x4 kb[C], vb[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) kb[c] = *reinterpret_cast<const u32x4*>(planes + 1024 * c);
+#pragma unroll
+        for (int c = 0; c < C; ++c) vb[c] = *reinterpret_cast<const u32x4*>(planes + kPlane + 1024 * c);
+        f32x4 s[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const f16x8 k0 = values_of(kb[c][0], kb[c][1]), k1 = values_of(kb[c][2], kb[c][3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                s[t][0] = mfma16(k0, qf[t][c], s[t][0]);
+                s[t][1] = mfma16(k1, qf[t][c], s[t][1]);
+            }
+        }
+        const int j0 = b * static_cast<int>(kBlockTokens);
+        const bool edge = j0 + 31 > shift + first_token ||
+                          (a.window && j0 <= last_seen - static_cast<int>(a.window));
+        const float factor = key_scale * a.exponent;
+        f16x8 p[NT];
+        float to_values[NT];  // 0 for a row that sees none of the block, whatever its scale
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            to_values[t] = value_scale;
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = s[t][i >> 2][i & 3] * factor;
+            if (edge) {
+                if (j0 > pos[t] || (a.window && j0 + 31 <= pos[t] - static_cast<int>(a.window))) to_values[t] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int j = j0 + 16 * (i >> 2) + 4 * g + (i & 3);
+                    const bool sees = j <= pos[t] && (!a.window || j > pos[t] - static_cast<int>(a.window));
+                    x[i] = sees ? x[i] : -infinity();
+                }
+            }
+            float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+            top = max_of(across_halves(max_of(across_rows16(top))));
+            if (wave_any(top > m[t] + kGrowth)) {
+                const float to = fmaxf(m[t], top);
+                const float w = m[t] == to ? 1.0f : exp2_fast(m[t] - to);  // also where both are -inf
+                m[t] = to;
+                l[t] *= w;
+#pragma unroll
+                for (int i = 0; i < 2 * C; ++i) o[t][i] *= w;
+            }
+            const float base = m[t] == -infinity() ? 0.0f : m[t] - kShift;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float e = exp2_fast(x[i] - base);
+                l[t] += e;
+                p[t][i] = static_cast<_Float16>(e);
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const f16x8 v0 = values_of(vb[c][0], vb[c][1]), v1 = values_of(vb[c][2], vb[c][3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+                o[t][2 * c] += to_values[t] * mfma16(v0, p[t], zero);
+                o[t][2 * c + 1] += to_values[t] * mfma16(v1, p[t], zero);
+            }
+        }
+    }
+
+    // The waves' sums join, a few dimension groups at a time.
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float all = sum_of(across_halves(sum_of(across_rows16(l[t]))));
+        if (g == 0) stats_of[wave][16 * t + n] = float2{m[t], all};
+    }
+    const uint64_t part_row = static_cast<uint64_t>(part) * a.tokens * a.heads;
+    constexpr int kPieces = 4 * kJoin;  // of eight dimensions, a row
+    const uint32_t row = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
+    const uint32_t r = row0 + row, token = r / group, head = kv_head * group + r % group;
+#pragma unroll
+    for (int c0 = 0; c0 < C; c0 += kJoin) {
+        if (c0 != 0) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2 * kJoin; ++i)
+                if (c0 * 2 + i < 2 * C)
+                    *reinterpret_cast<f32x4*>(&sums_of[wave][16 * t + n][16 * i + 4 * g]) = o[t][c0 * 2 + i];
+        __syncthreads();
+        const uint32_t d = 32 * c0 + 8 * piece;
+        if (row >= here || d >= a.head_dim) continue;
+        float top = -infinity();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) top = fmaxf(top, stats_of[w][row].x);
+        f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 ml = stats_of[w][row];
+            const float weight = ml.x == -infinity() ? ml.y : exp2_fast(ml.x - top);  // saw nothing: 0, or NaN
+            sum = __builtin_fmaf(weight, ml.y, sum);
+            lo += weight * *reinterpret_cast<const f32x4*>(&sums_of[w][row][8 * piece]);
+            hi += weight * *reinterpret_cast<const f32x4*>(&sums_of[w][row][8 * piece + 4]);
+        }
+        if (a.stats == nullptr) {
+            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+            lo *= inv;
+            hi *= inv;
+            const f16x8 y = {static_cast<_Float16>(lo.x), static_cast<_Float16>(lo.y), static_cast<_Float16>(lo.z),
+                             static_cast<_Float16>(lo.w), static_cast<_Float16>(hi.x), static_cast<_Float16>(hi.y),
+                             static_cast<_Float16>(hi.z), static_cast<_Float16>(hi.w)};
+            _Float16* out = a.output + static_cast<uint64_t>(rows.at + token) * a.out_stride +
+                            static_cast<uint64_t>(head) * a.head_dim + d;
+            *reinterpret_cast<u32x4_a2*>(out) = __builtin_bit_cast(u32x4, y);
+        } else {
+            const uint64_t at = part_row + static_cast<uint64_t>(rows.at + token) * a.heads + head;
+            if (d == 0) a.stats[at] = float2{top, sum};
+            if (sum == 0.0f) continue;  // saw nothing: not read
+            float* out = a.sums + at * a.head_dim + d;
+            *reinterpret_cast<f32x4*>(out) = lo;
+            *reinterpret_cast<f32x4*>(out + 4) = hi;
+        }
+    }
+}
+
+struct CachePlan {
+    uint32_t row_tiles, tile_rows, chunk, parts;
+};
+
+CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_t max_context, uint64_t heads,
+                               uint64_t kv_heads, uint64_t head_dim) {
+    const uint64_t rows = max_queries * (heads / kv_heads);
+    CachePlan p{};
+    p.tile_rows = rows <= 16 ? 16 : rows <= 32 || head_dim > 128 ? 32 : 64;
+    p.row_tiles = static_cast<uint32_t>((rows + p.tile_rows - 1) / p.tile_rows);
+    const uint64_t blocks = (max_context + kBlockTokens - 1) / kBlockTokens + 1;
+    const uint64_t groups = sequences * p.row_tiles * kv_heads;
+    // About 2048 workgroups (eight on a compute unit), none of fewer than 8 blocks (two a wave).
+    uint64_t parts = groups >= 2048 ? 1 : (2048 + groups - 1) / groups;
+    uint64_t chunk = (blocks + parts - 1) / parts;
+    if (chunk < 8) chunk = 8;
+    parts = (blocks + chunk - 1) / chunk;
+    p.chunk = static_cast<uint32_t>(chunk);
+    p.parts = static_cast<uint32_t>(parts);
+    return p;
+}
+
+template <int NT>
+auto kernel_of(uint32_t c) -> void (*)(CacheAttentionArgs) {
+    switch (c) {
+        case 1: return cache_attention_kernel<1, NT>;
+        case 2: return cache_attention_kernel<2, NT>;
+        case 3: return cache_attention_kernel<3, NT>;
+        case 4: return cache_attention_kernel<4, NT>;
+        default: break;
+    }
+    if constexpr (NT <= 2) {
+        switch (c) {
+            case 5: return cache_attention_kernel<5, NT>;
+            case 6: return cache_attention_kernel<6, NT>;
+            case 7: return cache_attention_kernel<7, NT>;
+            case 8: return cache_attention_kernel<8, NT>;
+            default: break;
+        }
+    }
+    return nullptr;
+}
+
+bool bad_shape(uint64_t sequences, uint64_t query_tokens, uint64_t max_queries, uint64_t max_context, uint64_t heads,
+               uint64_t kv_heads, uint64_t head_dim) {
+    if (head_dim % 8 != 0 || head_dim > kMostHeadDim || heads > 65535 || kv_heads > heads) return true;
+    if (heads != 0 && (kv_heads == 0 || heads % kv_heads != 0)) return true;
+    return query_tokens > kMostTokens || sequences > kMostTokens || max_queries > kMostTokens ||
+           max_context > kMostTokens || query_tokens * heads > 0xFFFFFFFFull || max_queries * heads > 0x7FFFFFFFull;
+}
+
+}  // namespace
+}  // namespace mote::attention
+
+MOTE_EXPORT int mote_hip_cache_attention_workspace(uint64_t sequences, uint64_t query_tokens, uint64_t max_queries,
+                                                  uint64_t max_context, uint64_t q_heads, uint64_t kv_heads,
+                                                  uint64_t head_dim, size_t* bytes) noexcept {
+    using namespace mote::attention;
+    if (!bytes) return kInvalid;
+    *bytes = 0;
+    if (bad_shape(sequences, query_tokens, max_queries, max_context, q_heads, kv_heads, head_dim)) return kInvalid;
+    if (sequences == 0 || query_tokens == 0 || max_queries == 0 || q_heads == 0 || head_dim == 0) return 0;
+    const CachePlan p = plan_cache_attention(sequences, max_queries, max_context, q_heads, kv_heads, head_dim);
+    *bytes = static_cast<size_t>(parts_bytes(query_tokens * q_heads, p.parts, head_dim));
+    return 0;
+}
+
+MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache, const void* scales,
+                                               const void* query_offsets, const void* lengths,
+                                               const void* block_table, void* output, uint64_t sequences,
+                                               uint64_t query_tokens, uint64_t max_queries, uint64_t max_context,
+                                               uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim,
+                                               uint64_t q_stride, uint64_t output_stride, uint64_t table_blocks,
+                                               uint64_t cache_blocks, float scale, uint64_t window, void* workspace,
+                                               size_t workspace_bytes, void* stream) noexcept {
+    using namespace mote::attention;
+    if (!q || !cache || !scales || !lengths || !block_table || !output || !stream) return kInvalid;
+    if (bad_shape(sequences, query_tokens, max_queries, max_context, q_heads, kv_heads, head_dim)) return kInvalid;
+    const float exponent = scale * kLog2e;
+    if (!(scale > 0.0f) || !std::isfinite(exponent)) return kInvalid;
+    if (table_blocks > kMostTokens / kBlockTokens || cache_blocks > 0x7FFFFFFFu) return kInvalid;
+    if (!query_offsets && (query_tokens != sequences || max_queries > 1)) return kInvalid;
+    if (output_stride < q_heads * head_dim) return kInvalid;
+    if (odd_address(q) || odd_address(output) || off_grid(cache, 16) || off_grid(scales, 4) ||
+        off_grid(query_offsets, 4) || off_grid(lengths, 4) || off_grid(block_table, 4))
+        return kInvalid;
+    if (sequences == 0 || query_tokens == 0 || max_queries == 0 || q_heads == 0 || head_dim == 0) return 0;
+    const CachePlan p = plan_cache_attention(sequences, max_queries, max_context, q_heads, kv_heads, head_dim);
+    const uint64_t rows = query_tokens * q_heads;
+    const uint64_t need = parts_bytes(rows, p.parts, head_dim);
+    if (need > 0 && (!workspace || off_grid(workspace, 16) || workspace_bytes < need)) return kInvalid;
+    if (sequences * p.row_tiles > kMostGrid / kv_heads / p.parts) return kInvalid;
+    CacheAttentionArgs a{};
+    a.q = static_cast<const _Float16*>(q);
+    a.cache = static_cast<const uint8_t*>(cache);
+    a.scales = static_cast<const float*>(scales);
+    a.offsets = static_cast<const int32_t*>(query_offsets);
+    a.lengths = static_cast<const int32_t*>(lengths);
+    a.table = static_cast<const int32_t*>(block_table);
+    a.output = static_cast<_Float16*>(output);
+    if (p.parts > 1) {
+        a.stats = static_cast<float2*>(workspace);
+        a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(rows, p.parts));
+    }
+    a.q_stride = q_stride;
+    a.out_stride = output_stride;
+    a.sequences = static_cast<uint32_t>(sequences);
+    a.tokens = static_cast<uint32_t>(query_tokens);
+    a.row_tiles = p.row_tiles;
+    a.heads = static_cast<uint32_t>(q_heads);
+    a.kv_heads = static_cast<uint32_t>(kv_heads);
+    a.head_dim = static_cast<uint32_t>(head_dim);
+    a.table_blocks = static_cast<uint32_t>(table_blocks);
+    a.cache_blocks = static_cast<uint32_t>(cache_blocks);
+    a.window = window >= table_blocks * kBlockTokens ? 0 : static_cast<uint32_t>(window);  // no shorter than any context
+    a.chunk = p.chunk;
+    a.parts = p.parts;
+    a.exponent = exponent;
+    const uint32_t c = padded_dim(a.head_dim) / 32;
+    const auto kernel = p.tile_rows == 16 ? kernel_of<1>(c) : p.tile_rows == 32 ? kernel_of<2>(c) : kernel_of<4>(c);
+    const auto s = static_cast<hipStream_t>(stream);
+    const uint64_t groups = sequences * p.row_tiles * kv_heads * p.parts;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, a);
+    const int status = static_cast<int>(hipGetLastError());
+    if (status != 0 || p.parts <= 1) return status;
+    return join_parts(workspace, output, rows, p.parts, q_heads, head_dim, output_stride, s);
+}

@@ -1,0 +1,367 @@
+// Attention of packed prompts: sequences of different lengths one behind the
+// other, grouped heads, causal or not, with or without a sliding window, over
+// binary16 keys and values.
+//
+// A workgroup takes 128 query rows of one head, 32 a wave, and walks the keys
+// they see in tiles of 64 that the four waves share through LDS.  S^T = K Q^T
+// and O^T = V^T P^T on the 32 x 32 x 16 matrix instruction: with keys as the
+// instruction's rows a lane ends with the scores of one query row, the running
+// maximum and sum need one exchange between the wave's halves, and the scores
+// are the operand of the second product where they lie.  Its other operand,
+// V^T, comes out of the row-major tile through LDS transpose reads.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "attention.hpp"
+#include "tile_ops.hpp"
+
+namespace mote::attention {
+namespace {
+
+constexpr uint32_t kTileRows = 128;
+constexpr int kTileKeys = 64;
+
+struct PromptArgs {
+    const _Float16* q;
+    const _Float16* k;
+    const _Float16* v;
+    _Float16* output;
+    const int32_t* query_offsets;
+    const int32_t* key_offsets;
+    float2* stats;  // null: one part, written to output
+    float* sums;
+    uint64_t q_stride, k_stride, v_stride, out_stride;
+    uint32_t sequences, tokens, keys, heads, kv_heads, head_dim, window, causal, parts;
+    float exponent;  // scale log2(e)
+};
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
+
+// Four rows by sixteen columns of a row-major binary16 tile, transposed: lane i
+// of each sixteen gives the address of piece i % 4 of row i / 4 and gets column i.
+__device__ __forceinline__ u32x2 read_transposed(const uint8_t* at) {
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at)));
+}
+
+// Position of 16-byte chunk c of row r in a tile of CH chunks a row: chunks of a
+// row are exchanged within aligned groups of a power of two, so that rows read
+// together lie in different banks.
+template <int CH>
+__device__ __forceinline__ constexpr int group_of() { return (CH & -CH) > 16 ? 16 : (CH & -CH); }
+template <int CH>
+__device__ __forceinline__ int key_chunk(int r, int c) { return r * CH + (c ^ (r & (group_of<CH>() - 1))); }
+template <int CH>
+__device__ __forceinline__ int value_chunk(int r, int c) { return r * CH + (c ^ ((2 * r) & (group_of<CH>() - 1))); }
+
+// The pair with halves that are not finite replaced by zero.
+__device__ __forceinline__ uint32_t finite_of(uint32_t pair) {
+    uint32_t r = pair;
+    if ((pair & 0x7C00u) == 0x7C00u) r &= 0xFFFF0000u;
+    if ((pair & 0x7C000000u) == 0x7C000000u) r &= 0x0000FFFFu;
+    return r;
+}
+
+template <int DP>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kernel(PromptArgs a) {
+    constexpr int CH = DP / 8, KS = DP / 16, DT = DP / 32;
+    constexpr int kLoads = kTileKeys * CH / 256;  // 16-byte chunks of a thread in each tile
+    __shared__ u32x4 key_tile[kTileKeys * CH];
+    __shared__ u32x4 value_tile[kTileKeys * CH];
+    __shared__ int taken_out;  // the last tile, from 1, with values that are not finite taken out
+
+    const uint32_t head = blockIdx.y, part = blockIdx.z;
+    const uint32_t kv_head = head / (a.heads / a.kv_heads);
+    const Unit u = locate(blockIdx.x, a.sequences, [&](uint32_t s) {
+        return (static_cast<uint32_t>(span_of(a.query_offsets, s, a.tokens).n) + kTileRows - 1) / kTileRows;
+    });
+    if (!u.found) return;
+    const Span queries = span_of(a.query_offsets, u.sequence, a.tokens);
+    const Span keys = span_of(a.key_offsets, u.sequence, a.keys);
+    const int row0 = static_cast<int>((u.of - 1 - u.local) * kTileRows);  // the longest walks first
+    const int shift = keys.n - queries.n;  // position of the first query
+    const int last_row = min(row0 + static_cast<int>(kTileRows), queries.n) - 1;
+    const int window = static_cast<int>(a.window);
+
+    // The keys that any row of the tile sees, and this part's tiles of them.
+    const int end = a.causal ? min(max(last_row + shift + 1, 0), keys.n) : keys.n;
+    const int begin = window ? min(max(row0 + shift - window + 1, 0), end) & ~(kTileKeys - 1) : 0;
+    const int tiles = (end - begin + kTileKeys - 1) / kTileKeys;
+    const int per_part = (tiles + static_cast<int>(a.parts) - 1) / static_cast<int>(a.parts);
+    const int tile0 = static_cast<int>(part) * per_part, tile1 = min(tiles, tile0 + per_part);
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const int wave_row = row0 + 32 * wave;
+    const int row = wave_row + n;
+    const int pos = row + shift;
+    const int wave_last = min(wave_row + 31, queries.n - 1) + shift;  // position of the wave's last row
+
+    f16x8 qf[KS];
+    {
+        const _Float16* q = a.q + static_cast<uint64_t>(queries.at + min(row, queries.n - 1)) * a.q_stride +
+                            static_cast<uint64_t>(head) * a.head_dim;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const uint32_t d = 16 * i + 8 * h;
+            u32x4 x = {0, 0, 0, 0};
+            if (d < a.head_dim) x = *reinterpret_cast<const u32x4_a2*>(q + d);
+            qf[i] = __builtin_bit_cast(f16x8, x);
+        }
+    }
+
+    const _Float16* const k = a.k + static_cast<uint64_t>(keys.at) * a.k_stride + static_cast<uint64_t>(kv_head) * a.head_dim;
+    const _Float16* const v = a.v + static_cast<uint64_t>(keys.at) * a.v_stride + static_cast<uint64_t>(kv_head) * a.head_dim;
+    u32x4 next_k[kLoads], next_v[kLoads];
+    const auto load_tile = [&](int tile) {
+        const int j0 = begin + tile * kTileKeys;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
+            next_k[i] = next_v[i] = u32x4{0, 0, 0, 0};
+            if (j0 + r < keys.n && 8u * c < a.head_dim) {
+                next_k[i] = *reinterpret_cast<const u32x4_a2*>(k + static_cast<uint64_t>(j0 + r) * a.k_stride + 8 * c);
+                next_v[i] = *reinterpret_cast<const u32x4_a2*>(v + static_cast<uint64_t>(j0 + r) * a.v_stride + 8 * c);
+            }
+        }
+    };
+
+    f32x16 o[DT];
+#pragma unroll
+    for (int i = 0; i < DT; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+    float m = -infinity(), l = 0.0f;
+
+    if (threadIdx.x == 0) taken_out = 0;
+    if (tile0 < tile1) load_tile(tile0);
+    for (int tile = tile0; tile < tile1; ++tile) {
+        __syncthreads();  // the last tile has been read
+        const int j0 = begin + tile * kTileKeys;
+        // Whether some row of the workgroup does not see all of the tile.
+        const bool partly = (a.causal && j0 + kTileKeys - 1 > row0 + shift) || (window && j0 <= last_row + shift - window);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
+            key_tile[key_chunk<CH>(r, c)] = next_k[i];
+            if (partly) {
+                // A value that is not finite must not reach the rows that do not
+                // see its key through a weight of zero.
+                bool bad = false;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t fine = finite_of(next_v[i][w]);
+                    bad |= fine != next_v[i][w];
+                    next_v[i][w] = fine;
+                }
+                if (bad) taken_out = tile + 1;
+            }
+            value_tile[value_chunk<CH>(r, c)] = next_v[i];
+        }
+        __syncthreads();
+        if (tile + 1 < tile1) load_tile(tile + 1);
+        if (a.causal && (j0 > wave_last || (window && j0 + kTileKeys - 1 <= wave_row + shift - window))) continue;
+
+        f32x16 s[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+                s[t] = mfma32(__builtin_bit_cast(f16x8, key_tile[key_chunk<CH>(32 * t + n, 2 * i + h)]), qf[i], s[t]);
+        }
+        const bool masked = j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > wave_row + shift) ||
+                            (window && j0 <= wave_last - window);
+        if (masked) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                const int j = j0 + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * h + (i & 3);
+                const bool sees = j < keys.n && (!a.causal || j <= pos) && (!window || j > pos - window);
+                s[i >> 4][i & 15] = sees ? s[i >> 4][i & 15] : -infinity();
+            }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+        top = max_of(across_halves(top)) * a.exponent;
+        if (wave_any(top > m + kGrowth)) {
+            const float to = fmaxf(m, top);
+            const float w = m == to ? 1.0f : exp2_fast(m - to);  // also where both are -inf
+            m = to;
+            l *= w;
+#pragma unroll
+            for (int i = 0; i < DT; ++i) o[i] *= w;
+        }
+        const float base = m == -infinity() ? 0.0f : m - kShift;
+        f16x8 p[4];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], a.exponent, -base));
+            l += e;
+            p[i >> 3][i & 7] = static_cast<_Float16>(e);
+        }
+
+        // V^T: dimensions 32 i + n, keys 16 c + {4 h .. 4 h + 3, 8 + 4 h ..}.
+        const auto values = [&](int i, int c) {
+            const int r = 16 * c + 4 * h + ((lane & 15) >> 2), piece = lane & 3;
+            const int chunk = 4 * i + 2 * ((lane >> 4) & 1) + (piece >> 1);
+            const uint8_t* tile_at = reinterpret_cast<const uint8_t*>(value_tile);
+            const u32x2 lo = read_transposed(tile_at + value_chunk<CH>(r, chunk) * 16 + 8 * (piece & 1));
+            const u32x2 hi = read_transposed(tile_at + value_chunk<CH>(r + 8, chunk) * 16 + 8 * (piece & 1));
+            return u32x4{lo.x, lo.y, hi.x, hi.y};
+        };
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) o[i] = mfma32(__builtin_bit_cast(f16x8, values(i, c)), p[c], o[i]);
+        if (taken_out == tile + 1) {  // the rows that see those values get them here
+#pragma unroll 1
+            for (int j = j0; j < min(j0 + kTileKeys, keys.n); ++j) {
+                const bool sees = (!a.causal || j <= pos) && (!window || j > pos - window);
+                const _Float16* at = v + static_cast<uint64_t>(j) * a.v_stride;
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const uint32_t d = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
+                        const float x = d < a.head_dim ? static_cast<float>(at[d]) : 0.0f;
+                        if (sees && !(fabsf(x) < infinity())) o[i][r] += x;
+                    }
+            }
+        }
+    }
+
+    l = sum_of(across_halves(l));
+    if (row >= queries.n) return;
+    const uint64_t token = static_cast<uint64_t>(queries.at + row);
+    if (a.stats == nullptr) {
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        _Float16* out = a.output + token * a.out_stride + static_cast<uint64_t>(head) * a.head_dim;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t d = 32 * i + 2 * r + 4 * h;
+                if (d >= a.head_dim) continue;
+                const f16x2 lo = {static_cast<_Float16>(o[i][r] * inv), static_cast<_Float16>(o[i][r + 1] * inv)};
+                const f16x2 hi = {static_cast<_Float16>(o[i][r + 2] * inv), static_cast<_Float16>(o[i][r + 3] * inv)};
+                *reinterpret_cast<u32x2_a2*>(out + d) =
+                    u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+            }
+    } else {
+        const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
+        const uint64_t at = part * rows + token * a.heads + head;
+        const float base = m == -infinity() ? m : m - kShift;
+        if (h == 0) a.stats[at] = float2{base, l};
+        if (l == 0.0f) return;  // saw nothing: not read
+        float* out = a.sums + at * a.head_dim;
+#pragma unroll
+        for (int i = 0; i < DT; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t d = 32 * i + 2 * r + 4 * h;
+                if (d < a.head_dim) *reinterpret_cast<f32x4*>(out + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+            }
+    }
+}
+
+struct PromptPlan {
+    uint32_t tiles, parts;
+};
+
+PromptPlan plan_prompt(uint64_t sequences, uint64_t tokens, uint64_t max_keys, uint64_t heads) {
+    const uint64_t with = sequences < tokens ? sequences : tokens;  // sequences with a query at all
+    PromptPlan p{};
+    p.tiles = static_cast<uint32_t>((tokens + (kTileRows - 1) * with) / kTileRows);
+    const uint64_t groups = p.tiles * heads, most = (max_keys + 255) / 256;  // no part under four tiles
+    uint64_t parts = groups >= 256 ? 1 : 512 / groups;
+    if (parts > most) parts = most;
+    p.parts = static_cast<uint32_t>(parts > 1 ? parts : 1);
+    return p;
+}
+
+bool bad_shape(uint64_t sequences, uint64_t tokens, uint64_t keys, uint64_t max_keys, uint64_t heads,
+               uint64_t kv_heads, uint64_t head_dim) {
+    if (head_dim % 8 != 0 || head_dim > kMostHeadDim || heads > 65535 || kv_heads > heads) return true;
+    if (heads != 0 && (kv_heads == 0 || heads % kv_heads != 0)) return true;
+    return tokens > kMostTokens || keys > kMostTokens || max_keys > kMostTokens || sequences > kMostTokens ||
+           tokens * heads > 0xFFFFFFFFull;
+}
+
+}  // namespace
+}  // namespace mote::attention
+
+MOTE_EXPORT int mote_hip_prompt_attention_workspace(uint64_t sequences, uint64_t query_tokens, uint64_t key_tokens,
+                                                   uint64_t max_keys, uint64_t q_heads, uint64_t kv_heads,
+                                                   uint64_t head_dim, size_t* bytes) noexcept {
+    using namespace mote::attention;
+    if (!bytes) return kInvalid;
+    *bytes = 0;
+    if (bad_shape(sequences, query_tokens, key_tokens, max_keys, q_heads, kv_heads, head_dim)) return kInvalid;
+    if (sequences == 0 || query_tokens == 0 || q_heads == 0 || head_dim == 0) return 0;
+    const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads);
+    *bytes = static_cast<size_t>(parts_bytes(query_tokens * q_heads, p.parts, head_dim));
+    return 0;
+}
+
+MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, const void* v, void* output,
+                                             const void* query_offsets, const void* key_offsets, uint64_t sequences,
+                                             uint64_t query_tokens, uint64_t key_tokens, uint64_t max_keys,
+                                             uint64_t q_heads, uint64_t kv_heads, uint64_t head_dim,
+                                             uint64_t q_stride, uint64_t k_stride, uint64_t v_stride,
+                                             uint64_t output_stride, float scale, int causal, uint64_t window,
+                                             void* workspace, size_t workspace_bytes, void* stream) noexcept {
+    using namespace mote::attention;
+    if (!q || !k || !v || !output || !query_offsets || !stream) return kInvalid;
+    if (bad_shape(sequences, query_tokens, key_tokens, max_keys, q_heads, kv_heads, head_dim)) return kInvalid;
+    const float exponent = scale * kLog2e;
+    if (!(scale > 0.0f) || !std::isfinite(exponent)) return kInvalid;
+    if ((causal != 0 && causal != 1) || (!causal && window != 0)) return kInvalid;
+    if (!key_offsets && key_tokens != query_tokens) return kInvalid;
+    if (output_stride < q_heads * head_dim) return kInvalid;
+    if (odd_address(q) || odd_address(k) || odd_address(v) || odd_address(output) || off_grid(query_offsets, 4) ||
+        off_grid(key_offsets, 4))
+        return kInvalid;
+    if (sequences == 0 || query_tokens == 0 || q_heads == 0 || head_dim == 0) return 0;
+    const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads);
+    const uint64_t rows = query_tokens * q_heads, need = parts_bytes(rows, p.parts, head_dim);
+    if (need > 0 && (!workspace || off_grid(workspace, 16) || workspace_bytes < need)) return kInvalid;
+    if (p.tiles > kMostGrid) return kInvalid;
+    PromptArgs a{};
+    a.q = static_cast<const _Float16*>(q);
+    a.k = static_cast<const _Float16*>(k);
+    a.v = static_cast<const _Float16*>(v);
+    a.output = static_cast<_Float16*>(output);
+    a.query_offsets = static_cast<const int32_t*>(query_offsets);
+    a.key_offsets = static_cast<const int32_t*>(key_offsets ? key_offsets : query_offsets);
+    if (p.parts > 1) {
+        a.stats = static_cast<float2*>(workspace);
+        a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + stats_bytes(rows, p.parts));
+    }
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.out_stride = output_stride;
+    a.sequences = static_cast<uint32_t>(sequences);
+    a.tokens = static_cast<uint32_t>(query_tokens);
+    a.keys = static_cast<uint32_t>(key_tokens);
+    a.heads = static_cast<uint32_t>(q_heads);
+    a.kv_heads = static_cast<uint32_t>(kv_heads);
+    a.head_dim = static_cast<uint32_t>(head_dim);
+    a.window = window >= key_tokens ? 0 : static_cast<uint32_t>(window);  // no shorter than any sequence
+    a.causal = static_cast<uint32_t>(causal);
+    a.parts = p.parts;
+    a.exponent = exponent;
+    const auto kernel = head_dim <= 64    ? prompt_attention_kernel<64>
+                        : head_dim <= 96  ? prompt_attention_kernel<96>
+                        : head_dim <= 128 ? prompt_attention_kernel<128>
+                        : head_dim <= 192 ? prompt_attention_kernel<192>
+                                          : prompt_attention_kernel<256>;
+    const auto s = static_cast<hipStream_t>(stream);
+    hipLaunchKernelGGL(kernel, dim3(p.tiles, a.heads, p.parts), dim3(256), 0, s, a);
+    const int status = static_cast<int>(hipGetLastError());
+    if (status != 0 || p.parts <= 1) return status;
+    return join_parts(workspace, output, rows, p.parts, q_heads, head_dim, output_stride, s);
+}

@@ -116,6 +116,98 @@ def rope_tables_f32(positions, cos, sin, tokens, rotary_dim, theta, stream) -> N
     )
 
 
+KV_BLOCK_TOKENS = 32  # tokens of a block of the 8-bit cache
+
+
+def kv_plane_bytes(head_dim: int) -> int:
+    """Bytes of one head's keys (or values) of a cache block: a block holds
+    2 * kv_heads of them, with as many float scales."""
+    return KV_BLOCK_TOKENS * (-(-head_dim // 32) * 32)
+
+
+def prompt_attention_workspace(sequences, query_tokens, key_tokens, max_keys, q_heads, kv_heads, head_dim) -> int:
+    """Bytes of workspace that prompt_attention_f16 needs for these sizes."""
+    need = ctypes.c_size_t(0)
+    check(
+        lib().mote_hip_prompt_attention_workspace(
+            sequences, query_tokens, key_tokens, max_keys, q_heads, kv_heads, head_dim, ctypes.byref(need)
+        ),
+        "size prompt attention workspace",
+    )
+    return need.value
+
+
+def prompt_attention_f16(q, k, v, out, query_offsets, key_offsets, sequences, query_tokens, key_tokens, max_keys,
+                         q_heads, kv_heads, head_dim, scale, workspace, workspace_bytes, stream, causal=True,
+                         window=0, strides=None) -> None:
+    """Attention of packed sequences over their own keys.  `strides`: elements
+    between the rows of q, k, v and out (None: rows without gaps);
+    `key_offsets` None: the query offsets."""
+    sq, sk, sv, so = strides or (q_heads * head_dim, kv_heads * head_dim, kv_heads * head_dim, q_heads * head_dim)
+    check(
+        lib().mote_hip_prompt_attention_f16(
+            q, k, v, out, query_offsets, key_offsets, sequences, query_tokens, key_tokens, max_keys, q_heads,
+            kv_heads, head_dim, sq, sk, sv, so, scale, int(causal), window, workspace, workspace_bytes, _s(stream)
+        ),
+        "launch prompt attention kernel",
+    )
+
+
+def kv_cache_append_q8(k, v, offsets, positions, block_table, cache, scales, sequences, tokens, kv_heads, head_dim,
+                       table_blocks, cache_blocks, stream, strides=None) -> None:
+    """Packed rows of k and v into the 8-bit cache, from `positions` on."""
+    sk, sv = strides or (kv_heads * head_dim, kv_heads * head_dim)
+    check(
+        lib().mote_hip_kv_cache_append_q8(
+            k, v, offsets, positions, block_table, cache, scales, sequences, tokens, kv_heads, head_dim, sk, sv,
+            table_blocks, cache_blocks, _s(stream)
+        ),
+        "launch cache append kernel",
+    )
+
+
+def kv_cache_read_q8_f16(cache, scales, offsets, positions, block_table, k, v, sequences, tokens, kv_heads, head_dim,
+                         table_blocks, cache_blocks, stream, strides=None) -> None:
+    """Tokens of the 8-bit cache, from `positions` on, to packed rows of k and v."""
+    sk, sv = strides or (kv_heads * head_dim, kv_heads * head_dim)
+    check(
+        lib().mote_hip_kv_cache_read_q8_f16(
+            cache, scales, offsets, positions, block_table, k, v, sequences, tokens, kv_heads, head_dim, sk, sv,
+            table_blocks, cache_blocks, _s(stream)
+        ),
+        "launch cache read kernel",
+    )
+
+
+def cache_attention_workspace(sequences, query_tokens, max_queries, max_context, q_heads, kv_heads, head_dim) -> int:
+    """Bytes of workspace that cache_attention_q8_f16 needs for these sizes."""
+    need = ctypes.c_size_t(0)
+    check(
+        lib().mote_hip_cache_attention_workspace(
+            sequences, query_tokens, max_queries, max_context, q_heads, kv_heads, head_dim, ctypes.byref(need)
+        ),
+        "size cache attention workspace",
+    )
+    return need.value
+
+
+def cache_attention_q8_f16(q, cache, scales, query_offsets, lengths, block_table, out, sequences, query_tokens,
+                           max_queries, max_context, q_heads, kv_heads, head_dim, table_blocks, cache_blocks, scale,
+                           workspace, workspace_bytes, stream, window=0, strides=None) -> None:
+    """Attention of each sequence's last tokens over the 8-bit cache.
+    `strides`: elements between the rows of q and out; `query_offsets` None:
+    one row a sequence."""
+    sq, so = strides or (q_heads * head_dim, q_heads * head_dim)
+    check(
+        lib().mote_hip_cache_attention_q8_f16(
+            q, cache, scales, query_offsets, lengths, block_table, out, sequences, query_tokens, max_queries,
+            max_context, q_heads, kv_heads, head_dim, sq, so, table_blocks, cache_blocks, scale, window, workspace,
+            workspace_bytes, _s(stream)
+        ),
+        "launch cache attention kernel",
+    )
+
+
 def variant_names() -> list[str]:
     h = lib()
     return [h.mote_q4_0_variant_name(i).decode() for i in range(h.mote_q4_0_variant_count())]
