@@ -63,12 +63,14 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t pair) {
     return r;
 }
 
-template <int DP>
+// DP: the padded head size.  DIRECT: rows and addresses on the 16-byte grid and
+// head_dim = DP, so tiles go from memory to LDS without passing registers.
+template <int DP, bool DIRECT>
 __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kernel(PromptArgs a) {
     constexpr int CH = DP / 8, KS = DP / 16, DT = DP / 32;
     constexpr int kLoads = kTileKeys * CH / 256;  // 16-byte chunks of a thread in each tile
-    __shared__ u32x4 key_tile[kTileKeys * CH];
-    __shared__ u32x4 value_tile[kTileKeys * CH];
+    constexpr int kTileBytes = kTileKeys * CH * 16;
+    __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two of [keys | values]
     __shared__ int taken_out;  // the last tile, from 1, with values that are not finite taken out
 
     const uint32_t head = blockIdx.y, part = blockIdx.z;
@@ -98,6 +100,55 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     const int pos = row + shift;
     const int wave_last = min(wave_row + 31, queries.n - 1) + shift;  // position of the wave's last row
 
+    const _Float16* const k = a.k + static_cast<uint64_t>(keys.at) * a.k_stride + static_cast<uint64_t>(kv_head) * a.head_dim;
+    const _Float16* const v = a.v + static_cast<uint64_t>(keys.at) * a.v_stride + static_cast<uint64_t>(kv_head) * a.head_dim;
+
+    // Chunk i of a thread lies at position 256 i + thread of a tile.
+    u32x4 next_k[DIRECT ? 1 : kLoads], next_v[DIRECT ? 1 : kLoads];
+    const auto load_tile = [&](int tile, uint8_t* to) {
+        const int j0 = begin + tile * kTileKeys;
+        if constexpr (DIRECT) {
+            const Buffer kb = buffer_at(k + static_cast<uint64_t>(j0) * a.k_stride);
+            const Buffer vb = buffer_at(v + static_cast<uint64_t>(j0) * a.v_stride);
+            const int last = keys.n - 1 - j0;  // rows past it repeat it; no row sees them
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
+                uint8_t* const dst = to + (256 * i + 64 * wave) * 16;
+                const uint32_t source = static_cast<uint32_t>(min(r, last));
+                load_lds16(kb, (source * static_cast<uint32_t>(a.k_stride) + 8 * (key_chunk<CH>(r, c) - r * CH)) * 2, 0, dst);
+                load_lds16(vb, (source * static_cast<uint32_t>(a.v_stride) + 8 * (value_chunk<CH>(r, c) - r * CH)) * 2, 0,
+                           dst + kTileBytes);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
+                next_k[i] = next_v[i] = u32x4{0, 0, 0, 0};
+                if (j0 + r < keys.n && 8u * c < a.head_dim) {
+                    next_k[i] = *reinterpret_cast<const u32x4_a2*>(k + static_cast<uint64_t>(j0 + r) * a.k_stride + 8 * c);
+                    next_v[i] = *reinterpret_cast<const u32x4_a2*>(v + static_cast<uint64_t>(j0 + r) * a.v_stride + 8 * c);
+                }
+            }
+        }
+    };
+    const auto store_tile = [&](uint8_t* to) {  // what load_tile left in registers
+        if constexpr (!DIRECT) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
+                *reinterpret_cast<u32x4*>(to + key_chunk<CH>(r, c) * 16) = next_k[i];
+                *reinterpret_cast<u32x4*>(to + kTileBytes + value_chunk<CH>(r, c) * 16) = next_v[i];
+            }
+        }
+    };
+
+    if (threadIdx.x == 0) taken_out = 0;
+    if (tile0 < tile1) {
+        load_tile(tile0, lds);
+        store_tile(lds);
+    }
+
     f16x8 qf[KS];
     {
         const _Float16* q = a.q + static_cast<uint64_t>(queries.at + min(row, queries.n - 1)) * a.q_stride +
@@ -111,22 +162,6 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         }
     }
 
-    const _Float16* const k = a.k + static_cast<uint64_t>(keys.at) * a.k_stride + static_cast<uint64_t>(kv_head) * a.head_dim;
-    const _Float16* const v = a.v + static_cast<uint64_t>(keys.at) * a.v_stride + static_cast<uint64_t>(kv_head) * a.head_dim;
-    u32x4 next_k[kLoads], next_v[kLoads];
-    const auto load_tile = [&](int tile) {
-        const int j0 = begin + tile * kTileKeys;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
-            next_k[i] = next_v[i] = u32x4{0, 0, 0, 0};
-            if (j0 + r < keys.n && 8u * c < a.head_dim) {
-                next_k[i] = *reinterpret_cast<const u32x4_a2*>(k + static_cast<uint64_t>(j0 + r) * a.k_stride + 8 * c);
-                next_v[i] = *reinterpret_cast<const u32x4_a2*>(v + static_cast<uint64_t>(j0 + r) * a.v_stride + 8 * c);
-            }
-        }
-    };
-
     f32x16 o[DT];
 #pragma unroll
     for (int i = 0; i < DT; ++i)
@@ -134,103 +169,115 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
     float m = -infinity(), l = 0.0f;
 
-    if (threadIdx.x == 0) taken_out = 0;
-    if (tile0 < tile1) load_tile(tile0);
-    for (int tile = tile0; tile < tile1; ++tile) {
-        __syncthreads();  // the last tile has been read
-        const int j0 = begin + tile * kTileKeys;
-        // Whether some row of the workgroup does not see all of the tile.
-        const bool partly = (a.causal && j0 + kTileKeys - 1 > row0 + shift) || (window && j0 <= last_row + shift - window);
+    // Lane addresses in a tile: of its key's chunks, of its piece of the values.
+    uint32_t key_at[KS], value_at[DT];
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
-            key_tile[key_chunk<CH>(r, c)] = next_k[i];
-            if (partly) {
-                // A value that is not finite must not reach the rows that do not
-                // see its key through a weight of zero.
-                bool bad = false;
+    for (int i = 0; i < KS; ++i) key_at[i] = key_chunk<CH>(n, 2 * i + h) * 16;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t fine = finite_of(next_v[i][w]);
-                    bad |= fine != next_v[i][w];
-                    next_v[i][w] = fine;
-                }
-                if (bad) taken_out = tile + 1;
-            }
-            value_tile[value_chunk<CH>(r, c)] = next_v[i];
-        }
-        __syncthreads();
-        if (tile + 1 < tile1) load_tile(tile + 1);
-        if (a.causal && (j0 > wave_last || (window && j0 + kTileKeys - 1 <= wave_row + shift - window))) continue;
+    for (int i = 0; i < DT; ++i) {
+        const int r = 4 * h + ((lane & 15) >> 2), piece = lane & 3;
+        const int chunk = 4 * i + 2 * ((lane >> 4) & 1) + (piece >> 1);
+        value_at[i] = kTileBytes + value_chunk<CH>(r, chunk) * 16 + 8 * (piece & 1);
+    }
 
-        f32x16 s[2];
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < KS; ++i)
-                s[t] = mfma32(__builtin_bit_cast(f16x8, key_tile[key_chunk<CH>(32 * t + n, 2 * i + h)]), qf[i], s[t]);
+    for (int tile = tile0; tile < tile1; ++tile) {
+        uint8_t* const here = lds + ((tile - tile0) & 1) * 2 * kTileBytes;
+        uint8_t* const there = lds + (1 - ((tile - tile0) & 1)) * 2 * kTileBytes;
+        if constexpr (DIRECT) {
+            wait_counts<vm_wait(0)>();
+            group_barrier();
+            order_fence();
+        } else {
+            __syncthreads();
         }
-        const bool masked = j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > wave_row + shift) ||
-                            (window && j0 <= wave_last - window);
-        if (masked) {
+        const int j0 = begin + tile * kTileKeys;
+        // Where some row of the workgroup does not see all of the tile, a value that
+        // is not finite must not reach it through a weight of zero: such values are
+        // taken out here and added below to the rows that see them.
+        if (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > row0 + shift) ||
+            (window && j0 <= last_row + shift - window)) {
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                u32x4* const at = reinterpret_cast<u32x4*>(here + kTileBytes) + threadIdx.x + 256 * i;
+                const u32x4 x = *at;
+                u32x4 fine;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) fine[w] = finite_of(x[w]);
+                if (fine[0] != x[0] || fine[1] != x[1] || fine[2] != x[2] || fine[3] != x[3]) {
+                    *at = fine;
+                    bad = true;
+                }
+            }
+            if (bad) taken_out = tile + 1;
+            __syncthreads();
+        }
+        if (tile + 1 < tile1) load_tile(tile + 1, there);
+        if (!(a.causal && (j0 > wave_last || (window && j0 + kTileKeys - 1 <= wave_row + shift - window)))) {
+            f32x16 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                    s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + key_at[i] + 32 * CH * 16 * t), qf[i], s[t]);
+            }
+            if (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > wave_row + shift) ||
+                (window && j0 <= wave_last - window)) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int j = j0 + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * h + (i & 3);
+                    const bool sees = j < keys.n && (!a.causal || j <= pos) && (!window || j > pos - window);
+                    s[i >> 4][i & 15] = sees ? s[i >> 4][i & 15] : -infinity();
+                }
+            }
+            float top = s[0][0];
+#pragma unroll
+            for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+            top = max_of(across_halves(top)) * a.exponent;
+            if (wave_any(top > m + kGrowth)) {
+                const float to = fmaxf(m, top);
+                const float w = m == to ? 1.0f : exp2_fast(m - to);  // also where both are -inf
+                m = to;
+                l *= w;
+#pragma unroll
+                for (int i = 0; i < DT; ++i) o[i] *= w;
+            }
+            const float base = m == -infinity() ? 0.0f : m - kShift;
+            f16x8 p[4];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
-                const int j = j0 + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * h + (i & 3);
-                const bool sees = j < keys.n && (!a.causal || j <= pos) && (!window || j > pos - window);
-                s[i >> 4][i & 15] = sees ? s[i >> 4][i & 15] : -infinity();
+                const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], a.exponent, -base));
+                l += e;
+                p[i >> 3][i & 7] = static_cast<_Float16>(e);
             }
-        }
-        float top = s[0][0];
+            // V^T: dimensions 32 i + n, keys 16 c + {4 h .. 4 h + 3, 8 + 4 h ..}.
 #pragma unroll
-        for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
-        top = max_of(across_halves(top)) * a.exponent;
-        if (wave_any(top > m + kGrowth)) {
-            const float to = fmaxf(m, top);
-            const float w = m == to ? 1.0f : exp2_fast(m - to);  // also where both are -inf
-            m = to;
-            l *= w;
+            for (int i = 0; i < DT; ++i)
 #pragma unroll
-            for (int i = 0; i < DT; ++i) o[i] *= w;
-        }
-        const float base = m == -infinity() ? 0.0f : m - kShift;
-        f16x8 p[4];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], a.exponent, -base));
-            l += e;
-            p[i >> 3][i & 7] = static_cast<_Float16>(e);
-        }
-
-        // V^T: dimensions 32 i + n, keys 16 c + {4 h .. 4 h + 3, 8 + 4 h ..}.
-        const auto values = [&](int i, int c) {
-            const int r = 16 * c + 4 * h + ((lane & 15) >> 2), piece = lane & 3;
-            const int chunk = 4 * i + 2 * ((lane >> 4) & 1) + (piece >> 1);
-            const uint8_t* tile_at = reinterpret_cast<const uint8_t*>(value_tile);
-            const u32x2 lo = read_transposed(tile_at + value_chunk<CH>(r, chunk) * 16 + 8 * (piece & 1));
-            const u32x2 hi = read_transposed(tile_at + value_chunk<CH>(r + 8, chunk) * 16 + 8 * (piece & 1));
-            return u32x4{lo.x, lo.y, hi.x, hi.y};
-        };
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[i] = mfma32(__builtin_bit_cast(f16x8, values(i, c)), p[c], o[i]);
-        if (taken_out == tile + 1) {  // the rows that see those values get them here
+                for (int c = 0; c < 4; ++c) {
+                    const uint8_t* at = here + value_at[i] + 16 * CH * 16 * c;
+                    const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * CH * 16);
+                    o[i] = mfma32(__builtin_bit_cast(f16x8, u32x4{lo.x, lo.y, hi.x, hi.y}), p[c], o[i]);
+                }
+            if (taken_out == tile + 1) {
 #pragma unroll 1
-            for (int j = j0; j < min(j0 + kTileKeys, keys.n); ++j) {
-                const bool sees = (!a.causal || j <= pos) && (!window || j > pos - window);
-                const _Float16* at = v + static_cast<uint64_t>(j) * a.v_stride;
+                for (int j = j0; j < min(j0 + kTileKeys, keys.n); ++j) {
+                    const bool sees = (!a.causal || j <= pos) && (!window || j > pos - window);
+                    const _Float16* at = v + static_cast<uint64_t>(j) * a.v_stride;
 #pragma unroll
-                for (int i = 0; i < DT; ++i)
+                    for (int i = 0; i < DT; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        const uint32_t d = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
-                        const float x = d < a.head_dim ? static_cast<float>(at[d]) : 0.0f;
-                        if (sees && !(fabsf(x) < infinity())) o[i][r] += x;
-                    }
+                        for (int r = 0; r < 16; ++r) {
+                            const uint32_t d = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
+                            const float x = d < a.head_dim ? static_cast<float>(at[d]) : 0.0f;
+                            if (sees && !(fabsf(x) < infinity())) o[i][r] += x;
+                        }
+                }
             }
         }
+        if (tile + 1 < tile1) store_tile(there);
     }
 
     l = sum_of(across_halves(l));
@@ -354,11 +401,18 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
     a.causal = static_cast<uint32_t>(causal);
     a.parts = p.parts;
     a.exponent = exponent;
-    const auto kernel = head_dim <= 64    ? prompt_attention_kernel<64>
-                        : head_dim <= 96  ? prompt_attention_kernel<96>
-                        : head_dim <= 128 ? prompt_attention_kernel<128>
-                        : head_dim <= 192 ? prompt_attention_kernel<192>
-                                          : prompt_attention_kernel<256>;
+    const bool direct = !off_grid(k, 16) && !off_grid(v, 16) && k_stride % 8 == 0 && v_stride % 8 == 0 &&
+                        k_stride < (uint64_t{1} << 24) && v_stride < (uint64_t{1} << 24);
+    const auto kernel = direct && head_dim == 64    ? prompt_attention_kernel<64, true>
+                        : direct && head_dim == 96  ? prompt_attention_kernel<96, true>
+                        : direct && head_dim == 128 ? prompt_attention_kernel<128, true>
+                        : direct && head_dim == 192 ? prompt_attention_kernel<192, true>
+                        : direct && head_dim == 256 ? prompt_attention_kernel<256, true>
+                        : head_dim <= 64            ? prompt_attention_kernel<64, false>
+                        : head_dim <= 96            ? prompt_attention_kernel<96, false>
+                        : head_dim <= 128           ? prompt_attention_kernel<128, false>
+                        : head_dim <= 192           ? prompt_attention_kernel<192, false>
+                                                    : prompt_attention_kernel<256, false>;
     const auto s = static_cast<hipStream_t>(stream);
     hipLaunchKernelGGL(kernel, dim3(p.tiles, a.heads, p.parts), dim3(256), 0, s, a);
     const int status = static_cast<int>(hipGetLastError());
