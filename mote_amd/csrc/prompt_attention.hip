@@ -73,9 +73,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two of [keys | values]
     __shared__ int taken_out;  // the last tile, from 1, with values that are not finite taken out
 
-    const uint32_t head = blockIdx.y, part = blockIdx.z;
-    const uint32_t kv_head = head / (a.heads / a.kv_heads);
-    const Unit u = locate(blockIdx.x, a.sequences, [&](uint32_t s) {
+    const uint32_t kv_head = blockIdx.x % a.kv_heads, part = blockIdx.z;
+    const uint32_t head = kv_head * (a.heads / a.kv_heads) + blockIdx.x / a.kv_heads;
+    const Unit u = locate(blockIdx.y, a.sequences, [&](uint32_t s) {
         return (static_cast<uint32_t>(span_of(a.query_offsets, s, a.tokens).n) + kTileRows - 1) / kTileRows;
     });
     if (!u.found) return;
@@ -105,20 +105,32 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 
     // Chunk i of a thread lies at position 256 i + thread of a tile.
     u32x4 next_k[DIRECT ? 1 : kLoads], next_v[DIRECT ? 1 : kLoads];
+    uint32_t source_k[kLoads], source_v[kLoads];  // DIRECT: their bytes from the tile's first row
+    const auto set_source = [&](int i, int last) {
+        const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
+        const uint32_t from = static_cast<uint32_t>(min(r, last));
+        source_k[i] = (from * static_cast<uint32_t>(a.k_stride) + 8 * (key_chunk<CH>(r, c) - r * CH)) * 2;
+        source_v[i] = (from * static_cast<uint32_t>(a.v_stride) + 8 * (value_chunk<CH>(r, c) - r * CH)) * 2;
+    };
+    if constexpr (DIRECT) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) set_source(i, kTileKeys - 1);
+    }
     const auto load_tile = [&](int tile, uint8_t* to) {
         const int j0 = begin + tile * kTileKeys;
         if constexpr (DIRECT) {
             const Buffer kb = buffer_at(k + static_cast<uint64_t>(j0) * a.k_stride);
             const Buffer vb = buffer_at(v + static_cast<uint64_t>(j0) * a.v_stride);
-            const int last = keys.n - 1 - j0;  // rows past it repeat it; no row sees them
+            const int last = keys.n - 1 - j0;
+            if (last < kTileKeys - 1) {  // rows past the last repeat it; no row sees them
+#pragma unroll
+                for (int i = 0; i < kLoads; ++i) set_source(i, last);
+            }
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
-                const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
                 uint8_t* const dst = to + (256 * i + 64 * wave) * 16;
-                const uint32_t source = static_cast<uint32_t>(min(r, last));
-                load_lds16(kb, (source * static_cast<uint32_t>(a.k_stride) + 8 * (key_chunk<CH>(r, c) - r * CH)) * 2, 0, dst);
-                load_lds16(vb, (source * static_cast<uint32_t>(a.v_stride) + 8 * (value_chunk<CH>(r, c) - r * CH)) * 2, 0,
-                           dst + kTileBytes);
+                load_lds16(kb, source_k[i], 0, dst);
+                load_lds16(vb, source_v[i], 0, dst + kTileBytes);
             }
         } else {
 #pragma unroll
@@ -162,11 +174,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         }
     }
 
+    const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     f32x16 o[DT];
 #pragma unroll
-    for (int i = 0; i < DT; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[i][r] = 0.0f;
+    for (int i = 0; i < DT; ++i) o[i] = zero;
     float m = -infinity(), l = 0.0f;
 
     // Lane addresses in a tile: of its key's chunks, of its piece of the values.
@@ -216,13 +227,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         if (!(a.causal && (j0 > wave_last || (window && j0 + kTileKeys - 1 <= wave_row + shift - window)))) {
             f32x16 s[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int i = 0; i < KS; ++i)
-                    s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + key_at[i] + 32 * CH * 16 * t), qf[i], s[t]);
-            }
+                    s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + key_at[i] + 32 * CH * 16 * t), qf[i],
+                                  i == 0 ? zero : s[t]);
             if (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > wave_row + shift) ||
                 (window && j0 <= wave_last - window)) {
 #pragma unroll
@@ -375,7 +384,7 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
     const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads);
     const uint64_t rows = query_tokens * q_heads, need = parts_bytes(rows, p.parts, head_dim);
     if (need > 0 && (!workspace || off_grid(workspace, 16) || workspace_bytes < need)) return kInvalid;
-    if (p.tiles > kMostGrid) return kInvalid;
+    if (p.tiles > 65535) return kInvalid;
     PromptArgs a{};
     a.q = static_cast<const _Float16*>(q);
     a.k = static_cast<const _Float16*>(k);
@@ -414,7 +423,7 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
                         : head_dim <= 192           ? prompt_attention_kernel<192, false>
                                                     : prompt_attention_kernel<256, false>;
     const auto s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(kernel, dim3(p.tiles, a.heads, p.parts), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3(a.heads, p.tiles, p.parts), dim3(256), 0, s, a);
     const int status = static_cast<int>(hipGetLastError());
     if (status != 0 || p.parts <= 1) return status;
     return join_parts(workspace, output, rows, p.parts, q_heads, head_dim, output_stride, s);
