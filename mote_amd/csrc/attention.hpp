@@ -37,6 +37,7 @@ typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
 constexpr float kGrowth = 6.0f;
 constexpr float kShift = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeastScale = 0x1p-64f;  // of values: times 127 far below binary16, and its inverse in range
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float infinity() { return __builtin_inff(); }
@@ -72,12 +73,29 @@ __device__ __forceinline__ Span span_of(const int32_t* offsets, uint32_t s, uint
     const int a = min(max(offsets[s], 0), most), b = min(max(offsets[s + 1], 0), most);
     return {a, max(b - a, 0)};
 }
+__device__ __forceinline__ Span span_at(Span mine, int lane) {  // the span that `lane` holds
+    return {__builtin_amdgcn_readlane(mine.at, lane), __builtin_amdgcn_readlane(mine.n, lane)};
+}
+
+// Sums of a wave's lanes up to and with each.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    const auto add = [&](auto shifted) { v += static_cast<uint32_t>(shifted); };
+    const auto at = [&]() { return static_cast<int>(v); };
+    add(__builtin_amdgcn_update_dpp(0, at(), 0x111, 0xF, 0xF, false));  // row_shr:1
+    add(__builtin_amdgcn_update_dpp(0, at(), 0x112, 0xF, 0xF, false));  // row_shr:2
+    add(__builtin_amdgcn_update_dpp(0, at(), 0x114, 0xF, 0xF, false));  // row_shr:4
+    add(__builtin_amdgcn_update_dpp(0, at(), 0x118, 0xF, 0xF, false));  // row_shr:8
+    add(__builtin_amdgcn_update_dpp(0, at(), 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
+    add(__builtin_amdgcn_update_dpp(0, at(), 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
+    return v;
+}
 
 // Unit `unit` of the units of all sequences in order, count(s) of sequence s:
-// its sequence and its number there.  Each wave looks it up by itself, 64
-// sequences at a time.
+// its sequence, its number there and the lane that counted it.  Each wave looks
+// it up by itself, 64 sequences at a time.
 struct Unit {
     uint32_t sequence, local, of;
+    int lane;
     bool found;
 };
 template <typename Count>
@@ -86,49 +104,94 @@ __device__ __forceinline__ Unit locate(uint32_t unit, uint32_t sequences, Count 
     uint32_t base = 0;
     for (uint32_t s0 = 0; s0 < sequences; s0 += 64) {
         const uint32_t n = s0 + lane < sequences ? count(s0 + lane) : 0;
-        uint32_t upto = n;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t other = __shfl_up(upto, d, 64);
-            if (lane >= static_cast<uint32_t>(d)) upto += other;
-        }
+        const uint32_t upto = wave_scan(n);
         const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > unit);
         if (past != 0) {
             const int at = __builtin_ctzll(past);
             const uint32_t mine = __builtin_amdgcn_readlane(n, at);
             const uint32_t before = base + __builtin_amdgcn_readlane(upto, at) - mine;
-            return {s0 + at, unit - before, mine, true};
+            return {s0 + at, unit - before, mine, at, true};
         }
         base += __builtin_amdgcn_readlane(upto, 63);
     }
-    return {0, 0, 0, false};
+    return {0, 0, 0, 0, false};
 }
 
 // Parts of the keys computed apart: part s of row r (token x heads + head) has
 // (m, l) in stats[s][r] and sum_j 2^(c s_j - m) v_j in sums[s][r][head_dim].
 // out = sum_s 2^(m_s - M) sums_s / sum_s 2^(m_s - M) l_s with M = max m_s; zeros
-// where no part saw a key.  A wave per row, four dimensions a lane.
+// where no part saw a key.  W waves a row, each its share of the parts (64 at
+// most, the statistics of one in a lane); a wave's lanes take four dimensions
+// each and as many parts at a time as find room.
+constexpr uint32_t kMostParts = 256;
+
+template <int W>
 __global__ __launch_bounds__(256) void parts_join_kernel(const float2* __restrict__ stats,
                                                          const float* __restrict__ sums, _Float16* output,
                                                          uint32_t rows, uint32_t parts, uint32_t heads,
-                                                         uint32_t head_dim, uint64_t out_stride) {
-    const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+                                                         uint32_t head_dim, uint32_t lanes, uint64_t out_stride) {
+    __shared__ __align__(16) float joined[W == 1 ? 1 : 4][W == 1 ? 4 : 256];
+    __shared__ float2 joined_stats[4];
+    __shared__ float weights[4][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t row = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     if (row >= rows) return;
-    float top = -infinity();
-    for (uint32_t s = 0; s < parts; ++s) top = fmaxf(top, stats[static_cast<uint64_t>(s) * rows + row].x);
-    const uint32_t d = lane * 4;
-    if (d >= head_dim) return;
+    const uint32_t share = (parts + W - 1) / W, first = W == 1 ? 0 : wave * share;
+    const uint32_t mine = first < parts ? min(share, parts - first) : 0;
+    float2 ml = {-infinity(), 0.0f};
+    if (lane < mine) ml = stats[static_cast<uint64_t>(first + lane) * rows + row];
+    float top = ml.x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    // A part that saw nothing has l = 0 and no sums; one with m = -inf and another l has NaN there.
+    const float weight = ml.y == 0.0f ? 0.0f : ml.x == -infinity() ? ml.y : exp2_fast(ml.x - top);
+    float l = wave_sum(weight * ml.y);
+    weights[wave][lane] = weight;  // read by this wave alone
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    float l = 0.0f;
-    for (uint32_t s = 0; s < parts; ++s) {
-        const float2 ml = stats[static_cast<uint64_t>(s) * rows + row];
-        if (ml.y == 0.0f) continue;  // saw nothing: its sums were not written
-        const float w = ml.x == -infinity() ? ml.y : exp2_fast(ml.x - top);  // the first only where ml.y is NaN
-        l = __builtin_fmaf(w, ml.y, l);
-        acc += w * *reinterpret_cast<const f32x4*>(sums + (static_cast<uint64_t>(s) * rows + row) * head_dim + d);
+    const uint32_t d = (lane & (lanes - 1)) * 4;
+    const uint32_t at_once = 64 / lanes;  // lanes: a power of two, four times it at least head_dim
+    const float* from = sums + (static_cast<uint64_t>(first) * rows + row) * head_dim + (d < head_dim ? d : 0);
+    const uint64_t step = static_cast<uint64_t>(rows) * head_dim;
+    for (uint32_t s0 = 0; s0 < mine; s0 += 4 * at_once) {
+        f32x4 x[4];
+        float w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {  // four loads in flight; past the last part: the first, weighing nothing
+            const uint32_t s = s0 + i * at_once + lane / lanes;
+            w[i] = s < mine ? weights[wave][s] : 0.0f;
+            x[i] = *reinterpret_cast<const f32x4*>(from + (s < mine ? s : 0) * step);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += w[i] != 0.0f ? w[i] * x[i][e] : 0.0f;
     }
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    acc *= inv;
+    for (uint32_t over = lanes; over < 64; over <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], static_cast<int>(over), 64);
+    if constexpr (W > 1) {
+        if (lane < lanes) *reinterpret_cast<f32x4*>(&joined[wave][4 * lane]) = acc;
+        if (lane == 0) joined_stats[wave] = float2{top, l};
+        __syncthreads();
+        if (wave != 0) return;
+        float all = -infinity();
+#pragma unroll
+        for (int w = 0; w < 4; ++w) all = fmaxf(all, joined_stats[w].x);
+        acc = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float2 of = joined_stats[w];
+            const float by = of.y == 0.0f ? 0.0f : of.x == -infinity() ? of.y : exp2_fast(of.x - all);
+            l = __builtin_fmaf(by, of.y, l);
+            acc += by * *reinterpret_cast<const f32x4*>(&joined[w][4 * (lane & (lanes - 1))]);
+        }
+    }
+    if (lane >= lanes || d >= head_dim) return;
+    acc *= l != 0.0f ? 1.0f / l : 0.0f;
     typedef _Float16 f16x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
     _Float16* out = output + (row / heads) * out_stride + (row % heads) * static_cast<uint64_t>(head_dim) + d;
     *reinterpret_cast<f16x4_a2*>(out) =
@@ -144,11 +207,15 @@ constexpr uint64_t parts_bytes(uint64_t rows, uint64_t parts, uint64_t head_dim)
 
 inline int join_parts(const void* workspace, void* output, uint64_t rows, uint32_t parts, uint64_t heads,
                       uint64_t head_dim, uint64_t out_stride, hipStream_t stream) {
-    hipLaunchKernelGGL(parts_join_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), 0, stream,
+    uint32_t lanes = 2;
+    while (lanes * 4 < head_dim) lanes *= 2;
+    const bool many = parts > 8;
+    const auto kernel = many ? parts_join_kernel<4> : parts_join_kernel<1>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(many ? rows : (rows + 3) / 4)), dim3(256), 0, stream,
                        static_cast<const float2*>(workspace),
                        reinterpret_cast<const float*>(static_cast<const char*>(workspace) + stats_bytes(rows, parts)),
                        static_cast<_Float16*>(output), static_cast<uint32_t>(rows), parts,
-                       static_cast<uint32_t>(heads), static_cast<uint32_t>(head_dim), out_stride);
+                       static_cast<uint32_t>(heads), static_cast<uint32_t>(head_dim), lanes, out_stride);
     return static_cast<int>(hipGetLastError());
 }
 

@@ -8,8 +8,8 @@
 // tile.  With keys as the instruction's rows, a lane ends with the scores of one
 // query row for tokens 4 g .. 4 g + 3 of each half block (g = lane / 16), which is
 // the operand that the second product wants of it: no score leaves its register.
-// Bytes become the exact binary16 integers u - 128; the planes' scales are
-// applied in 32 bits, to the scores and to each block's sums.
+// Bytes become the exact binary16 integers u - 128; the planes' scales join the
+// scores and the exponents in 32 bits.
 //
 // One pass is bound by the cache's bytes.  A workgroup takes `chunk` blocks of
 // one (sequence, rows, key head), its four waves every fourth block each, and
@@ -55,7 +55,7 @@ __device__ __forceinline__ f16x8 values_of(uint32_t lo, uint32_t hi) {
 
 // C: 32-dimension groups of the padded head; NT: 16-row tiles of a workgroup.
 template <int C, int NT>
-__global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttentionArgs a) {
+__global__ __launch_bounds__(256, NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) void cache_attention_kernel(CacheAttentionArgs a) {
     constexpr int kRows = 16 * NT;
     constexpr int kJoin = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // dimension groups joined at a time: 256 pieces of 8
     constexpr int kRowFloats = 32 * kJoin + 4;            // padded: rows start 4 banks apart
@@ -108,6 +108,7 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttentionArgs
         }
     }
 
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     f32x4 o[NT][2 * C];
     float m[NT], l[NT];
 #pragma unroll
@@ -115,54 +116,72 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttentionArgs
         m[t] = -infinity();
         l[t] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 2 * C; ++i) o[t][i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < 2 * C; ++i) o[t][i] = zero;
     }
 
     const int32_t* table = a.table + static_cast<uint64_t>(seq) * a.table_blocks;
     constexpr uint32_t kPlane = 1024 * C;
-    for (int b = b0 + static_cast<int>(wave); b < b1; b += 4) {
-        const int32_t block = table[b];
-        if (block < 0 || static_cast<uint32_t>(block) >= a.cache_blocks) continue;  // none there
-        const uint64_t at = static_cast<uint64_t>(block) * a.kv_heads + kv_head;
+    const uint32_t seen = a.window ? a.window : 0x80000000u;  // a row sees tokens (pos - seen, pos]
+    struct Block {
+        u32x4 k[C], v[C];
+        float key_scale, value_scale;
+        bool there;
+    };
+    // Block numbers are read one block ahead of the block itself.
+    const auto number = [&](int b) { return b < b1 ? table[b] : -1; };
+    const auto fetch = [&](int32_t block) {
+        Block f;
+        f.there = block >= 0 && static_cast<uint32_t>(block) < a.cache_blocks;
+        const uint64_t at = static_cast<uint64_t>(f.there ? block : 0) * a.kv_heads + kv_head;
         const uint8_t* planes = a.cache + at * (2 * kPlane) + lane * 16;
-        const float key_scale = a.scales[at * 2], value_scale = a.scales[at * 2 + 1];
-        u32x4 kb[C], vb[C];
 #pragma unroll
-        for (int c = 0; c < C; ++c) kb[c] = *reinterpret_cast<const u32x4*>(planes + 1024 * c);
+        for (int c = 0; c < C; ++c) f.k[c] = *reinterpret_cast<const u32x4*>(planes + 1024 * c);
 #pragma unroll
-        for (int c = 0; c < C; ++c) vb[c] = *reinterpret_cast<const u32x4*>(planes + kPlane + 1024 * c);
+        for (int c = 0; c < C; ++c) f.v[c] = *reinterpret_cast<const u32x4*>(planes + kPlane + 1024 * c);
+        f.key_scale = a.scales[at * 2];
+        f.value_scale = a.scales[at * 2 + 1];
+        return f;
+    };
+    int b = b0 + static_cast<int>(wave);
+    if (a.cache_blocks == 0) b = b1;  // nothing to point at
+    int32_t next = number(b + 4);
+    Block f{};
+    if (b < b1) f = fetch(number(b));
+    for (; b < b1; b += 4) {
+        Block ahead = f;
+        if (b + 4 < b1) ahead = fetch(next);
+        next = number(b + 8);
         f32x4 s[NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
         for (int c = 0; c < C; ++c) {
-            const f16x8 k0 = values_of(kb[c][0], kb[c][1]), k1 = values_of(kb[c][2], kb[c][3]);
+            const f16x8 k0 = values_of(f.k[c][0], f.k[c][1]), k1 = values_of(f.k[c][2], f.k[c][3]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                s[t][0] = mfma16(k0, qf[t][c], s[t][0]);
-                s[t][1] = mfma16(k1, qf[t][c], s[t][1]);
+                s[t][0] = mfma16(k0, qf[t][c], c == 0 ? zero : s[t][0]);
+                s[t][1] = mfma16(k1, qf[t][c], c == 0 ? zero : s[t][1]);
             }
         }
         const int j0 = b * static_cast<int>(kBlockTokens);
-        const bool edge = j0 + 31 > shift + first_token ||
+        const bool edge = !f.there || j0 + 31 > shift + first_token ||
                           (a.window && j0 <= last_seen - static_cast<int>(a.window));
-        const float factor = key_scale * a.exponent;
+        // The values' scale joins the exponent, 2^(x + log2 s), so that the products
+        // of all blocks add up in one sum; the weights' sum is divided by it again.
+        // A scale of zero counts as one too small to show.
+        const float factor = f.key_scale * a.exponent;
+        const float scale = f.value_scale < kLeastScale ? kLeastScale : f.value_scale;
+        const float more = __builtin_amdgcn_logf(scale);
+        const float less = scale == scale ? __builtin_amdgcn_rcpf(scale) : 1.0f;
         f16x8 p[NT];
-        float to_values[NT];  // 0 for a row that sees none of the block, whatever its scale
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            to_values[t] = value_scale;
             float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = s[t][i >> 2][i & 3] * factor;
+            for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(s[t][i >> 2][i & 3], factor, more);
             if (edge) {
-                if (j0 > pos[t] || (a.window && j0 + 31 <= pos[t] - static_cast<int>(a.window))) to_values[t] = 0.0f;
+                const int from_last = (f.there ? pos[t] : -static_cast<int>(kMostTokens)) - j0 - 4 * g;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = j0 + 16 * (i >> 2) + 4 * g + (i & 3);
-                    const bool sees = j <= pos[t] && (!a.window || j > pos[t] - static_cast<int>(a.window));
-                    x[i] = sees ? x[i] : -infinity();
-                }
+                for (int i = 0; i < 8; ++i)
+                    if (static_cast<uint32_t>(from_last - (16 * (i >> 2) + (i & 3))) >= seen) x[i] = -infinity();
             }
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             top = max_of(across_halves(max_of(across_rows16(top))));
@@ -175,23 +194,25 @@ __global__ __launch_bounds__(256) void cache_attention_kernel(CacheAttentionArgs
                 for (int i = 0; i < 2 * C; ++i) o[t][i] *= w;
             }
             const float base = m[t] == -infinity() ? 0.0f : m[t] - kShift;
+            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float e = exp2_fast(x[i] - base);
-                l[t] += e;
+                sum += e;
                 p[t][i] = static_cast<_Float16>(e);
             }
+            l[t] = __builtin_fmaf(sum, less, l[t]);
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const f16x8 v0 = values_of(vb[c][0], vb[c][1]), v1 = values_of(vb[c][2], vb[c][3]);
+            const f16x8 v0 = values_of(f.v[c][0], f.v[c][1]), v1 = values_of(f.v[c][2], f.v[c][3]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-                o[t][2 * c] += to_values[t] * mfma16(v0, p[t], zero);
-                o[t][2 * c + 1] += to_values[t] * mfma16(v1, p[t], zero);
+                o[t][2 * c] = mfma16(v0, p[t], o[t][2 * c]);
+                o[t][2 * c + 1] = mfma16(v1, p[t], o[t][2 * c + 1]);
             }
         }
+        f = ahead;
     }
 
     // The waves' sums join, a few dimension groups at a time.
@@ -262,8 +283,9 @@ CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_
     p.row_tiles = static_cast<uint32_t>((rows + p.tile_rows - 1) / p.tile_rows);
     const uint64_t blocks = (max_context + kBlockTokens - 1) / kBlockTokens + 1;
     const uint64_t groups = sequences * p.row_tiles * kv_heads;
-    // About 2048 workgroups (eight on a compute unit), none of fewer than 8 blocks (two a wave).
-    uint64_t parts = groups >= 2048 ? 1 : (2048 + groups - 1) / groups;
+    // About 1024 workgroups (four on a compute unit), none of fewer than 8 blocks (two a wave).
+    uint64_t parts = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;
+    if (parts > kMostParts) parts = kMostParts;
     uint64_t chunk = (blocks + parts - 1) / parts;
     if (chunk < 8) chunk = 8;
     parts = (blocks + chunk - 1) / chunk;

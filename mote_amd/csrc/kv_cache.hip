@@ -45,16 +45,18 @@ struct Piece {
 };
 
 __device__ __forceinline__ Piece piece_of(const CacheArgs& a, uint32_t unit, uint32_t head, uint32_t which) {
-    const auto begin = [&](uint32_t s) { return max(a.positions[s], 0); };
+    Span rows;  // first of the lane's sequence, then of the workgroup's
+    uint32_t first;
     const Unit u = locate(unit, a.sequences, [&](uint32_t s) {
-        const Span rows = span_of(a.offsets, s, a.tokens);
-        const uint32_t p = begin(s);
-        return rows.n > 0 ? (p + rows.n - 1) / kBlockTokens - p / kBlockTokens + 1 : 0u;
+        rows = span_of(a.offsets, s, a.tokens);
+        first = max(a.positions[s], 0);
+        return rows.n > 0 ? (first + rows.n - 1) / kBlockTokens - first / kBlockTokens + 1 : 0u;
     });
     Piece r{0, 0, 0, 0, false};
     if (!u.found) return r;
-    const Span rows = span_of(a.offsets, u.sequence, a.tokens);
-    const uint32_t first = begin(u.sequence), block = first / kBlockTokens + u.local;
+    rows = span_at(rows, u.lane);
+    first = __builtin_amdgcn_readlane(first, u.lane);
+    const uint32_t block = first / kBlockTokens + u.local;
     if (block >= a.table_blocks) return r;
     const int32_t id = a.table[static_cast<uint64_t>(u.sequence) * a.table_blocks + block];
     if (id < 0 || static_cast<uint32_t>(id) >= a.cache_blocks) return r;

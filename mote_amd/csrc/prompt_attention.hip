@@ -75,12 +75,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 
     const uint32_t kv_head = blockIdx.x % a.kv_heads, part = blockIdx.z;
     const uint32_t head = kv_head * (a.heads / a.kv_heads) + blockIdx.x / a.kv_heads;
+    Span queries, keys;  // first of the lane's sequence, then of the workgroup's
     const Unit u = locate(blockIdx.y, a.sequences, [&](uint32_t s) {
-        return (static_cast<uint32_t>(span_of(a.query_offsets, s, a.tokens).n) + kTileRows - 1) / kTileRows;
+        queries = span_of(a.query_offsets, s, a.tokens);
+        keys = span_of(a.key_offsets, s, a.keys);
+        return (static_cast<uint32_t>(queries.n) + kTileRows - 1) / kTileRows;
     });
     if (!u.found) return;
-    const Span queries = span_of(a.query_offsets, u.sequence, a.tokens);
-    const Span keys = span_of(a.key_offsets, u.sequence, a.keys);
+    queries = span_at(queries, u.lane);
+    keys = span_at(keys, u.lane);
     const int row0 = static_cast<int>((u.of - 1 - u.local) * kTileRows);  // the longest walks first
     const int shift = keys.n - queries.n;  // position of the first query
     const int last_row = min(row0 + static_cast<int>(kTileRows), queries.n) - 1;
@@ -98,6 +101,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     const int wave_row = row0 + 32 * wave;
     const int row = wave_row + n;
     const int pos = row + shift;
+    // The row sees keys (last_seen - seen, last_seen].
+    const int last_seen = a.causal ? pos : keys.n - 1;
+    const uint32_t seen = window ? a.window : 0x80000000u;
     const int wave_last = min(wave_row + 31, queries.n - 1) + shift;  // position of the wave's last row
 
     const _Float16* const k = a.k + static_cast<uint64_t>(keys.at) * a.k_stride + static_cast<uint64_t>(kv_head) * a.head_dim;
@@ -169,7 +175,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         for (int i = 0; i < KS; ++i) {
             const uint32_t d = 16 * i + 8 * h;
             u32x4 x = {0, 0, 0, 0};
-            if (d < a.head_dim) x = *reinterpret_cast<const u32x4_a2*>(q + d);
+            if (DIRECT || d < a.head_dim) x = *reinterpret_cast<const u32x4_a2*>(q + d);
             qf[i] = __builtin_bit_cast(f16x8, x);
         }
     }
@@ -234,11 +240,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
                                   i == 0 ? zero : s[t]);
             if (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > wave_row + shift) ||
                 (window && j0 <= wave_last - window)) {
+                const int from_last = last_seen - j0 - 4 * h;
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const int j = j0 + 32 * (i >> 4) + 8 * ((i & 15) >> 2) + 4 * h + (i & 3);
-                    const bool sees = j < keys.n && (!a.causal || j <= pos) && (!window || j > pos - window);
-                    s[i >> 4][i & 15] = sees ? s[i >> 4][i & 15] : -infinity();
+                    const int j = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3);
+                    if (static_cast<uint32_t>(from_last - j) >= seen) s[i >> 4][i & 15] = -infinity();
                 }
             }
             float top = s[0][0];
@@ -273,16 +279,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
             if (taken_out == tile + 1) {
 #pragma unroll 1
                 for (int j = j0; j < min(j0 + kTileKeys, keys.n); ++j) {
-                    const bool sees = (!a.causal || j <= pos) && (!window || j > pos - window);
-                    const _Float16* at = v + static_cast<uint64_t>(j) * a.v_stride;
+                    const bool sees = static_cast<uint32_t>(last_seen - j) < seen;
+                    const _Float16* at = v + static_cast<uint64_t>(j) * a.v_stride + 4 * h;
 #pragma unroll
-                    for (int i = 0; i < DT; ++i)
+                    for (int i = 0; i < DT; ++i) {
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) {
-                            const uint32_t d = 32 * i + 8 * (r >> 2) + 4 * h + (r & 3);
-                            const float x = d < a.head_dim ? static_cast<float>(at[d]) : 0.0f;
-                            if (sees && !(fabsf(x) < infinity())) o[i][r] += x;
+                        for (int r = 0; r < 16; r += 4) {
+                            const uint32_t d = 32 * i + 2 * r;
+                            if (!DIRECT && d >= a.head_dim) continue;
+                            const u32x2 four = *reinterpret_cast<const u32x2_a2*>(at + d);
+                            const float x[4] = {half_lo_to_float(four.x), half_hi_to_float(four.x),
+                                                half_lo_to_float(four.y), half_hi_to_float(four.y)};
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                o[i][r + e] += sees && !(fabsf(x[e]) < infinity()) ? x[e] : 0.0f;
                         }
+                        order_fence();  // rare, and not to be paid for in registers
+                    }
                 }
             }
         }
@@ -300,7 +313,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const uint32_t d = 32 * i + 2 * r + 4 * h;
-                if (d >= a.head_dim) continue;
+                if (!DIRECT && d >= a.head_dim) continue;
                 const f16x2 lo = {static_cast<_Float16>(o[i][r] * inv), static_cast<_Float16>(o[i][r + 1] * inv)};
                 const f16x2 hi = {static_cast<_Float16>(o[i][r + 2] * inv), static_cast<_Float16>(o[i][r + 3] * inv)};
                 *reinterpret_cast<u32x2_a2*>(out + d) =
@@ -318,7 +331,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
                 const uint32_t d = 32 * i + 2 * r + 4 * h;
-                if (d < a.head_dim) *reinterpret_cast<f32x4*>(out + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+                if (DIRECT || d < a.head_dim) *reinterpret_cast<f32x4*>(out + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
             }
     }
 }
