@@ -38,13 +38,13 @@ struct CacheArgs {
 
 // The part of a sequence's rows that lies in one block.
 struct Piece {
-    uint64_t plane;   // of scales and, times 32 P, of the cache
-    uint64_t row;     // packed row of its first token
-    uint32_t from, n; // its first slot and its tokens
+    uint64_t planes;   // its head's plane of keys; of scales and, times 32 P, of the cache
+    uint64_t row;      // packed row of its first token
+    uint32_t from, n;  // its first slot and its tokens
     bool found;
 };
 
-__device__ __forceinline__ Piece piece_of(const CacheArgs& a, uint32_t unit, uint32_t head, uint32_t which) {
+__device__ __forceinline__ Piece piece_of(const CacheArgs& a, uint32_t unit, uint32_t head) {
     Span rows;  // first of the lane's sequence, then of the workgroup's
     uint32_t first;
     const Unit u = locate(unit, a.sequences, [&](uint32_t s) {
@@ -62,7 +62,7 @@ __device__ __forceinline__ Piece piece_of(const CacheArgs& a, uint32_t unit, uin
     if (id < 0 || static_cast<uint32_t>(id) >= a.cache_blocks) return r;
     const uint32_t at = max(first, block * kBlockTokens);
     const uint32_t end = min(first + static_cast<uint32_t>(rows.n), (block + 1) * kBlockTokens);
-    return {(static_cast<uint64_t>(id) * a.heads + head) * 2 + which, static_cast<uint64_t>(rows.at) + (at - first),
+    return {(static_cast<uint64_t>(id) * a.heads + head) * 2, static_cast<uint64_t>(rows.at) + (at - first),
             at % kBlockTokens, end - at, true};
 }
 
@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t byte_of(uint32_t t, uint32_t d) {
         return (((c * 4 + ((d & 31) >> 3)) * 16 + (t & 15)) * 2 + (t >> 4)) * 8 + (d & 7);
 }
 
-constexpr uint32_t kMostPlane = 32 * 256;
+constexpr uint32_t kMostPlane = kBlockTokens * kMostHeadDim;
 
 __device__ __forceinline__ float scale_from_bits(uint32_t most) {
     // `most` is the largest magnitude's pattern: infinities and NaN order above every number.
@@ -88,66 +88,60 @@ __device__ __forceinline__ uint32_t to_byte(float x) {
     return static_cast<uint32_t>(static_cast<int>(fminf(fmaxf(__builtin_rintf(x), -127.0f), 127.0f)) + 128);
 }
 
-// One workgroup per (block piece, head, keys or values).
-template <bool VALUES>
-__device__ __forceinline__ void append_piece(const CacheArgs& a, uint32_t unit, uint32_t head) {
-    __shared__ __align__(16) uint8_t image[kMostPlane];
-    __shared__ uint32_t most_of[4];
-    const Piece p = piece_of(a, unit, head, VALUES);
-    if (!p.found) return;
-    const uint32_t plane_bytes = kBlockTokens * padded_dim(a.head_dim);
-    uint8_t* plane = a.cache + p.plane * plane_bytes;
-    const _Float16* rows = (VALUES ? a.v + p.row * a.v_stride : a.k + p.row * a.k_stride) +
-                           static_cast<uint64_t>(head) * a.head_dim;
-    const uint64_t stride = VALUES ? a.v_stride : a.k_stride;
-    const uint32_t t = threadIdx.x >> 3, sub = threadIdx.x & 7;  // eight threads a token
-    const uint32_t chunks = a.head_dim / 8;
-    constexpr int kChunks = 4;  // 16-byte chunks of a thread: 256 dimensions by eight threads
-    u32x4 x[kChunks];
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < kChunks; ++i) {
-        const uint32_t c = sub + 8 * i;
-        x[i] = u32x4{0, 0, 0, 0};
-        if (t < p.n && c < chunks) x[i] = *reinterpret_cast<const u32x4_a2*>(rows + t * stride + c * 8);
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            most = max(most, x[i][w] & 0x7FFFu);
-            most = max(most, (x[i][w] >> 16) & 0x7FFFu);
-        }
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) most = max(most, static_cast<uint32_t>(__shfl_xor(most, d, 64)));
-    if ((threadIdx.x & 63) == 0) most_of[threadIdx.x >> 6] = most;
-    float* const scale_at = a.scales + p.plane;
-    const float old = p.from != 0 ? *scale_at : 0.0f;
-    __syncthreads();
-    most = max(max(most_of[0], most_of[1]), max(most_of[2], most_of[3]));
+// The largest of a wave's lanes, in lane 63.
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+    const auto with = [&](int other) { v = max(v, static_cast<uint32_t>(other)); };
+    with(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x111, 0xF, 0xF, false));  // row_shr:1, 2, 4, 8
+    with(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x112, 0xF, 0xF, false));
+    with(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x114, 0xF, 0xF, false));
+    with(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x118, 0xF, 0xF, false));
+    with(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x142, 0xA, 0xF, false));  // row_bcast:15
+    with(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x143, 0xC, 0xF, false));  // row_bcast:31
+    return v;
+}
+
+constexpr int kChunks = 4;  // 16-byte chunks of a thread: 256 dimensions by the eight threads of a token
+
+// The plane's scale after the new tokens, whose largest magnitude's pattern is
+// `most`; `old` is 0 for a block begun anew.
+struct Scale {
+    float scale, inverse;  // inverse: 0 for an all-zero plane and for NaN (bytes 128)
+    float old;
+};
+__device__ __forceinline__ Scale new_scale(uint32_t most, float old) {
     const float need = scale_from_bits(most);
     const float scale = old != old || need != need ? __builtin_nanf("") : fmaxf(old, need);
-    const float inverse = scale > 0.0f ? 1.0f / scale : 0.0f;  // 0 for an all-zero plane and for NaN: bytes 128
-    const bool keep = p.from != 0 && scale == old;  // earlier bytes stay as they are
-    // The plane's image: earlier tokens' bytes, rounded again where the scale has grown.
-    if (p.from != 0) {
-        const float ratio = old * inverse;
+    return {scale, scale > 0.0f ? 1.0f / scale : 0.0f, old};
+}
+
+// Writes the new tokens' bytes, `x` being the thread's chunks of its token.
+template <bool VALUES>
+__device__ __forceinline__ void write_plane(const CacheArgs& a, const Piece& p, const u32x4 (&x)[kChunks],
+                                            const Scale& s, uint8_t* image) {
+    const uint32_t plane_bytes = kBlockTokens * padded_dim(a.head_dim);
+    uint8_t* const plane = a.cache + (p.planes + VALUES) * plane_bytes;
+    const uint32_t t = threadIdx.x >> 3, sub = threadIdx.x & 7, chunks = a.head_dim / 8;
+    const bool keep = p.from != 0 && s.scale == s.old;  // the earlier bytes stay as they are: only the new are written
+    // Otherwise the plane goes through its image in LDS: the earlier tokens' bytes
+    // rounded again to the larger scale, or zeros where none is written.
+    if (p.from != 0 && !keep) {
+        const float ratio = s.old * s.inverse;
         for (uint32_t i = threadIdx.x; i < plane_bytes / 16; i += 256) {
             u32x4 b = reinterpret_cast<const u32x4*>(plane)[i];
-            if (!keep) {
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    uint32_t r = 0;
+            for (int w = 0; w < 4; ++w) {
+                uint32_t r = 0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float u = static_cast<float>((b[w] >> (8 * j)) & 255u) - 128.0f;
-                        r |= to_byte(scale > 0.0f ? u * ratio : 0.0f) << (8 * j);
-                    }
-                    b[w] = r;
+                for (int j = 0; j < 4; ++j) {
+                    const float u = static_cast<float>((b[w] >> (8 * j)) & 255u) - 128.0f;
+                    r |= to_byte(s.scale > 0.0f ? u * ratio : 0.0f) << (8 * j);
                 }
+                b[w] = r;
             }
             reinterpret_cast<u32x4*>(image)[i] = b;
         }
         __syncthreads();
-    } else if (p.n < kBlockTokens || a.head_dim % 32 != 0) {
+    } else if (!keep && (p.n < kBlockTokens || a.head_dim % 32 != 0)) {
         for (uint32_t i = threadIdx.x; i < plane_bytes / 16; i += 256)
             reinterpret_cast<u32x4*>(image)[i] = u32x4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
         __syncthreads();
@@ -157,46 +151,141 @@ __device__ __forceinline__ void append_piece(const CacheArgs& a, uint32_t unit, 
         for (int i = 0; i < kChunks; ++i) {
             const uint32_t c = sub + 8 * i;
             if (c >= chunks) break;
+            uint32_t b[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float e = (j & 1) ? half_hi_to_float(x[i][j / 2]) : half_lo_to_float(x[i][j / 2]);
-                image[byte_of<VALUES>(p.from + t, c * 8 + j)] =
-                    static_cast<uint8_t>(scale > 0.0f ? to_byte(e * inverse) : 128u);
+                b[j] = s.scale > 0.0f ? to_byte(e * s.inverse) : 128u;
+            }
+            uint8_t* const to = (keep ? plane : image) + byte_of<VALUES>(p.from + t, c * 8);
+            if constexpr (VALUES) {  // dimensions are 16 bytes apart
+#pragma unroll
+                for (int j = 0; j < 8; ++j) to[16 * j] = static_cast<uint8_t>(b[j]);
+            } else {
+                *reinterpret_cast<u32x2*>(to) = u32x2{b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24,
+                                                      b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24};
             }
         }
     }
+    if (keep) return;
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < plane_bytes / 16; i += 256)
         reinterpret_cast<u32x4*>(plane)[i] = reinterpret_cast<const u32x4*>(image)[i];
-    if (threadIdx.x == 0 && !keep) *scale_at = scale;
+    if (threadIdx.x == 0) a.scales[p.planes + VALUES] = s.scale;
 }
 
+// One workgroup per (block piece, head): eight threads a token, which hold its
+// values of both planes while the planes' scales are found.
 __global__ __launch_bounds__(256) void append_kernel(CacheArgs a) {
-    if (blockIdx.z == 0)
-        append_piece<false>(a, blockIdx.x, blockIdx.y);
-    else
-        append_piece<true>(a, blockIdx.x, blockIdx.y);
+    __shared__ __align__(16) uint8_t image[2][kMostPlane];
+    __shared__ uint32_t most_of[2][4];
+    const uint32_t head = blockIdx.y;
+    const Piece p = piece_of(a, blockIdx.x, head);
+    if (!p.found) return;
+    const float old_k = p.from != 0 ? a.scales[p.planes] : 0.0f, old_v = p.from != 0 ? a.scales[p.planes + 1] : 0.0f;
+    const uint32_t t = threadIdx.x >> 3, sub = threadIdx.x & 7, chunks = a.head_dim / 8;
+    const _Float16* const k = a.k + (p.row + t) * a.k_stride + static_cast<uint64_t>(head) * a.head_dim;
+    const _Float16* const v = a.v + (p.row + t) * a.v_stride + static_cast<uint64_t>(head) * a.head_dim;
+    u32x4 xk[kChunks], xv[kChunks];
+    uint32_t most_k = 0, most_v = 0;
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i) {
+        const uint32_t c = sub + 8 * i;
+        xk[i] = xv[i] = u32x4{0, 0, 0, 0};
+        if (t < p.n && c < chunks) {
+            xk[i] = *reinterpret_cast<const u32x4_a2*>(k + c * 8);
+            xv[i] = *reinterpret_cast<const u32x4_a2*>(v + c * 8);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kChunks; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            most_k = max(most_k, max(xk[i][w] & 0x7FFFu, (xk[i][w] >> 16) & 0x7FFFu));
+            most_v = max(most_v, max(xv[i][w] & 0x7FFFu, (xv[i][w] >> 16) & 0x7FFFu));
+        }
+    most_k = wave_most(most_k);
+    most_v = wave_most(most_v);
+    if ((threadIdx.x & 63) == 63) {
+        most_of[0][threadIdx.x >> 6] = most_k;
+        most_of[1][threadIdx.x >> 6] = most_v;
+    }
+    __syncthreads();
+    const auto all = [&](const uint32_t (&of)[4]) { return max(max(of[0], of[1]), max(of[2], of[3])); };
+    write_plane<false>(a, p, xk, new_scale(all(most_of[0]), old_k), image[0]);
+    write_plane<true>(a, p, xv, new_scale(all(most_of[1]), old_v), image[1]);
 }
 
-template <bool VALUES>
-__device__ __forceinline__ void read_piece(const CacheArgs& a, uint32_t unit, uint32_t head) {
-    const uint32_t t = threadIdx.x >> 3, sub = threadIdx.x & 7;
-    const Piece p = piece_of(a, unit, head, VALUES);
-    if (!p.found || t >= p.n) return;
-    const uint32_t plane_bytes = kBlockTokens * padded_dim(a.head_dim);
-    const uint8_t* plane = a.cache + p.plane * plane_bytes;
-    const float scale = a.scales[p.plane];
-    const uint64_t stride = VALUES ? a.v_stride : a.k_stride;
-    _Float16* row = (VALUES ? a.v : a.k) + (p.row + t) * stride + static_cast<uint64_t>(head) * a.head_dim;
-    for (uint32_t d = sub; d < a.head_dim; d += 8)
-        row[d] = static_cast<_Float16>((static_cast<float>(plane[byte_of<VALUES>(p.from + t, d)]) - 128.0f) * scale);
+// (u - 128) s in binary16 for the bytes of a dword.
+__device__ __forceinline__ void values_of(uint32_t b, float scale, _Float16 (&out)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        out[j] = static_cast<_Float16>((static_cast<float>((b >> (8 * j)) & 255u) - 128.0f) * scale);
 }
 
+// One workgroup per (block piece, head): planes come in 16 bytes a thread, pass
+// through LDS as rows of tokens and leave in 16-byte chunks of a row.
 __global__ __launch_bounds__(256) void read_kernel(CacheArgs a) {
-    if (blockIdx.z == 0)
-        read_piece<false>(a, blockIdx.x, blockIdx.y);
-    else
-        read_piece<true>(a, blockIdx.x, blockIdx.y);
+    constexpr uint32_t kMostRow = kMostHeadDim + 8;  // rows 16 bytes past a multiple of the banks
+    __shared__ __align__(16) _Float16 rows[kBlockTokens * kMostRow];
+    const uint32_t head = blockIdx.y;
+    const Piece p = piece_of(a, blockIdx.x, head);
+    if (!p.found) return;
+    const uint32_t padded = padded_dim(a.head_dim), loads = kBlockTokens * padded / 16, row = padded + 8;
+    const float scale_k = a.scales[p.planes], scale_v = a.scales[p.planes + 1];
+    const u32x4* const plane = reinterpret_cast<const u32x4*>(a.cache + p.planes * (kBlockTokens * padded));
+    constexpr int kLoads = kMostPlane / 16 / 256;
+    u32x4 bk[kLoads], bv[kLoads];
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const uint32_t at = threadIdx.x + 256 * i;
+        bk[i] = bv[i] = u32x4{0, 0, 0, 0};
+        if (at < loads) {
+            bk[i] = plane[at];
+            bv[i] = plane[loads + at];
+        }
+    }
+    const uint32_t chunks = a.head_dim / 8;
+    const auto store = [&](_Float16* to, uint64_t stride) {
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < p.n * chunks; i += 256) {
+            const uint32_t t = i / chunks, c = i % chunks;
+            *reinterpret_cast<u32x4_a2*>(to + (p.row + t) * stride + static_cast<uint64_t>(head) * a.head_dim + 8 * c) =
+                *reinterpret_cast<const u32x4*>(rows + (p.from + t) * row + 8 * c);
+        }
+    };
+    // Position of 16 bytes: (c, g, m); keys: tokens m and 16 + m, dimensions 32 c + 8 g ..
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const uint32_t at = threadIdx.x + 256 * i, m = at & 15, d = (at >> 4) * 8;
+        if (at >= loads) break;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            _Float16 x[8];
+            values_of(bk[i][2 * half], scale_k, reinterpret_cast<_Float16(&)[4]>(x[0]));
+            values_of(bk[i][2 * half + 1], scale_k, reinterpret_cast<_Float16(&)[4]>(x[4]));
+            f16x8 y;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = x[j];
+            *reinterpret_cast<f16x8*>(rows + (m + 16 * half) * row + d) = y;
+        }
+    }
+    store(a.k, a.k_stride);
+    __syncthreads();
+    // values: dimensions 32 c + m and 16 more, tokens 4 g .. and 16 + 4 g ..
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+        const uint32_t at = threadIdx.x + 256 * i, m = at & 15, g = (at >> 4) & 3, c = at >> 6;
+        if (at >= loads) break;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            _Float16 x[4];
+            values_of(bv[i][w], scale_v, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) rows[(16 * (w & 1) + 4 * g + j) * row + 32 * c + 16 * (w >> 1) + m] = x[j];
+        }
+    }
+    store(a.v, a.v_stride);
 }
 
 // Checks shared by both directions; 1: go on.
@@ -242,8 +331,8 @@ MOTE_EXPORT int mote_hip_kv_cache_append_q8(const void* k, const void* v, const 
                       static_cast<uint32_t>(sequences), static_cast<uint32_t>(tokens), static_cast<uint32_t>(kv_heads),
                       static_cast<uint32_t>(head_dim), static_cast<uint32_t>(table_blocks),
                       static_cast<uint32_t>(cache_blocks)};
-    hipLaunchKernelGGL(append_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(kv_heads), 2),
-                       dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    hipLaunchKernelGGL(append_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(kv_heads)), dim3(256),
+                       0, static_cast<hipStream_t>(stream), a);
     return static_cast<int>(hipGetLastError());
 }
 
@@ -265,7 +354,7 @@ MOTE_EXPORT int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* sca
                       static_cast<_Float16*>(v), k_stride, v_stride, static_cast<uint32_t>(sequences),
                       static_cast<uint32_t>(tokens), static_cast<uint32_t>(kv_heads), static_cast<uint32_t>(head_dim),
                       static_cast<uint32_t>(table_blocks), static_cast<uint32_t>(cache_blocks)};
-    hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(kv_heads), 2), dim3(256),
+    hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(kv_heads)), dim3(256),
                        0, static_cast<hipStream_t>(stream), a);
     return static_cast<int>(hipGetLastError());
 }
