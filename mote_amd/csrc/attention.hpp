@@ -37,6 +37,7 @@ typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
 constexpr float kGrowth = 6.0f;
 constexpr float kShift = 8.0f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeastFactor = 0x1p-100f;  // of scores: a masked one stays -inf, others vanish
 constexpr float kLeastScale = 0x1p-64f;  // of values: times 127 far below binary16, and its inverse in range
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -116,6 +117,67 @@ __device__ __forceinline__ Unit locate(uint32_t unit, uint32_t sequences, Count 
     }
     return {0, 0, 0, 0, false};
 }
+
+// The running sums of the row that a lane of a 32-row wave holds half of: of the 32
+// D dimensions, 8 (r / 4) + 4 h + r % 4 of each 32 in o[.][r], h being the lane's half.
+template <int D>
+struct RowSums {
+    f32x16 o[D];
+    float m, l;  // l: of the lane's keys alone
+
+    static __device__ __forceinline__ f32x16 zero() {
+        return f32x16{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < D; ++i) o[i] = zero();
+        m = -infinity();
+        l = 0.0f;
+    }
+    // Makes room for exponents up to `top` (of the row, the same in both halves).
+    __device__ __forceinline__ void grow_to(float top) {
+        if (!wave_any(top > m + kGrowth)) return;
+        const float to = fmaxf(m, top);
+        const float w = m == to ? 1.0f : exp2_fast(m - to);  // also where both are -inf
+        m = to;
+        l *= w;
+#pragma unroll
+        for (int i = 0; i < D; ++i) o[i] *= w;
+    }
+    // What exponents are taken less of.
+    __device__ __forceinline__ float base() const { return m == -infinity() ? 0.0f : m - kShift; }
+    // The row's result to `out`, or with statistics its part to row `at` of them.
+    template <bool WHOLE>
+    __device__ __forceinline__ void write(_Float16* out, float2* stats, float* sums, uint64_t at, uint32_t head_dim,
+                                          int h) {
+        const float all = sum_of(across_halves(l));
+        if (stats == nullptr) {
+            const float inv = all != 0.0f ? 1.0f / all : 0.0f;
+#pragma unroll
+            for (int i = 0; i < D; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4) {
+                    const uint32_t d = 32 * i + 2 * r + 4 * h;
+                    if (!WHOLE && d >= head_dim) continue;
+                    const f16x2 lo = {static_cast<_Float16>(o[i][r] * inv), static_cast<_Float16>(o[i][r + 1] * inv)};
+                    const f16x2 hi = {static_cast<_Float16>(o[i][r + 2] * inv), static_cast<_Float16>(o[i][r + 3] * inv)};
+                    *reinterpret_cast<u32x2_a2*>(out + d) =
+                        u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+                }
+            return;
+        }
+        if (h == 0) stats[at] = float2{m == -infinity() ? m : m - kShift, all};
+        if (all == 0.0f) return;  // saw nothing: not read
+#pragma unroll
+        for (int i = 0; i < D; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const uint32_t d = 32 * i + 2 * r + 4 * h;
+                if (WHOLE || d < head_dim)
+                    *reinterpret_cast<f32x4*>(sums + at * head_dim + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
+            }
+    }
+};
 
 // Parts of the keys computed apart: part s of row r (token x heads + head) has
 // (m, l) in stats[s][r] and sum_j 2^(c s_j - m) v_j in sums[s][r][head_dim].

@@ -19,6 +19,7 @@
 #include <cstdint>
 
 #include "attention.hpp"
+#include "tile_ops.hpp"
 
 namespace mote::attention {
 namespace {
@@ -271,6 +272,197 @@ __global__ __launch_bounds__(256, NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) v
     }
 }
 
+// Many rows: 128 of a (sequence, key head), 32 a wave, over tiles of two blocks
+// that the four waves share through LDS as binary16, each byte converted once for
+// all rows.  As in the prompts' kernel S^T = K Q^T and O^T = V^T P^T run on the
+// 32 x 32 x 16 instruction; the planes' order makes both operands of a lane 16
+// consecutive bytes of LDS, key row 16 c + 8 b + 4 h + r of a tile being token
+// 16 b + 8 c + 4 h + r of the block.  CT: 32-dimension groups there is room for.
+constexpr uint32_t kTileRows = 128;
+
+template <int CT>
+__global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(CacheAttentionArgs a) {
+    constexpr int KS = 2 * CT;
+    constexpr int kPlaneHalfs = 1024 * CT;             // a block's plane as binary16
+    constexpr int kTileBytes = 2 * 2 * kPlaneHalfs;    // two blocks of keys, or of values
+    constexpr int kLoads = (2 * 64 * CT + 255) / 256;  // 16-byte chunks of a thread in two planes
+    __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two of [keys | values]
+
+    uint32_t id = blockIdx.x;
+    const uint32_t kv_head = id % a.kv_heads;
+    id /= a.kv_heads;
+    const uint32_t part = id % a.parts;
+    id /= a.parts;
+    const uint32_t row_tile = id % a.row_tiles, seq = id / a.row_tiles;
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int n = lane & 31, h = lane >> 5;
+    const uint32_t group = a.heads / a.kv_heads, groups = padded_dim(a.head_dim) / 32;
+    Span rows = {static_cast<int>(seq), 1};
+    if (a.offsets != nullptr) rows = span_of(a.offsets, seq, a.tokens);
+    const uint32_t row0 = row_tile * kTileRows, all_rows = static_cast<uint32_t>(rows.n) * group;
+    if (row0 >= all_rows) return;
+    const int length = min(max(a.lengths[seq], 0), static_cast<int>(a.table_blocks * kBlockTokens));
+    const int shift = length - rows.n;  // position of the first query
+    const int window = static_cast<int>(a.window);
+    const auto position = [&](uint32_t r) { return shift + static_cast<int>(min(r, all_rows - 1) / group); };
+    const int last_of_tile = position(row0 + kTileRows - 1);
+    const uint32_t wave_row = row0 + 32 * wave, r = wave_row + n;
+    const int wave_first = position(wave_row), wave_last = position(wave_row + 31), pos = position(r);
+
+    // Tiles of 64 tokens that any row sees, and this part's.
+    const int end = max(last_of_tile + 1, 0);
+    const int begin = window ? min(max(position(row0) - window + 1, 0), end) & ~63 : 0;
+    const int tiles = (end - begin + 63) / 64;
+    const int per_part = (tiles + static_cast<int>(a.parts) - 1) / static_cast<int>(a.parts);
+    const int tile0 = static_cast<int>(part) * per_part;
+    const int tile1 = a.cache_blocks == 0 ? tile0 : min(tiles, tile0 + per_part);
+
+    const int32_t* const table = a.table + static_cast<uint64_t>(seq) * a.table_blocks;
+    const int last_block = (end + 31) / 32 - 1;
+    struct Scales {
+        float key[2], value[2];
+        bool there[2];
+    };
+    u32x4 raw_k[kLoads], raw_v[kLoads];
+    const auto load_tile = [&](int tile) {
+        Scales f;
+        uint64_t at[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            const int b = begin / 32 + 2 * tile + t;
+            const int32_t block = table[min(b, last_block)];
+            f.there[t] = b <= last_block && block >= 0 && static_cast<uint32_t>(block) < a.cache_blocks;
+            at[t] = static_cast<uint64_t>(f.there[t] ? block : 0) * a.kv_heads + kv_head;
+            f.key[t] = a.scales[at[t] * 2];
+            f.value[t] = a.scales[at[t] * 2 + 1];
+        }
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int wave_at = 4 * i + wave, t = wave_at / CT;  // 64 chunks a wave: dimension group wave_at % CT of block t
+            const uint32_t c = static_cast<uint32_t>(wave_at % CT);
+            raw_k[i] = raw_v[i] = u32x4{0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+            if (t < 2 && c < groups) {
+                const uint8_t* const from = a.cache + (t ? at[1] : at[0]) * (2048 * groups) + 1024 * c + lane * 16;
+                raw_k[i] = *reinterpret_cast<const u32x4*>(from);
+                raw_v[i] = *reinterpret_cast<const u32x4*>(from + 1024 * groups);
+            }
+        }
+        return f;
+    };
+    const auto store_tile = [&](uint8_t* to) {
+        const int g = lane >> 4, at = lane & 15;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int wave_at = 4 * i + wave, t = wave_at / CT, c = wave_at % CT;
+            if (t >= 2) break;
+            // keys: tokens `at` and 16 + at, dimensions 32 c + 8 g ..
+            uint8_t* const key = to + ((t * KS + 2 * c + (g >> 1)) * 64 + 32 * (g & 1) + 16 * (at >> 3) + (at & 7)) * 16;
+            *reinterpret_cast<f16x8*>(key) = values_of(raw_k[i][0], raw_k[i][1]);
+            *reinterpret_cast<f16x8*>(key + 128) = values_of(raw_k[i][2], raw_k[i][3]);
+            // values: dimensions 32 c + at and 16 more, tokens 4 g .. and 16 + 4 g ..
+            uint8_t* const value = to + kTileBytes + ((t * KS + 2 * c + (g >> 1)) * 64 + 32 * (g & 1) + at) * 16;
+            *reinterpret_cast<f16x8*>(value) = values_of(raw_v[i][0], raw_v[i][1]);
+            *reinterpret_cast<f16x8*>(value + 256) = values_of(raw_v[i][2], raw_v[i][3]);
+        }
+    };
+
+    Scales scales{};
+    if (tile0 < tile1) scales = load_tile(tile0);
+    f16x8 qf[KS];
+    const uint32_t valid = min(r, all_rows - 1), token = valid / group, head = kv_head * group + valid % group;
+    {
+        const _Float16* const q = a.q + static_cast<uint64_t>(rows.at + token) * a.q_stride +
+                                  static_cast<uint64_t>(head) * a.head_dim;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const uint32_t d = 16 * i + 8 * h;
+            u32x4 x = {0, 0, 0, 0};
+            if (d < a.head_dim) x = *reinterpret_cast<const u32x4_a2*>(q + d);
+            qf[i] = __builtin_bit_cast(f16x8, x);
+        }
+    }
+    if (tile0 < tile1) store_tile(lds);
+    RowSums<CT> sums;
+    sums.clear();
+    const uint32_t seen = window ? a.window : 0x80000000u;  // the row sees tokens (pos - seen, pos]
+
+    for (int tile = tile0; tile < tile1; ++tile) {
+        uint8_t* const here = lds + ((tile - tile0) & 1) * 2 * kTileBytes;
+        uint8_t* const there = lds + (1 - ((tile - tile0) & 1)) * 2 * kTileBytes;
+        __syncthreads();
+        const Scales now = scales;
+        if (tile + 1 < tile1) scales = load_tile(tile + 1);
+        const int j0 = begin + tile * 64;
+        if (j0 <= wave_last && !(window && j0 + 63 <= wave_first - window)) {
+            f32x16 s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                    s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + ((t * KS + i) * 64 + lane) * 16), qf[i],
+                                  i == 0 ? RowSums<CT>::zero() : s[t]);
+            // Exponents are s factor + more: see the few rows' kernel for the values' scale.
+            float factor[2], more[2], less[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float by = now.key[t] * a.exponent, scale = now.value[t] < kLeastScale ? kLeastScale : now.value[t];
+                factor[t] = by < kLeastFactor ? kLeastFactor : by;
+                more[t] = __builtin_amdgcn_logf(scale);
+                less[t] = scale == scale ? __builtin_amdgcn_rcpf(scale) : 1.0f;
+                if (!now.there[t] || j0 + 32 * t + 31 > wave_first || (window && j0 + 32 * t <= wave_last - window)) {
+                    const int from_last = (now.there[t] ? pos : -static_cast<int>(kMostTokens)) - j0 - 32 * t - 4 * h;
+                    bool any = false;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int j = 16 * ((i >> 2) & 1) + 8 * (i >> 3) + (i & 3);
+                        const bool sees = static_cast<uint32_t>(from_last - j) < seen;
+                        any |= sees;
+                        s[t][i] = sees ? s[t][i] : -infinity();
+                    }
+                    if (!any) factor[t] = 1.0f, more[t] = 0.0f;  // whatever the block's scales are
+                }
+            }
+            float top[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                top[t] = s[t][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top[t] = fmaxf(top[t], s[t][i]);
+                top[t] = __builtin_fmaf(top[t], factor[t], more[t]);
+            }
+            sums.grow_to(max_of(across_halves(fmaxf(top[0], top[1]))));
+            const float base = sums.base();
+            f16x8 p[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const float add = more[t] - base;
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = exp2_fast(__builtin_fmaf(s[t][i], factor[t], add));
+                    sum += e;
+                    p[2 * t + (i >> 3)][i & 7] = static_cast<_Float16>(e);
+                }
+                sums.l = __builtin_fmaf(sum, less[t], sums.l);
+            }
+#pragma unroll
+            for (int i = 0; i < CT; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    sums.o[i] = mfma32(*reinterpret_cast<const f16x8*>(here + kTileBytes +
+                                                                       (((c >> 1) * KS + 2 * i + (c & 1)) * 64 + lane) * 16),
+                                       p[c], sums.o[i]);
+        }
+        if (tile + 1 < tile1) store_tile(there);
+    }
+    if (r >= all_rows) return;  // both halves of the row
+    const uint64_t out_row = static_cast<uint64_t>(rows.at + token);
+    sums.template write<false>(a.output + out_row * a.out_stride + static_cast<uint64_t>(head) * a.head_dim, a.stats,
+                               a.sums, static_cast<uint64_t>(part) * a.tokens * a.heads + out_row * a.heads + head,
+                               a.head_dim, h);
+}
+
 struct CachePlan {
     uint32_t row_tiles, tile_rows, chunk, parts;
 };
@@ -279,10 +471,18 @@ CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_
                                uint64_t kv_heads, uint64_t head_dim) {
     const uint64_t rows = max_queries * (heads / kv_heads);
     CachePlan p{};
-    p.tile_rows = rows <= 16 ? 16 : rows <= 32 || head_dim > 128 ? 32 : 64;
+    p.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 && head_dim <= 128 ? 64 : kTileRows;
     p.row_tiles = static_cast<uint32_t>((rows + p.tile_rows - 1) / p.tile_rows);
     const uint64_t blocks = (max_context + kBlockTokens - 1) / kBlockTokens + 1;
     const uint64_t groups = sequences * p.row_tiles * kv_heads;
+    if (p.tile_rows == kTileRows) {
+        // Two workgroups a compute unit, none of fewer than four tiles.
+        uint64_t parts = groups >= 256 ? 1 : 512 / groups;
+        const uint64_t most = (max_context + 255) / 256;
+        if (parts > most) parts = most;
+        p.parts = static_cast<uint32_t>(parts > 1 ? parts : 1);
+        return p;
+    }
     // About 1024 workgroups (four on a compute unit), none of fewer than 8 blocks (two a wave).
     uint64_t parts = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;
     if (parts > kMostParts) parts = kMostParts;
@@ -391,7 +591,14 @@ MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache
     a.parts = p.parts;
     a.exponent = exponent;
     const uint32_t c = padded_dim(a.head_dim) / 32;
-    const auto kernel = p.tile_rows == 16 ? kernel_of<1>(c) : p.tile_rows == 32 ? kernel_of<2>(c) : kernel_of<4>(c);
+    const auto kernel = p.tile_rows == 16   ? kernel_of<1>(c)
+                        : p.tile_rows == 32 ? kernel_of<2>(c)
+                        : p.tile_rows == 64 ? kernel_of<4>(c)
+                        : c <= 2            ? cache_tiles_kernel<2>
+                        : c == 3            ? cache_tiles_kernel<3>
+                        : c == 4            ? cache_tiles_kernel<4>
+                        : c <= 6            ? cache_tiles_kernel<6>
+                                            : cache_tiles_kernel<8>;
     const auto s = static_cast<hipStream_t>(stream);
     const uint64_t groups = sequences * p.row_tiles * kv_heads * p.parts;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, a);

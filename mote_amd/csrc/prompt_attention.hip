@@ -180,11 +180,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         }
     }
 
-    const f32x16 zero = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    f32x16 o[DT];
-#pragma unroll
-    for (int i = 0; i < DT; ++i) o[i] = zero;
-    float m = -infinity(), l = 0.0f;
+    RowSums<DT> sums;
+    sums.clear();
 
     // Lane addresses in a tile: of its key's chunks, of its piece of the values.
     uint32_t key_at[KS], value_at[DT];
@@ -237,7 +234,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
                 for (int i = 0; i < KS; ++i)
                     s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + key_at[i] + 32 * CH * 16 * t), qf[i],
-                                  i == 0 ? zero : s[t]);
+                                  i == 0 ? RowSums<DT>::zero() : s[t]);
             if (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > wave_row + shift) ||
                 (window && j0 <= wave_last - window)) {
                 const int from_last = last_seen - j0 - 4 * h;
@@ -250,21 +247,13 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
             float top = s[0][0];
 #pragma unroll
             for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
-            top = max_of(across_halves(top)) * a.exponent;
-            if (wave_any(top > m + kGrowth)) {
-                const float to = fmaxf(m, top);
-                const float w = m == to ? 1.0f : exp2_fast(m - to);  // also where both are -inf
-                m = to;
-                l *= w;
-#pragma unroll
-                for (int i = 0; i < DT; ++i) o[i] *= w;
-            }
-            const float base = m == -infinity() ? 0.0f : m - kShift;
+            sums.grow_to(max_of(across_halves(top)) * a.exponent);
+            const float base = sums.base();
             f16x8 p[4];
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
                 const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], a.exponent, -base));
-                l += e;
+                sums.l += e;
                 p[i >> 3][i & 7] = static_cast<_Float16>(e);
             }
             // V^T: dimensions 32 i + n, keys 16 c + {4 h .. 4 h + 3, 8 + 4 h ..}.
@@ -274,7 +263,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
                 for (int c = 0; c < 4; ++c) {
                     const uint8_t* at = here + value_at[i] + 16 * CH * 16 * c;
                     const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * CH * 16);
-                    o[i] = mfma32(__builtin_bit_cast(f16x8, u32x4{lo.x, lo.y, hi.x, hi.y}), p[c], o[i]);
+                    sums.o[i] = mfma32(__builtin_bit_cast(f16x8, u32x4{lo.x, lo.y, hi.x, hi.y}), p[c], sums.o[i]);
                 }
             if (taken_out == tile + 1) {
 #pragma unroll 1
@@ -292,7 +281,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
                                                 half_lo_to_float(four.y), half_hi_to_float(four.y)};
 #pragma unroll
                             for (int e = 0; e < 4; ++e)
-                                o[i][r + e] += sees && !(fabsf(x[e]) < infinity()) ? x[e] : 0.0f;
+                                sums.o[i][r + e] += sees && !(fabsf(x[e]) < infinity()) ? x[e] : 0.0f;
                         }
                         order_fence();  // rare, and not to be paid for in registers
                     }
@@ -302,38 +291,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         if (tile + 1 < tile1) store_tile(there);
     }
 
-    l = sum_of(across_halves(l));
     if (row >= queries.n) return;
     const uint64_t token = static_cast<uint64_t>(queries.at + row);
-    if (a.stats == nullptr) {
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-        _Float16* out = a.output + token * a.out_stride + static_cast<uint64_t>(head) * a.head_dim;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const uint32_t d = 32 * i + 2 * r + 4 * h;
-                if (!DIRECT && d >= a.head_dim) continue;
-                const f16x2 lo = {static_cast<_Float16>(o[i][r] * inv), static_cast<_Float16>(o[i][r + 1] * inv)};
-                const f16x2 hi = {static_cast<_Float16>(o[i][r + 2] * inv), static_cast<_Float16>(o[i][r + 3] * inv)};
-                *reinterpret_cast<u32x2_a2*>(out + d) =
-                    u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
-            }
-    } else {
-        const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
-        const uint64_t at = part * rows + token * a.heads + head;
-        const float base = m == -infinity() ? m : m - kShift;
-        if (h == 0) a.stats[at] = float2{base, l};
-        if (l == 0.0f) return;  // saw nothing: not read
-        float* out = a.sums + at * a.head_dim;
-#pragma unroll
-        for (int i = 0; i < DT; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                const uint32_t d = 32 * i + 2 * r + 4 * h;
-                if (DIRECT || d < a.head_dim) *reinterpret_cast<f32x4*>(out + d) = f32x4{o[i][r], o[i][r + 1], o[i][r + 2], o[i][r + 3]};
-            }
-    }
+    sums.template write<DIRECT>(a.output + token * a.out_stride + static_cast<uint64_t>(head) * a.head_dim, a.stats,
+                                a.sums, part * (static_cast<uint64_t>(a.tokens) * a.heads) + token * a.heads + head,
+                                a.head_dim, h);
 }
 
 struct PromptPlan {

@@ -270,7 +270,7 @@ def test_one_token(stream, length):
 
 
 @pytest.mark.parametrize("d", [8, 32, 40, 64, 72, 96, 104, 128, 136, 160, 192, 200, 224, 256])
-@pytest.mark.parametrize("n", [1, 5, 13])
+@pytest.mark.parametrize("n", [1, 5, 13, 40])
 def test_head_sizes(stream, d, n):
     check(stream, d, [n, n], [70, 300], 8, 2, d)
 
