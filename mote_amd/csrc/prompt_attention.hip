@@ -46,14 +46,22 @@ __device__ __forceinline__ u32x2 read_transposed(const uint8_t* at) {
 }
 
 // Position of 16-byte chunk c of row r in a tile of CH chunks a row: chunks of a
-// row are exchanged within aligned groups of a power of two, so that rows read
-// together lie in different banks.
+// row are exchanged within aligned groups of G, a power of two, so that what is read
+// together lies in different banks, of which 16 chunks fill all: no conflict is
+// counted in the 8192-token case, where c ^ r for keys and c ^ 2 r for values made
+// conflicts a third of the LDS cycles.  16 / G neighbouring rows differ by their
+// place alone.
 template <int CH>
-__device__ __forceinline__ constexpr int group_of() { return (CH & -CH) > 16 ? 16 : (CH & -CH); }
-template <int CH>
-__device__ __forceinline__ int key_chunk(int r, int c) { return r * CH + (c ^ (r & (group_of<CH>() - 1))); }
-template <int CH>
-__device__ __forceinline__ int value_chunk(int r, int c) { return r * CH + (c ^ ((2 * r) & (group_of<CH>() - 1))); }
+struct Swizzle {
+    static constexpr int G = (CH & -CH) > 16 ? 16 : (CH & -CH);
+    // Keys: chunks c and c + 1 of any 8 neighbouring rows, and c of any 16.
+    static __device__ __forceinline__ int key(int r, int c) {
+        const int q = r / (16 / G);
+        return r * CH + (c ^ ((q * 2) % G | (q / (G / 2)) % 2));
+    }
+    // Values: four chunks of any 4 neighbouring rows.
+    static __device__ __forceinline__ int value(int r, int c) { return r * CH + (c ^ (4 * (r / (16 / G)) % G)); }
+};
 
 // The pair with halves that are not finite replaced by zero.
 __device__ __forceinline__ uint32_t finite_of(uint32_t pair) {
@@ -115,8 +123,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     const auto set_source = [&](int i, int last) {
         const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
         const uint32_t from = static_cast<uint32_t>(min(r, last));
-        source_k[i] = (from * static_cast<uint32_t>(a.k_stride) + 8 * (key_chunk<CH>(r, c) - r * CH)) * 2;
-        source_v[i] = (from * static_cast<uint32_t>(a.v_stride) + 8 * (value_chunk<CH>(r, c) - r * CH)) * 2;
+        source_k[i] = (from * static_cast<uint32_t>(a.k_stride) + 8 * (Swizzle<CH>::key(r, c) - r * CH)) * 2;
+        source_v[i] = (from * static_cast<uint32_t>(a.v_stride) + 8 * (Swizzle<CH>::value(r, c) - r * CH)) * 2;
     };
     if constexpr (DIRECT) {
 #pragma unroll
@@ -155,8 +163,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 const int at = static_cast<int>(threadIdx.x) + 256 * i, r = at / CH, c = at % CH;
-                *reinterpret_cast<u32x4*>(to + key_chunk<CH>(r, c) * 16) = next_k[i];
-                *reinterpret_cast<u32x4*>(to + kTileBytes + value_chunk<CH>(r, c) * 16) = next_v[i];
+                *reinterpret_cast<u32x4*>(to + Swizzle<CH>::key(r, c) * 16) = next_k[i];
+                *reinterpret_cast<u32x4*>(to + kTileBytes + Swizzle<CH>::value(r, c) * 16) = next_v[i];
             }
         }
     };
@@ -186,12 +194,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     // Lane addresses in a tile: of its key's chunks, of its piece of the values.
     uint32_t key_at[KS], value_at[DT];
 #pragma unroll
-    for (int i = 0; i < KS; ++i) key_at[i] = key_chunk<CH>(n, 2 * i + h) * 16;
+    for (int i = 0; i < KS; ++i) key_at[i] = Swizzle<CH>::key(n, 2 * i + h) * 16;
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
         const int r = 4 * h + ((lane & 15) >> 2), piece = lane & 3;
         const int chunk = 4 * i + 2 * ((lane >> 4) & 1) + (piece >> 1);
-        value_at[i] = kTileBytes + value_chunk<CH>(r, chunk) * 16 + 8 * (piece & 1);
+        value_at[i] = kTileBytes + Swizzle<CH>::value(r, chunk) * 16 + 8 * (piece & 1);
     }
 
     for (int tile = tile0; tile < tile1; ++tile) {
