@@ -144,6 +144,14 @@ struct RowSums {
 #pragma unroll
         for (int i = 0; i < D; ++i) o[i] *= w;
     }
+    __device__ __forceinline__ bool finite() const {
+        float all = 0.0f;  // any that is not makes NaN
+#pragma unroll
+        for (int i = 0; i < D; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) all = __builtin_fmaf(o[i][r], 0.0f, all);
+        return all == 0.0f;
+    }
     // What exponents are taken less of.
     __device__ __forceinline__ float base() const { return m == -infinity() ? 0.0f : m - kShift; }
     // The row's result to `out`, or with statistics its part to row `at` of them.

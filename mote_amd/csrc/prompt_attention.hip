@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "attention.hpp"
 #include "tile_ops.hpp"
@@ -79,12 +80,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
     constexpr int kLoads = kTileKeys * CH / 256;  // 16-byte chunks of a thread in each tile
     constexpr int kTileBytes = kTileKeys * CH * 16;
     __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two of [keys | values]
-    __shared__ int taken_out;  // the last tile, from 1, with values that are not finite taken out
+    __shared__ int not_finite;  // a wave's sums are not
+    __shared__ int taken_out;   // the last tile, from 1, with values that are not finite taken out
 
-    const uint32_t kv_head = blockIdx.x % a.kv_heads, part = blockIdx.z;
-    const uint32_t head = kv_head * (a.heads / a.kv_heads) + blockIdx.x / a.kv_heads;
+    // Key heads first, so that with eight of them each XCD's L2 keeps one; then the
+    // query heads that share them; then the tiles.
+    const uint32_t kv_head = blockIdx.x, part = a.parts == 1 ? 0 : blockIdx.z % a.parts;
+    const uint32_t head = kv_head * gridDim.y + blockIdx.y;
     Span queries, keys;  // first of the lane's sequence, then of the workgroup's
-    const Unit u = locate(blockIdx.y, a.sequences, [&](uint32_t s) {
+    const Unit u = locate(a.parts == 1 ? blockIdx.z : blockIdx.z / a.parts, a.sequences, [&](uint32_t s) {
         queries = span_of(a.query_offsets, s, a.tokens);
         keys = span_of(a.key_offsets, s, a.keys);
         return (static_cast<uint32_t>(queries.n) + kTileRows - 1) / kTileRows;
@@ -169,7 +173,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         }
     };
 
-    if (threadIdx.x == 0) taken_out = 0;
+    if (threadIdx.x == 0) not_finite = taken_out = 0;
     if (tile0 < tile1) {
         load_tile(tile0, lds);
         store_tile(lds);
@@ -202,6 +206,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
         value_at[i] = kTileBytes + Swizzle<CH>::value(r, chunk) * 16 + 8 * (piece & 1);
     }
 
+    // A value that is not finite, in a key that some row of the tile does not see,
+    // reaches that row through a weight of zero as NaN.  None is looked for on the
+    // way: where sums end up not finite the walk is done again, carefully.  (Looking
+    // at each partly seen tile first cost 24 packed prompts 9 of 143 us.)
+    const auto walk = [&](auto kind) {
+    constexpr bool careful = decltype(kind)::value;
+    if (tile0 < tile1) {
+        if constexpr (DIRECT && careful) {  // the last tile may have cut them
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) set_source(i, kTileKeys - 1);
+        }
+        if constexpr (careful) {
+            load_tile(tile0, lds);
+            store_tile(lds);
+        }
+    }
     for (int tile = tile0; tile < tile1; ++tile) {
         uint8_t* const here = lds + ((tile - tile0) & 1) * 2 * kTileBytes;
         uint8_t* const there = lds + (1 - ((tile - tile0) & 1)) * 2 * kTileBytes;
@@ -213,11 +233,10 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
             __syncthreads();
         }
         const int j0 = begin + tile * kTileKeys;
-        // Where some row of the workgroup does not see all of the tile, a value that
-        // is not finite must not reach it through a weight of zero: such values are
-        // taken out here and added below to the rows that see them.
-        if (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > row0 + shift) ||
-            (window && j0 <= last_row + shift - window)) {
+        // Carefully: such values are taken out of tiles that some row of the workgroup
+        // does not see all of, and added below to the rows that do.
+        if (careful && (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > row0 + shift) ||
+                        (window && j0 <= last_row + shift - window))) {
             bool bad = false;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
@@ -273,7 +292,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
                     const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * CH * 16);
                     sums.o[i] = mfma32(__builtin_bit_cast(f16x8, u32x4{lo.x, lo.y, hi.x, hi.y}), p[c], sums.o[i]);
                 }
-            if (taken_out == tile + 1) {
+            if (careful && taken_out == tile + 1) {
 #pragma unroll 1
                 for (int j = j0; j < min(j0 + kTileKeys, keys.n); ++j) {
                     const bool sees = static_cast<uint32_t>(last_seen - j) < seen;
@@ -297,6 +316,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void prompt_attention_kerne
             }
         }
         if (tile + 1 < tile1) store_tile(there);
+    }
+    };
+    walk(std::false_type());
+    if (wave_any(!sums.finite())) not_finite = 1;
+    __syncthreads();
+    if (not_finite) {
+        sums.clear();
+        walk(std::true_type());
     }
 
     if (row >= queries.n) return;
@@ -406,7 +433,7 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
                         : head_dim <= 192           ? prompt_attention_kernel<192, false>
                                                     : prompt_attention_kernel<256, false>;
     const auto s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(kernel, dim3(a.heads, p.tiles, p.parts), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.heads / a.kv_heads, p.tiles * p.parts), dim3(256), 0, s, a);
     const int status = static_cast<int>(hipGetLastError());
     if (status != 0 || p.parts <= 1) return status;
     return join_parts(workspace, output, rows, p.parts, q_heads, head_dim, output_stride, s);
