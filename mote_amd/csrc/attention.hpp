@@ -78,6 +78,22 @@ __device__ __forceinline__ Span span_at(Span mine, int lane) {  // the span that
     return {__builtin_amdgcn_readlane(mine.at, lane), __builtin_amdgcn_readlane(mine.n, lane)};
 }
 
+// The largest of a wave's lanes, in all of them.
+template <int Ctrl, int RowMask = 0xF>
+__device__ __forceinline__ float max_dpp(float v) {
+    const int b = __builtin_bit_cast(int, v);
+    return fmaxf(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(b, b, Ctrl, RowMask, 0xF, false)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = max_dpp<0xB1>(v);        // quad_perm [1,0,3,2]
+    v = max_dpp<0x4E>(v);        // quad_perm [2,3,0,1]
+    v = max_dpp<0x141>(v);       // row_half_mirror
+    v = max_dpp<0x140>(v);       // row_mirror
+    v = max_dpp<0x142, 0xA>(v);  // row_bcast:15 into rows 1 and 3
+    v = max_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+
 // Sums of a wave's lanes up to and with each.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
     const auto add = [&](auto shifted) { v += static_cast<uint32_t>(shifted); };
@@ -208,11 +224,22 @@ __global__ __launch_bounds__(256) void parts_join_kernel(const float2* __restric
     if (row >= rows) return;
     const uint32_t share = (parts + W - 1) / W, first = W == 1 ? 0 : wave * share;
     const uint32_t mine = first < parts ? min(share, parts - first) : 0;
+    const uint32_t d = (lane & (lanes - 1)) * 4;
+    const uint32_t at_once = 64 / lanes, own = lane / lanes;  // lanes: a power of two, four times it at least head_dim
+    const float* from = sums + (static_cast<uint64_t>(first) * rows + row) * head_dim + (d < head_dim ? d : 0);
+    const uint64_t step = static_cast<uint64_t>(rows) * head_dim;
+    f32x4 x[4];
+    const auto load = [&](uint32_t s0) {  // past the last part: the first, weighing nothing
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t s = s0 + i * at_once + own;
+            x[i] = *reinterpret_cast<const f32x4*>(from + (s < mine ? s : 0) * step);
+        }
+    };
     float2 ml = {-infinity(), 0.0f};
     if (lane < mine) ml = stats[static_cast<uint64_t>(first + lane) * rows + row];
-    float top = ml.x;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    if (mine != 0) load(0);
+    const float top = wave_max(ml.x);
     // A part that saw nothing has l = 0 and no sums; one with m = -inf and another l has NaN there.
     const float weight = ml.y == 0.0f ? 0.0f : ml.x == -infinity() ? ml.y : exp2_fast(ml.x - top);
     float l = wave_sum(weight * ml.y);
@@ -221,23 +248,15 @@ __global__ __launch_bounds__(256) void parts_join_kernel(const float2* __restric
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t d = (lane & (lanes - 1)) * 4;
-    const uint32_t at_once = 64 / lanes;  // lanes: a power of two, four times it at least head_dim
-    const float* from = sums + (static_cast<uint64_t>(first) * rows + row) * head_dim + (d < head_dim ? d : 0);
-    const uint64_t step = static_cast<uint64_t>(rows) * head_dim;
     for (uint32_t s0 = 0; s0 < mine; s0 += 4 * at_once) {
-        f32x4 x[4];
-        float w[4];
+        if (s0 != 0) load(s0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // four loads in flight; past the last part: the first, weighing nothing
-            const uint32_t s = s0 + i * at_once + lane / lanes;
-            w[i] = s < mine ? weights[wave][s] : 0.0f;
-            x[i] = *reinterpret_cast<const f32x4*>(from + (s < mine ? s : 0) * step);
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t s = s0 + i * at_once + own;
+            const float w = s < mine ? weights[wave][s] : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] += w != 0.0f ? w * x[i][e] : 0.0f;
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc[e] += w[i] != 0.0f ? w[i] * x[i][e] : 0.0f;
     }
     for (uint32_t over = lanes; over < 64; over <<= 1)
 #pragma unroll
