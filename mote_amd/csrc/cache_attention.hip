@@ -54,14 +54,16 @@ __device__ __forceinline__ f16x8 values_of(uint32_t lo, uint32_t hi) {
     return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// C: 32-dimension groups of the padded head; NT: 16-row tiles of a workgroup.
-template <int C, int NT>
-__global__ __launch_bounds__(256, NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) void cache_attention_kernel(CacheAttentionArgs a) {
+// C: 32-dimension groups of the padded head; NT: 16-row tiles of a workgroup;
+// WAVES: 4, or 16 where all of a short context goes through one workgroup.
+template <int C, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES > 4 ? 4 : NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) void
+cache_attention_kernel(CacheAttentionArgs a) {
     constexpr int kRows = 16 * NT;
     constexpr int kJoin = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // dimension groups joined at a time: 256 pieces of 8
     constexpr int kRowFloats = 32 * kJoin + 4;            // padded: rows start 4 banks apart
-    __shared__ __align__(16) float sums_of[4][kRows][kRowFloats];
-    __shared__ float2 stats_of[4][kRows];
+    __shared__ __align__(16) float sums_of[WAVES][kRows][kRowFloats];
+    __shared__ float2 stats_of[WAVES][kRows];
 
     uint32_t id = blockIdx.x;
     const uint32_t part = id % a.parts;
@@ -123,45 +125,52 @@ __global__ __launch_bounds__(256, NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) v
     const int32_t* table = a.table + static_cast<uint64_t>(seq) * a.table_blocks;
     constexpr uint32_t kPlane = 1024 * C;
     const uint32_t seen = a.window ? a.window : 0x80000000u;  // a row sees tokens (pos - seen, pos]
-    struct Block {
-        u32x4 k[C], v[C];
+    // A block's numbers are read two blocks ahead; its keys are on their way from
+    // where the last block's have been used, its values likewise, in the same registers.
+    struct Place {
+        const uint8_t* planes;
         float key_scale, value_scale;
         bool there;
     };
-    // Block numbers are read one block ahead of the block itself.
     const auto number = [&](int b) { return b < b1 ? table[b] : -1; };
-    const auto fetch = [&](int32_t block) {
-        Block f;
+    const auto place_of = [&](int32_t block) {
+        Place f;
         f.there = block >= 0 && static_cast<uint32_t>(block) < a.cache_blocks;
         const uint64_t at = static_cast<uint64_t>(f.there ? block : 0) * a.kv_heads + kv_head;
-        const uint8_t* planes = a.cache + at * (2 * kPlane) + lane * 16;
-#pragma unroll
-        for (int c = 0; c < C; ++c) f.k[c] = *reinterpret_cast<const u32x4*>(planes + 1024 * c);
-#pragma unroll
-        for (int c = 0; c < C; ++c) f.v[c] = *reinterpret_cast<const u32x4*>(planes + kPlane + 1024 * c);
+        f.planes = a.cache + at * (2 * kPlane) + lane * 16;
         f.key_scale = a.scales[at * 2];
         f.value_scale = a.scales[at * 2 + 1];
         return f;
     };
+    u32x4 kb[C], vb[C];
+    const auto load = [&](u32x4 (&to)[C], const uint8_t* from) {
+#pragma unroll
+        for (int c = 0; c < C; ++c) to[c] = *reinterpret_cast<const u32x4*>(from + 1024 * c);
+    };
     int b = b0 + static_cast<int>(wave);
     if (a.cache_blocks == 0) b = b1;  // nothing to point at
-    int32_t next = number(b + 4);
-    Block f{};
-    if (b < b1) f = fetch(number(b));
-    for (; b < b1; b += 4) {
-        Block ahead = f;
-        if (b + 4 < b1) ahead = fetch(next);
-        next = number(b + 8);
+    int32_t next = number(b + WAVES);
+    Place f{}, ahead{};
+    if (b < b1) {
+        f = place_of(number(b));
+        load(kb, f.planes);
+        load(vb, f.planes + kPlane);
+    }
+    for (; b < b1; b += WAVES) {
+        const bool more_to_come = b + WAVES < b1;
+        if (more_to_come) ahead = place_of(next);
+        next = number(b + 2 * WAVES);
         f32x4 s[NT][2];
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const f16x8 k0 = values_of(f.k[c][0], f.k[c][1]), k1 = values_of(f.k[c][2], f.k[c][3]);
+            const f16x8 k0 = values_of(kb[c][0], kb[c][1]), k1 = values_of(kb[c][2], kb[c][3]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 s[t][0] = mfma16(k0, qf[t][c], c == 0 ? zero : s[t][0]);
                 s[t][1] = mfma16(k1, qf[t][c], c == 0 ? zero : s[t][1]);
             }
         }
+        if (more_to_come) load(kb, ahead.planes);
         const int j0 = b * static_cast<int>(kBlockTokens);
         const bool edge = !f.there || j0 + 31 > shift + first_token ||
                           (a.window && j0 <= last_seen - static_cast<int>(a.window));
@@ -206,13 +215,14 @@ __global__ __launch_bounds__(256, NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) v
         }
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            const f16x8 v0 = values_of(f.v[c][0], f.v[c][1]), v1 = values_of(f.v[c][2], f.v[c][3]);
+            const f16x8 v0 = values_of(vb[c][0], vb[c][1]), v1 = values_of(vb[c][2], vb[c][3]);
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 o[t][2 * c] = mfma16(v0, p[t], o[t][2 * c]);
                 o[t][2 * c + 1] = mfma16(v1, p[t], o[t][2 * c + 1]);
             }
         }
+        if (more_to_come) load(vb, ahead.planes + kPlane);
         f = ahead;
     }
 
@@ -240,11 +250,11 @@ __global__ __launch_bounds__(256, NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) v
         if (row >= here || d >= a.head_dim) continue;
         float top = -infinity();
 #pragma unroll
-        for (int w = 0; w < 4; ++w) top = fmaxf(top, stats_of[w][row].x);
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats_of[w][row].x);
         f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
         float sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float2 ml = stats_of[w][row];
             const float weight = ml.x == -infinity() ? ml.y : exp2_fast(ml.x - top);  // saw nothing: 0, or NaN
             sum = __builtin_fmaf(weight, ml.y, sum);
@@ -464,13 +474,14 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
 }
 
 struct CachePlan {
-    uint32_t row_tiles, tile_rows, chunk, parts;
+    uint32_t row_tiles, tile_rows, chunk, parts, waves;
 };
 
 CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_t max_context, uint64_t heads,
                                uint64_t kv_heads, uint64_t head_dim) {
     const uint64_t rows = max_queries * (heads / kv_heads);
     CachePlan p{};
+    p.waves = 4;
     p.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 && head_dim <= 128 ? 64 : kTileRows;
     p.row_tiles = static_cast<uint32_t>((rows + p.tile_rows - 1) / p.tile_rows);
     const uint64_t blocks = (max_context + kBlockTokens - 1) / kBlockTokens + 1;
@@ -481,6 +492,16 @@ CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_
         const uint64_t most = (max_context + 255) / 256;
         if (parts > most) parts = most;
         p.parts = static_cast<uint32_t>(parts > 1 ? parts : 1);
+        return p;
+    }
+    if (p.tile_rows <= 32 && head_dim * p.tile_rows <= 2048) {
+        p.waves = 16;
+        uint64_t parts = blocks <= 48 || groups >= 256 ? 1 : (256 + groups - 1) / groups;
+        if (parts > kMostParts) parts = kMostParts;
+        uint64_t chunk = (blocks + parts - 1) / parts;
+        if (chunk < 16 && parts > 1) chunk = 16;
+        p.chunk = static_cast<uint32_t>(chunk);
+        p.parts = static_cast<uint32_t>((blocks + chunk - 1) / chunk);
         return p;
     }
     // About 1024 workgroups (four on a compute unit), none of fewer than 8 blocks (two a wave).
@@ -494,21 +515,26 @@ CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_
     return p;
 }
 
-template <int NT>
+template <int NT, int WAVES>
 auto kernel_of(uint32_t c) -> void (*)(CacheAttentionArgs) {
     switch (c) {
-        case 1: return cache_attention_kernel<1, NT>;
-        case 2: return cache_attention_kernel<2, NT>;
-        case 3: return cache_attention_kernel<3, NT>;
-        case 4: return cache_attention_kernel<4, NT>;
+        case 1: return cache_attention_kernel<1, NT, WAVES>;
+        case 2: return cache_attention_kernel<2, NT, WAVES>;
         default: break;
     }
-    if constexpr (NT <= 2) {
+    if constexpr (WAVES == 4 || NT == 1) {
         switch (c) {
-            case 5: return cache_attention_kernel<5, NT>;
-            case 6: return cache_attention_kernel<6, NT>;
-            case 7: return cache_attention_kernel<7, NT>;
-            case 8: return cache_attention_kernel<8, NT>;
+            case 3: return cache_attention_kernel<3, NT, WAVES>;
+            case 4: return cache_attention_kernel<4, NT, WAVES>;
+            default: break;
+        }
+    }
+    if constexpr (WAVES == 4 && NT <= 2) {
+        switch (c) {
+            case 5: return cache_attention_kernel<5, NT, WAVES>;
+            case 6: return cache_attention_kernel<6, NT, WAVES>;
+            case 7: return cache_attention_kernel<7, NT, WAVES>;
+            case 8: return cache_attention_kernel<8, NT, WAVES>;
             default: break;
         }
     }
@@ -591,9 +617,9 @@ MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache
     a.parts = p.parts;
     a.exponent = exponent;
     const uint32_t c = padded_dim(a.head_dim) / 32;
-    const auto kernel = p.tile_rows == 16   ? kernel_of<1>(c)
-                        : p.tile_rows == 32 ? kernel_of<2>(c)
-                        : p.tile_rows == 64 ? kernel_of<4>(c)
+    const auto kernel = p.tile_rows == 16   ? p.waves == 16 ? kernel_of<1, 16>(c) : kernel_of<1, 4>(c)
+                        : p.tile_rows == 32 ? p.waves == 16 ? kernel_of<2, 16>(c) : kernel_of<2, 4>(c)
+                        : p.tile_rows == 64 ? kernel_of<4, 4>(c)
                         : c <= 2            ? cache_tiles_kernel<2>
                         : c == 3            ? cache_tiles_kernel<3>
                         : c == 4            ? cache_tiles_kernel<4>
@@ -601,7 +627,7 @@ MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache
                                             : cache_tiles_kernel<8>;
     const auto s = static_cast<hipStream_t>(stream);
     const uint64_t groups = sequences * p.row_tiles * kv_heads * p.parts;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(64 * p.waves), 0, s, a);
     const int status = static_cast<int>(hipGetLastError());
     if (status != 0 || p.parts <= 1) return status;
     return join_parts(workspace, output, rows, p.parts, q_heads, head_dim, output_stride, s);
