@@ -54,14 +54,20 @@ __device__ __forceinline__ f16x8 values_of(uint32_t lo, uint32_t hi) {
     return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
 
-// C: 32-dimension groups of the padded head; NT: 16-row tiles of a workgroup;
-// WAVES: 4, or 16 where all of a short context goes through one workgroup.
-template <int C, int NT, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, WAVES > 4 ? 4 : NT == 1 && C <= 4 ? 3 : NT * C <= 8 ? 2 : 1) void
+// Waves of a workgroup: sixteen, one workgroup a compute unit, where a wave does
+// with 128 registers.  (One sequence of 131 000 tokens, 8 key heads of 128: 52 us,
+// with four waves and four times the workgroups 58; 32 of 6000: 71 and 79; 64 of up
+// to 8192: 107 and 113.)
+constexpr int waves_of(int c, int nt) { return c * nt <= 4 ? 16 : 4; }
+
+// C: 32-dimension groups of the padded head; NT: 16-row tiles of a workgroup.
+template <int C, int NT>
+__global__ __launch_bounds__(64 * waves_of(C, NT), waves_of(C, NT) == 16 ? 4 : NT * C <= 8 ? 2 : 1) void
 cache_attention_kernel(CacheAttentionArgs a) {
+    constexpr int WAVES = waves_of(C, NT);
     constexpr int kRows = 16 * NT;
-    constexpr int kJoin = NT == 1 ? 4 : NT == 2 ? 2 : 1;  // dimension groups joined at a time: 256 pieces of 8
-    constexpr int kRowFloats = 32 * kJoin + 4;            // padded: rows start 4 banks apart
+    constexpr int kJoin = 4 / NT;               // dimension groups joined at a time: 256 pieces of 8
+    constexpr int kRowFloats = 32 * kJoin + 4;  // padded: rows start 4 banks apart
     __shared__ __align__(16) float sums_of[WAVES][kRows][kRowFloats];
     __shared__ float2 stats_of[WAVES][kRows];
 
@@ -481,64 +487,65 @@ CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_
                                uint64_t kv_heads, uint64_t head_dim) {
     const uint64_t rows = max_queries * (heads / kv_heads);
     CachePlan p{};
-    p.waves = 4;
-    p.tile_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 && head_dim <= 128 ? 64 : kTileRows;
+    // Two small tiles that read the blocks twice, from cache, beat one of twice the
+    // rows, whose registers leave room for few waves: heads of 128, 16 sequences of
+    // 8000 tokens, 20 rows 52 us on 16-row tiles and 57 on one of 32; 48 rows 84 on
+    // 16, 75 on 32, 98 on one of 64 and 105 on one of 128; 80 rows 116, 107 and (128)
+    // 111; 120 rows 157, 123 and 116.  Heads of 256, 3000 tokens, 64 rows: 74 on 16, 84 on 128.
+    p.tile_rows = rows <= 32 || (head_dim > 128 && rows <= 64) ? 16 : rows <= 96 && head_dim <= 128 ? 32 : kTileRows;
     p.row_tiles = static_cast<uint32_t>((rows + p.tile_rows - 1) / p.tile_rows);
-    const uint64_t blocks = (max_context + kBlockTokens - 1) / kBlockTokens + 1;
     const uint64_t groups = sequences * p.row_tiles * kv_heads;
     if (p.tile_rows == kTileRows) {
         // Two workgroups a compute unit, none of fewer than four tiles.
+        p.waves = 4;
         uint64_t parts = groups >= 256 ? 1 : 512 / groups;
         const uint64_t most = (max_context + 255) / 256;
         if (parts > most) parts = most;
         p.parts = static_cast<uint32_t>(parts > 1 ? parts : 1);
         return p;
     }
-    if (p.tile_rows <= 32 && head_dim * p.tile_rows <= 2048) {
-        p.waves = 16;
-        uint64_t parts = blocks <= 48 || groups >= 256 ? 1 : (256 + groups - 1) / groups;
-        if (parts > kMostParts) parts = kMostParts;
-        uint64_t chunk = (blocks + parts - 1) / parts;
-        if (chunk < 16 && parts > 1) chunk = 16;
-        p.chunk = static_cast<uint32_t>(chunk);
-        p.parts = static_cast<uint32_t>((blocks + chunk - 1) / chunk);
-        return p;
-    }
-    // About 1024 workgroups (four on a compute unit), none of fewer than 8 blocks (two a wave).
-    uint64_t parts = groups >= 1024 ? 1 : (1024 + groups - 1) / groups;
+    // Sixteen waves to a compute unit, none with less than one block (of sixteen) or
+    // two (of four).  Contexts of up to three blocks for each of sixteen waves stay in
+    // one launch: 600 tokens 6.9 us against 9.8 in parts, 1500 tokens 10.0 both ways.
+    p.waves = static_cast<uint32_t>(waves_of(static_cast<int>(padded_dim(static_cast<uint32_t>(head_dim)) / 32),
+                                             static_cast<int>(p.tile_rows / 16)));
+    const uint64_t blocks = (max_context + kBlockTokens - 1) / kBlockTokens + 1;
+    const uint64_t wanted = p.waves == 16 ? 256 : 1024, least = p.waves == 16 ? 16 : 8;
+    uint64_t parts = groups >= wanted || (p.waves == 16 && blocks <= 48) ? 1 : (wanted + groups - 1) / groups;
     if (parts > kMostParts) parts = kMostParts;
     uint64_t chunk = (blocks + parts - 1) / parts;
-    if (chunk < 8) chunk = 8;
-    parts = (blocks + chunk - 1) / chunk;
+    if (chunk < least) chunk = least;
     p.chunk = static_cast<uint32_t>(chunk);
-    p.parts = static_cast<uint32_t>(parts);
+    p.parts = static_cast<uint32_t>((blocks + chunk - 1) / chunk);
     return p;
 }
 
-template <int NT, int WAVES>
-auto kernel_of(uint32_t c) -> void (*)(CacheAttentionArgs) {
+auto kernel_of(uint32_t tile_rows, uint32_t c) -> void (*)(CacheAttentionArgs) {
+    if (tile_rows == 16) switch (c) {
+        case 1: return cache_attention_kernel<1, 1>;
+        case 2: return cache_attention_kernel<2, 1>;
+        case 3: return cache_attention_kernel<3, 1>;
+        case 4: return cache_attention_kernel<4, 1>;
+        case 5: return cache_attention_kernel<5, 1>;
+        case 6: return cache_attention_kernel<6, 1>;
+        case 7: return cache_attention_kernel<7, 1>;
+        default: return cache_attention_kernel<8, 1>;
+    }
+    if (tile_rows == 32) switch (c) {
+        case 1: return cache_attention_kernel<1, 2>;
+        case 2: return cache_attention_kernel<2, 2>;
+        case 3: return cache_attention_kernel<3, 2>;
+        default: return cache_attention_kernel<4, 2>;
+    }
     switch (c) {
-        case 1: return cache_attention_kernel<1, NT, WAVES>;
-        case 2: return cache_attention_kernel<2, NT, WAVES>;
-        default: break;
+        case 1:
+        case 2: return cache_tiles_kernel<2>;
+        case 3: return cache_tiles_kernel<3>;
+        case 4: return cache_tiles_kernel<4>;
+        case 5:
+        case 6: return cache_tiles_kernel<6>;
+        default: return cache_tiles_kernel<8>;
     }
-    if constexpr (WAVES == 4 || NT == 1) {
-        switch (c) {
-            case 3: return cache_attention_kernel<3, NT, WAVES>;
-            case 4: return cache_attention_kernel<4, NT, WAVES>;
-            default: break;
-        }
-    }
-    if constexpr (WAVES == 4 && NT <= 2) {
-        switch (c) {
-            case 5: return cache_attention_kernel<5, NT, WAVES>;
-            case 6: return cache_attention_kernel<6, NT, WAVES>;
-            case 7: return cache_attention_kernel<7, NT, WAVES>;
-            case 8: return cache_attention_kernel<8, NT, WAVES>;
-            default: break;
-        }
-    }
-    return nullptr;
 }
 
 bool bad_shape(uint64_t sequences, uint64_t query_tokens, uint64_t max_queries, uint64_t max_context, uint64_t heads,
@@ -616,15 +623,7 @@ MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache
     a.chunk = p.chunk;
     a.parts = p.parts;
     a.exponent = exponent;
-    const uint32_t c = padded_dim(a.head_dim) / 32;
-    const auto kernel = p.tile_rows == 16   ? p.waves == 16 ? kernel_of<1, 16>(c) : kernel_of<1, 4>(c)
-                        : p.tile_rows == 32 ? p.waves == 16 ? kernel_of<2, 16>(c) : kernel_of<2, 4>(c)
-                        : p.tile_rows == 64 ? kernel_of<4, 4>(c)
-                        : c <= 2            ? cache_tiles_kernel<2>
-                        : c == 3            ? cache_tiles_kernel<3>
-                        : c == 4            ? cache_tiles_kernel<4>
-                        : c <= 6            ? cache_tiles_kernel<6>
-                                            : cache_tiles_kernel<8>;
+    const auto kernel = kernel_of(p.tile_rows, padded_dim(a.head_dim) / 32);
     const auto s = static_cast<hipStream_t>(stream);
     const uint64_t groups = sequences * p.row_tiles * kv_heads * p.parts;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(64 * p.waves), 0, s, a);
