@@ -94,44 +94,41 @@ __device__ __forceinline__ float wave_max(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
-// Sums of a wave's lanes up to and with each.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
-    const auto add = [&](auto shifted) { v += static_cast<uint32_t>(shifted); };
-    const auto at = [&]() { return static_cast<int>(v); };
-    add(__builtin_amdgcn_update_dpp(0, at(), 0x111, 0xF, 0xF, false));  // row_shr:1
-    add(__builtin_amdgcn_update_dpp(0, at(), 0x112, 0xF, 0xF, false));  // row_shr:2
-    add(__builtin_amdgcn_update_dpp(0, at(), 0x114, 0xF, 0xF, false));  // row_shr:4
-    add(__builtin_amdgcn_update_dpp(0, at(), 0x118, 0xF, 0xF, false));  // row_shr:8
-    add(__builtin_amdgcn_update_dpp(0, at(), 0x142, 0xA, 0xF, false));  // row_bcast:15 into rows 1 and 3
-    add(__builtin_amdgcn_update_dpp(0, at(), 0x143, 0xC, 0xF, false));  // row_bcast:31 into rows 2 and 3
-    return v;
-}
-
-// Unit `unit` of the units of all sequences in order, count(s) of sequence s:
-// its sequence, its number there and the lane that counted it.  Each wave looks
-// it up by itself, 64 sequences at a time.
+// Where work is divided by sequence: a sequence of n rows at offset a has its units
+// from a / PER + EACH s on (its number being s), room for as many as n / PER + EACH.
+// So a unit's sequence is found by its slot alone, from the offsets in order, 64 at
+// a time: one load for up to 64 sequences, two for 4096.  Each wave looks it up by
+// itself.  visit(s) is called, before it is known which is found, by a lane of each
+// sequence that is near; `lane` is the one whose sequence it is.
 struct Unit {
-    uint32_t sequence, local, of;
+    uint32_t sequence, local;
     int lane;
     bool found;
 };
-template <typename Count>
-__device__ __forceinline__ Unit locate(uint32_t unit, uint32_t sequences, Count count) {
+template <uint32_t PER, uint32_t EACH, typename Visit>
+__device__ __forceinline__ Unit locate(uint32_t unit, const int32_t* offsets, uint32_t sequences, uint32_t tokens,
+                                       Visit visit) {
     const uint32_t lane = threadIdx.x & 63;
-    uint32_t base = 0;
-    for (uint32_t s0 = 0; s0 < sequences; s0 += 64) {
-        const uint32_t n = s0 + lane < sequences ? count(s0 + lane) : 0;
-        const uint32_t upto = wave_scan(n);
-        const uint64_t past = __builtin_amdgcn_ballot_w64(base + upto > unit);
-        if (past != 0) {
-            const int at = __builtin_ctzll(past);
-            const uint32_t mine = __builtin_amdgcn_readlane(n, at);
-            const uint32_t before = base + __builtin_amdgcn_readlane(upto, at) - mine;
-            return {s0 + at, unit - before, mine, at, true};
+    uint32_t first = 0, count = sequences;
+    for (;;) {
+        const uint32_t stride = (count + 63) / 64;
+        const uint32_t s = first + lane * stride;
+        uint32_t slot = 0xFFFFFFFFu;
+        if (lane * stride < count) {
+            if (stride == 1) visit(s);
+            slot = static_cast<uint32_t>(min(max(offsets[s], 0), static_cast<int>(tokens))) / PER + EACH * s;
         }
-        base += __builtin_amdgcn_readlane(upto, 63);
+        const uint64_t before = __builtin_amdgcn_ballot_w64(slot <= unit);
+        if (before == 0) return {0, 0, 0, false};
+        const int at = 63 - __builtin_clzll(before);
+        first += at * stride;
+        count = min(stride, count - at * stride);
+        if (stride == 1) return {first, unit - static_cast<uint32_t>(__builtin_amdgcn_readlane(slot, at)), at, true};
     }
-    return {0, 0, 0, 0, false};
+}
+// The units there are room for.
+constexpr uint64_t units_of(uint64_t per, uint64_t each, uint64_t sequences, uint64_t tokens) {
+    return tokens / per + each * sequences;
 }
 
 // The running sums of the row that a lane of a 32-row wave holds half of: of the 32

@@ -47,16 +47,16 @@ struct Piece {
 __device__ __forceinline__ Piece piece_of(const CacheArgs& a, uint32_t unit, uint32_t head) {
     Span rows;  // first of the lane's sequence, then of the workgroup's
     uint32_t first;
-    const Unit u = locate(unit, a.sequences, [&](uint32_t s) {
+    const Unit u = locate<kBlockTokens, 2>(unit, a.offsets, a.sequences, a.tokens, [&](uint32_t s) {
         rows = span_of(a.offsets, s, a.tokens);
         first = max(a.positions[s], 0);
-        return rows.n > 0 ? (first + rows.n - 1) / kBlockTokens - first / kBlockTokens + 1 : 0u;
     });
     Piece r{0, 0, 0, 0, false};
     if (!u.found) return r;
     rows = span_at(rows, u.lane);
     first = __builtin_amdgcn_readlane(first, u.lane);
     const uint32_t block = first / kBlockTokens + u.local;
+    if (block * kBlockTokens >= first + static_cast<uint32_t>(rows.n)) return r;  // room that it does not need
     if (block >= a.table_blocks) return r;
     const int32_t id = a.table[static_cast<uint64_t>(u.sequence) * a.table_blocks + block];
     if (id < 0 || static_cast<uint32_t>(id) >= a.cache_blocks) return r;
@@ -342,13 +342,6 @@ int check_cache_call(const void* k, const void* v, const void* offsets, const vo
     return 1;
 }
 
-// Blocks that `tokens` new tokens of `sequences` sequences can touch: n tokens of
-// one touch at most (n + 30) / 32 + 1.
-uint64_t most_pieces(uint64_t sequences, uint64_t tokens) {
-    const uint64_t with = sequences < tokens ? sequences : tokens;  // sequences with a token at all
-    return (tokens + 30 * with) / kBlockTokens + with;
-}
-
 }  // namespace
 }  // namespace mote::attention
 
@@ -361,7 +354,7 @@ MOTE_EXPORT int mote_hip_kv_cache_append_q8(const void* k, const void* v, const 
     const int go = check_cache_call(k, v, offsets, positions, block_table, cache, scales, sequences, tokens, kv_heads,
                                     head_dim, table_blocks, cache_blocks, stream);
     if (go != 1) return go;
-    const uint64_t pieces = most_pieces(sequences, tokens);
+    const uint64_t pieces = units_of(kBlockTokens, 2, sequences, tokens);
     if (pieces > kMostGrid) return kInvalid;
     const CacheArgs a{static_cast<const int32_t*>(offsets), static_cast<const int32_t*>(positions),
                       static_cast<const int32_t*>(block_table), static_cast<uint8_t*>(cache),
@@ -386,7 +379,7 @@ MOTE_EXPORT int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* sca
                                     head_dim, table_blocks, cache_blocks, stream);
     if (go != 1) return go;
     if (k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim) return kInvalid;
-    const uint64_t pieces = most_pieces(sequences, tokens);
+    const uint64_t pieces = units_of(kBlockTokens, 2, sequences, tokens);
     if (pieces > kMostGrid) return kInvalid;
     const CacheArgs a{static_cast<const int32_t*>(offsets), static_cast<const int32_t*>(positions),
                       static_cast<const int32_t*>(block_table), static_cast<uint8_t*>(const_cast<void*>(cache)),

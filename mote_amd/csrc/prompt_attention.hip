@@ -33,7 +33,7 @@ struct PromptArgs {
     float2* stats;  // null: one part, written to output
     float* sums;
     uint64_t q_stride, k_stride, v_stride, out_stride;
-    uint32_t sequences, tokens, keys, heads, kv_heads, head_dim, window, causal, parts;
+    uint32_t sequences, tokens, keys, heads, kv_heads, head_dim, window, causal, parts, first;
     float exponent;  // scale log2(e)
 };
 
@@ -87,18 +87,22 @@ __global__ __launch_bounds__(256, DP == 64 && DIRECT ? 4 : DP <= 128 ? 2 : 1) vo
 
     // Key heads first, so that with eight of them each XCD's L2 keeps one; then the
     // query heads that share them; then the tiles.
-    const uint32_t kv_head = blockIdx.x, part = a.parts == 1 ? 0 : blockIdx.z % a.parts;
+    const uint32_t kv_head = blockIdx.x;
     const uint32_t head = kv_head * gridDim.y + blockIdx.y;
     Span queries, keys;  // first of the lane's sequence, then of the workgroup's
-    const Unit u = locate(a.parts == 1 ? blockIdx.z : blockIdx.z / a.parts, a.sequences, [&](uint32_t s) {
-        queries = span_of(a.query_offsets, s, a.tokens);
-        keys = span_of(a.key_offsets, s, a.keys);
-        return (static_cast<uint32_t>(queries.n) + kTileRows - 1) / kTileRows;
-    });
+    const uint32_t z = a.first + blockIdx.z;
+    const uint32_t part = a.parts == 1 ? 0 : z % a.parts;
+    const Unit u = locate<kTileRows, 1>(a.parts == 1 ? z : z / a.parts, a.query_offsets, a.sequences, a.tokens,
+                                        [&](uint32_t s) {
+                                            queries = span_of(a.query_offsets, s, a.tokens);
+                                            keys = span_of(a.key_offsets, s, a.keys);
+                                        });
     if (!u.found) return;
     queries = span_at(queries, u.lane);
     keys = span_at(keys, u.lane);
-    const int row0 = static_cast<int>((u.of - 1 - u.local) * kTileRows);  // the longest walks first
+    const uint32_t row_tiles = (static_cast<uint32_t>(queries.n) + kTileRows - 1) / kTileRows;
+    if (u.local >= row_tiles) return;  // room that the sequence does not need
+    const int row0 = static_cast<int>((row_tiles - 1 - u.local) * kTileRows);  // the longest walks first
     const int shift = keys.n - queries.n;  // position of the first query
     const int last_row = min(row0 + static_cast<int>(kTileRows), queries.n) - 1;
     const int window = static_cast<int>(a.window);
@@ -336,13 +340,13 @@ __global__ __launch_bounds__(256, DP == 64 && DIRECT ? 4 : DP <= 128 ? 2 : 1) vo
 }
 
 struct PromptPlan {
-    uint32_t tiles, parts;
+    uint64_t tiles;
+    uint32_t parts;
 };
 
 PromptPlan plan_prompt(uint64_t sequences, uint64_t tokens, uint64_t max_keys, uint64_t heads) {
-    const uint64_t with = sequences < tokens ? sequences : tokens;  // sequences with a query at all
     PromptPlan p{};
-    p.tiles = static_cast<uint32_t>((tokens + (kTileRows - 1) * with) / kTileRows);
+    p.tiles = units_of(kTileRows, 1, sequences, tokens);
     const uint64_t groups = p.tiles * heads, most = (max_keys + 255) / 256;  // no part under four tiles
     uint64_t parts = groups >= 256 ? 1 : 512 / groups;
     if (parts > most) parts = most;
@@ -396,7 +400,6 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
     const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads);
     const uint64_t rows = query_tokens * q_heads, need = parts_bytes(rows, p.parts, head_dim);
     if (need > 0 && (!workspace || off_grid(workspace, 16) || workspace_bytes < need)) return kInvalid;
-    if (p.tiles > 65535) return kInvalid;
     PromptArgs a{};
     a.q = static_cast<const _Float16*>(q);
     a.k = static_cast<const _Float16*>(k);
@@ -435,8 +438,15 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
                         : head_dim <= 192           ? prompt_attention_kernel<192, false>
                                                     : prompt_attention_kernel<256, false>;
     const auto s = static_cast<hipStream_t>(stream);
-    hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.heads / a.kv_heads, p.tiles * p.parts), dim3(256), 0, s, a);
-    const int status = static_cast<int>(hipGetLastError());
-    if (status != 0 || p.parts <= 1) return status;
+    constexpr uint64_t kMostZ = 65535;
+    for (uint64_t first = 0; first < p.tiles * p.parts; first += kMostZ) {
+        const uint64_t left = p.tiles * p.parts - first;
+        a.first = static_cast<uint32_t>(first);
+        hipLaunchKernelGGL(kernel, dim3(a.kv_heads, a.heads / a.kv_heads, static_cast<unsigned>(left < kMostZ ? left : kMostZ)),
+                           dim3(256), 0, s, a);
+        const int status = static_cast<int>(hipGetLastError());
+        if (status != 0) return status;
+    }
+    if (p.parts <= 1) return 0;
     return join_parts(workspace, output, rows, p.parts, q_heads, head_dim, output_stride, s);
 }

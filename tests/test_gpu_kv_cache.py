@@ -127,6 +127,16 @@ def test_append_pieces_join(stream):
     held.check()
 
 
+def test_append_to_many_sequences(stream):
+    """More than a wave looks up at once, most of them with nothing new."""
+    rng = np.random.default_rng(17)
+    held = Held(Cache(300, 1, 32, rng), tables(rng, 150, 2, 300))
+    lengths = [int(n) for n in rng.choice([0, 0, 1, 5, 33], 150)]
+    positions = [int(p) for p in rng.integers(0, 31, 150)]
+    held.append(stream, rows(rng, sum(lengths), 1, 32), rows(rng, sum(lengths), 1, 32), lengths, positions)
+    held.check()
+
+
 def test_append_zeros_and_extremes(stream):
     rng = np.random.default_rng(3)
     held = Held(Cache(6, 1, 64, rng), tables(rng, 1, 6, 6))

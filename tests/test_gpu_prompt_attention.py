@@ -112,11 +112,31 @@ def test_head_groups(stream, heads, kv_heads):
 @pytest.mark.parametrize("queries,keys", [
     ([0, 5, 0, 1, 130, 0], [3, 5, 0, 40, 130, 9]),        # sequences without queries, or nothing at all
     ([1] * 70 + [50], [1] * 70 + [50]),                   # more sequences than a wave looks up at once
+    ([0, 3, 0, 200] * 40, [2, 3, 0, 200] * 40),
     ([5, 90, 3], [2, 40, 0]),                             # fewer keys than queries: the first see nothing
     ([128, 256, 64], [128, 256, 64]),                     # whole tiles
 ])
 def test_packed(stream, queries, keys):
     check(stream, len(queries), queries, keys, 2, 1, 64)
+
+
+@pytest.mark.parametrize("count", [4097, 70000])
+def test_very_many_sequences(stream, count):
+    """Of one token each (whose attention is its value) and now and then five: three
+    steps of the look-up, and more tiles than one launch has room for."""
+    rng = np.random.default_rng(count)
+    lengths = np.ones(count, np.int64)
+    lengths[rng.integers(0, count, 50)] = 5
+    q, k, v = tensors(count, lengths.tolist(), lengths.tolist(), 1, 1, 8)
+    call = Call(q, k, v, lengths.tolist(), lengths.tolist(), own_keys=True)
+    call.run(stream)
+    got = call.result(stream)
+    at = np.concatenate([[0], np.cumsum(lengths)])[:-1]
+    single = at[lengths == 1]
+    assert (got[single].view(np.uint16) == v[single].view(np.uint16)).all()
+    for a in at[lengths == 5]:
+        o, bound = attend(q[a:a + 5], k[a:a + 5], v[a:a + 5], call.scale)
+        assert_within(got[a:a + 5], o, bound)
 
 
 @pytest.mark.parametrize("window", [1, 2, 17, 63, 64, 65, 100, 129, 299, 300, 301, 1 << 40])
