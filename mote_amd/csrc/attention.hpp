@@ -167,26 +167,38 @@ struct RowSums {
     }
     // What exponents are taken less of.
     __device__ __forceinline__ float base() const { return m == -infinity() ? 0.0f : m - kShift; }
-    // The row's result to `out`, or with statistics its part to row `at` of them.
-    template <bool WHOLE>
-    __device__ __forceinline__ void write(_Float16* out, float2* stats, float* sums, uint64_t at, uint32_t head_dim,
-                                          int h) {
-        const float all = sum_of(across_halves(l));
-        if (stats == nullptr) {
-            const float inv = all != 0.0f ? 1.0f / all : 0.0f;
+    // The wave's results: through `stage`, 2 KB x D of LDS that is the wave's own, so
+    // that whole rows leave in 16-byte chunks of neighbouring lanes (a lane's own
+    // pieces are 8 bytes a row: 64 prompts of 64 tokens SSS us so).  row_at(i):
+    // where row i goes, null for none.
+    template <bool WHOLE, typename RowAt>
+    __device__ __forceinline__ void write(uint8_t* stage, uint32_t head_dim, RowAt row_at) const {
+        constexpr int CH = 4 * D, G = (CH & -CH) > 16 ? 16 : (CH & -CH);
+        const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+        const float all = sum_of(across_halves(l)), inv = all != 0.0f ? 1.0f / all : 0.0f;
+        const auto chunk = [&](int row, int c) { return stage + (row * CH + (c ^ (row / (16 / G) % G))) * 16; };
 #pragma unroll
-            for (int i = 0; i < D; ++i)
+        for (int i = 0; i < D; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; r += 4) {
-                    const uint32_t d = 32 * i + 2 * r + 4 * h;
-                    if (!WHOLE && d >= head_dim) continue;
-                    const f16x2 lo = {static_cast<_Float16>(o[i][r] * inv), static_cast<_Float16>(o[i][r + 1] * inv)};
-                    const f16x2 hi = {static_cast<_Float16>(o[i][r + 2] * inv), static_cast<_Float16>(o[i][r + 3] * inv)};
-                    *reinterpret_cast<u32x2_a2*>(out + d) =
-                        u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
-                }
-            return;
+            for (int r = 0; r < 16; r += 4) {
+                const f16x2 lo = {static_cast<_Float16>(o[i][r] * inv), static_cast<_Float16>(o[i][r + 1] * inv)};
+                const f16x2 hi = {static_cast<_Float16>(o[i][r + 2] * inv), static_cast<_Float16>(o[i][r + 3] * inv)};
+                *reinterpret_cast<u32x2*>(chunk(n, 4 * i + r / 4) + 8 * h) =
+                    u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+            }
+#pragma unroll
+        for (int j = 0; j < CH / 2; ++j) {
+            const int row = (64 * j + lane) / CH, c = (64 * j + lane) % CH;
+            _Float16* const to = row_at(row);
+            if (to != nullptr && (WHOLE || 8u * c < head_dim))
+                *reinterpret_cast<u32x4_a2*>(to + 8 * c) = *reinterpret_cast<const u32x4*>(chunk(row, c));
         }
+    }
+    // The row's part, to row `at` of the statistics and sums.
+    template <bool WHOLE>
+    __device__ __forceinline__ void write_part(float2* stats, float* sums, uint64_t at, uint32_t head_dim) const {
+        const int h = (threadIdx.x >> 5) & 1;
+        const float all = sum_of(across_halves(l));
         if (h == 0) stats[at] = float2{m == -infinity() ? m : m - kShift, all};
         if (all == 0.0f) return;  // saw nothing: not read
 #pragma unroll

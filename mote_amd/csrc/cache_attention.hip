@@ -472,11 +472,19 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
         }
         if (tile + 1 < tile1) store_tile(there);
     }
-    if (r >= all_rows) return;  // both halves of the row
-    const uint64_t out_row = static_cast<uint64_t>(rows.at + token);
-    sums.template write<false>(a.output + out_row * a.out_stride + static_cast<uint64_t>(head) * a.head_dim, a.stats,
-                               a.sums, static_cast<uint64_t>(part) * a.tokens * a.heads + out_row * a.heads + head,
-                               a.head_dim, h);
+    if (a.stats == nullptr) {
+        __syncthreads();  // no tile is read any more
+        sums.template write<false>(lds + wave * (2048 * CT), a.head_dim, [&](int i) -> _Float16* {
+            const uint32_t row = wave_row + i;
+            if (row >= all_rows) return nullptr;
+            return a.output + static_cast<uint64_t>(rows.at + row / group) * a.out_stride +
+                   static_cast<uint64_t>(kv_head * group + row % group) * a.head_dim;
+        });
+    } else if (r < all_rows) {
+        const uint64_t all = static_cast<uint64_t>(a.tokens) * a.heads;
+        sums.template write_part<false>(a.stats, a.sums,
+                                        part * all + static_cast<uint64_t>(rows.at + token) * a.heads + head, a.head_dim);
+    }
 }
 
 struct CachePlan {

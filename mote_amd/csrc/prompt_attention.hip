@@ -330,13 +330,22 @@ __global__ __launch_bounds__(256, DP == 64 && DIRECT ? 4 : DP <= 128 ? 2 : 1) vo
     if (not_finite) {
         sums.clear();
         walk(std::true_type());
+        __syncthreads();
     }
 
-    if (row >= queries.n) return;
-    const uint64_t token = static_cast<uint64_t>(queries.at + row);
-    sums.template write<DIRECT>(a.output + token * a.out_stride + static_cast<uint64_t>(head) * a.head_dim, a.stats,
-                                a.sums, part * (static_cast<uint64_t>(a.tokens) * a.heads) + token * a.heads + head,
-                                a.head_dim, h);
+    // No tile is read any more.
+    if (a.stats == nullptr) {
+        sums.template write<DIRECT>(lds + wave * (64 * DP), a.head_dim, [&](int i) -> _Float16* {
+            if (wave_row + i >= queries.n) return nullptr;
+            return a.output + static_cast<uint64_t>(queries.at + wave_row + i) * a.out_stride +
+                   static_cast<uint64_t>(head) * a.head_dim;
+        });
+    } else if (row < queries.n) {
+        const uint64_t rows = static_cast<uint64_t>(a.tokens) * a.heads;
+        sums.template write_part<DIRECT>(a.stats, a.sums,
+                                         part * rows + static_cast<uint64_t>(queries.at + row) * a.heads + head,
+                                         a.head_dim);
+    }
 }
 
 struct PromptPlan {
