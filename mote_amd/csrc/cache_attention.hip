@@ -504,12 +504,8 @@ CachePlan plan_cache_attention(uint64_t sequences, uint64_t max_queries, uint64_
     p.row_tiles = static_cast<uint32_t>((rows + p.tile_rows - 1) / p.tile_rows);
     const uint64_t groups = sequences * p.row_tiles * kv_heads;
     if (p.tile_rows == kTileRows) {
-        // Two workgroups a compute unit, none of fewer than four tiles.
         p.waves = 4;
-        uint64_t parts = groups >= 256 ? 1 : 512 / groups;
-        const uint64_t most = (max_context + 255) / 256;
-        if (parts > most) parts = most;
-        p.parts = static_cast<uint32_t>(parts > 1 ? parts : 1);
+        p.parts = choose_parts(groups, (max_context + 63) / 64 + 1, sequences * max_queries * heads, head_dim, 1.8, 2.2);
         return p;
     }
     // Sixteen waves to a compute unit, none with less than one block (of sixteen) or

@@ -353,13 +353,10 @@ struct PromptPlan {
     uint32_t parts;
 };
 
-PromptPlan plan_prompt(uint64_t sequences, uint64_t tokens, uint64_t max_keys, uint64_t heads) {
+PromptPlan plan_prompt(uint64_t sequences, uint64_t tokens, uint64_t max_keys, uint64_t heads, uint64_t head_dim) {
     PromptPlan p{};
     p.tiles = units_of(kTileRows, 1, sequences, tokens);
-    const uint64_t groups = p.tiles * heads, most = (max_keys + 255) / 256;  // no part under four tiles
-    uint64_t parts = groups >= 256 ? 1 : 512 / groups;
-    if (parts > most) parts = most;
-    p.parts = static_cast<uint32_t>(parts > 1 ? parts : 1);
+    p.parts = choose_parts(p.tiles * heads, (max_keys + kTileKeys - 1) / kTileKeys, tokens * heads, head_dim, 1.4, 2.0);
     return p;
 }
 
@@ -382,7 +379,7 @@ MOTE_EXPORT int mote_hip_prompt_attention_workspace(uint64_t sequences, uint64_t
     *bytes = 0;
     if (bad_shape(sequences, query_tokens, key_tokens, max_keys, q_heads, kv_heads, head_dim)) return kInvalid;
     if (sequences == 0 || query_tokens == 0 || q_heads == 0 || head_dim == 0) return 0;
-    const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads);
+    const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads, head_dim);
     *bytes = static_cast<size_t>(parts_bytes(query_tokens * q_heads, p.parts, head_dim));
     return 0;
 }
@@ -406,7 +403,7 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
         off_grid(key_offsets, 4))
         return kInvalid;
     if (sequences == 0 || query_tokens == 0 || q_heads == 0 || head_dim == 0) return 0;
-    const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads);
+    const PromptPlan p = plan_prompt(sequences, query_tokens, max_keys, q_heads, head_dim);
     const uint64_t rows = query_tokens * q_heads, need = parts_bytes(rows, p.parts, head_dim);
     if (need > 0 && (!workspace || off_grid(workspace, 16) || workspace_bytes < need)) return kInvalid;
     PromptArgs a{};
