@@ -333,7 +333,8 @@ int mote_hip_prompt_attention_f16(const void* q, const void* k, const void* v, v
  * block_table[s x table_blocks + b] (int32).  With P = head_dim rounded up to a
  * multiple of 32, `cache` is uint8 [cache_blocks][kv_heads][2][32 P] (planes of
  * keys and of values, 16-byte aligned) and `scales` float
- * [cache_blocks][kv_heads][2]; byte u of a plane stands for (u - 128) x its scale.
+ * [cache_blocks][kv_heads][2], not negative; byte u of a plane stands for (u - 128) x
+ * its scale.
  * With c = d / 32, element (token t of the block, dimension d) is byte
  *   keys:   [c][(d % 32) / 8][t % 16][t / 16][d % 8]                of [P/32][4][16][2][8]
  *   values: [c][(t % 16) / 4][d % 16][(d % 32) / 16][4 (t/16) + t%4]  of the same.

@@ -3,12 +3,21 @@
 // binary16 keys and values.
 //
 // A workgroup takes 128 query rows of one head, 32 a wave, and walks the keys
-// they see in tiles of 64 that the four waves share through LDS.  S^T = K Q^T
+// they see in tiles of 64 or 32 that the four waves share through LDS.  S^T = K Q^T
 // and O^T = V^T P^T on the 32 x 32 x 16 matrix instruction: with keys as the
 // instruction's rows a lane ends with the scores of one query row, the running
 // maximum and sum need one exchange between the wave's halves, and the scores
 // are the operand of the second product where they lie.  Its other operand,
 // V^T, comes out of the row-major tile through LDS transpose reads.
+//
+// 64 x 32 scores of 128 dimensions are 32 matrix instructions (1024 cycles) and
+// about 150 vector instructions, a fifth of them exponentials (1050 cycles); two
+// workgroups a compute unit run the one under the other.  1 x 8192 tokens, 32 heads
+// of 128, causal: 557 us, 990 TFLOP/s (a large library product here: 1175), the
+// matrix cores busy 54 % of the cycles at the 1.78 GHz that the card's power leaves;
+// two tiles of a compute unit take 3450 cycles, 2048 of them matrix instructions.
+// Short prompts wait for their starts: 6300 cycles before a workgroup's first
+// product, 24 prompts of up to 1000 tokens 123 us, 550 TFLOP/s.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -21,7 +30,6 @@ namespace mote::attention {
 namespace {
 
 constexpr uint32_t kTileRows = 128;
-constexpr int kTileKeys = 64;
 
 struct PromptArgs {
     const _Float16* q;
@@ -76,11 +84,18 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t pair) {
 // head_dim = DP, so tiles go from memory to LDS without passing registers.  (Heads
 // of 64: four workgroups a compute unit, 95 us in the windowed case against 98 with
 // the three that fit without the bound.)
-template <int DP, bool DIRECT>
-__global__ __launch_bounds__(256, DP == 64 && DIRECT ? 4 : DP <= 128 ? 2 : 1) void prompt_attention_kernel(PromptArgs a) {
+//
+// KEYS: of a tile.  Tiles of 32 keys leave room for three workgroups of 128
+// dimensions a compute unit, which cover each other's starts where there are many:
+// 64 prompts of 64 tokens 25 us against 30, of 256 92 against 103, 24 of up to 1000
+// 122 against 129, 8192 tokens level; with few workgroups tiles of 64 have the
+// fewer turns: 1024 tokens 26 against 32, 333 queries over 7333 keys 62 against 65.
+template <int DP, bool DIRECT, int KEYS>
+__global__ __launch_bounds__(256, DIRECT && DP == 64 ? 4 : KEYS == 32 ? 3 : DP <= 128 ? 2 : 1) void
+prompt_attention_kernel(PromptArgs a) {
     constexpr int CH = DP / 8, KS = DP / 16, DT = DP / 32;
-    constexpr int kLoads = kTileKeys * CH / 256;  // 16-byte chunks of a thread in each tile
-    constexpr int kTileBytes = kTileKeys * CH * 16;
+    constexpr int kLoads = KEYS * CH / 256;       // 16-byte chunks of a thread in each tile
+    constexpr int kTileBytes = KEYS * CH * 16;
     __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two of [keys | values]
     __shared__ int not_finite;  // a wave's sums are not
     __shared__ int taken_out;   // the last tile, from 1, with values that are not finite taken out
@@ -109,8 +124,8 @@ __global__ __launch_bounds__(256, DP == 64 && DIRECT ? 4 : DP <= 128 ? 2 : 1) vo
 
     // The keys that any row of the tile sees, and this part's tiles of them.
     const int end = a.causal ? min(max(last_row + shift + 1, 0), keys.n) : keys.n;
-    const int begin = window ? min(max(row0 + shift - window + 1, 0), end) & ~(kTileKeys - 1) : 0;
-    const int tiles = (end - begin + kTileKeys - 1) / kTileKeys;
+    const int begin = window ? min(max(row0 + shift - window + 1, 0), end) & ~(KEYS - 1) : 0;
+    const int tiles = (end - begin + KEYS - 1) / KEYS;
     const int per_part = (tiles + static_cast<int>(a.parts) - 1) / static_cast<int>(a.parts);
     const int tile0 = static_cast<int>(part) * per_part, tile1 = min(tiles, tile0 + per_part);
 
@@ -138,15 +153,15 @@ __global__ __launch_bounds__(256, DP == 64 && DIRECT ? 4 : DP <= 128 ? 2 : 1) vo
     };
     if constexpr (DIRECT) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) set_source(i, kTileKeys - 1);
+        for (int i = 0; i < kLoads; ++i) set_source(i, KEYS - 1);
     }
     const auto load_tile = [&](int tile, uint8_t* to) {
-        const int j0 = begin + tile * kTileKeys;
+        const int j0 = begin + tile * KEYS;
         if constexpr (DIRECT) {
             const Buffer kb = buffer_at(k + static_cast<uint64_t>(j0) * a.k_stride);
             const Buffer vb = buffer_at(v + static_cast<uint64_t>(j0) * a.v_stride);
             const int last = keys.n - 1 - j0;
-            if (last < kTileKeys - 1) {  // rows past the last repeat it; no row sees them
+            if (last < KEYS - 1) {  // rows past the last repeat it; no row sees them
 #pragma unroll
                 for (int i = 0; i < kLoads; ++i) set_source(i, last);
             }
@@ -217,112 +232,117 @@ __global__ __launch_bounds__(256, DP == 64 && DIRECT ? 4 : DP <= 128 ? 2 : 1) vo
     // way: where sums end up not finite the walk is done again, carefully.  (Looking
     // at each partly seen tile first cost 24 packed prompts 9 of 143 us.)
     const auto walk = [&](auto kind) {
-    constexpr bool careful = decltype(kind)::value;
-    if (tile0 < tile1) {
-        if constexpr (DIRECT && careful) {  // the last tile may have cut them
+        constexpr bool careful = decltype(kind)::value;
+        if (tile0 < tile1) {
+            if constexpr (DIRECT && careful) {  // the last tile may have cut them
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) set_source(i, kTileKeys - 1);
-        }
-        if constexpr (careful) {
-            load_tile(tile0, lds);
-            store_tile(lds);
-        }
-    }
-    for (int tile = tile0; tile < tile1; ++tile) {
-        uint8_t* const here = lds + ((tile - tile0) & 1) * 2 * kTileBytes;
-        uint8_t* const there = lds + (1 - ((tile - tile0) & 1)) * 2 * kTileBytes;
-        if constexpr (DIRECT) {
-            wait_counts<vm_wait(0)>();
-            group_barrier();
-            order_fence();
-        } else {
-            __syncthreads();
-        }
-        const int j0 = begin + tile * kTileKeys;
-        // Carefully: such values are taken out of tiles that some row of the workgroup
-        // does not see all of, and added below to the rows that do.
-        if (careful && (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > row0 + shift) ||
-                        (window && j0 <= last_row + shift - window))) {
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) {
-                u32x4* const at = reinterpret_cast<u32x4*>(here + kTileBytes) + threadIdx.x + 256 * i;
-                const u32x4 x = *at;
-                u32x4 fine;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) fine[w] = finite_of(x[w]);
-                if (fine[0] != x[0] || fine[1] != x[1] || fine[2] != x[2] || fine[3] != x[3]) {
-                    *at = fine;
-                    bad = true;
-                }
+                for (int i = 0; i < kLoads; ++i) set_source(i, KEYS - 1);
             }
-            if (bad) taken_out = tile + 1;
-            __syncthreads();
+            if constexpr (careful) {
+                load_tile(tile0, lds);
+                store_tile(lds);
+            }
         }
-        if (tile + 1 < tile1) load_tile(tile + 1, there);
-        if (!(a.causal && (j0 > wave_last || (window && j0 + kTileKeys - 1 <= wave_row + shift - window)))) {
-            f32x16 s[2];
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int i = 0; i < KS; ++i)
-                    s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + key_at[i] + 32 * CH * 16 * t), qf[i],
-                                  i == 0 ? RowSums<DT>::zero() : s[t]);
-            if (j0 + kTileKeys > keys.n || (a.causal && j0 + kTileKeys - 1 > wave_row + shift) ||
-                (window && j0 <= wave_last - window)) {
-                const int from_last = last_seen - j0 - 4 * h;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int j = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3);
-                    if (static_cast<uint32_t>(from_last - j) >= seen) s[i >> 4][i & 15] = -infinity();
-                }
+        for (int tile = tile0; tile < tile1; ++tile) {
+            uint8_t* const here = lds + ((tile - tile0) & 1) * 2 * kTileBytes;
+            uint8_t* const there = lds + (1 - ((tile - tile0) & 1)) * 2 * kTileBytes;
+            if constexpr (DIRECT) {
+                // The tile has come; what this wave read of the last one has arrived,
+                // since the others load over it once they are past the barrier.  (Said
+                // in assembly: after the builtin the compiler made the first LDS read
+                // wait for the loads of the next tile, 8192 tokens 584 us for 557.)
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                wait_counts<vm_wait(0)>();
+                group_barrier();
+                order_fence();
+            } else {
+                __syncthreads();
             }
-            float top = s[0][0];
+            const int j0 = begin + tile * KEYS;
+            // Carefully: such values are taken out of tiles that some row of the workgroup
+            // does not see all of, and added below to the rows that do.
+            if (careful && (j0 + KEYS > keys.n || (a.causal && j0 + KEYS - 1 > row0 + shift) ||
+                            (window && j0 <= last_row + shift - window))) {
+                bool bad = false;
 #pragma unroll
-            for (int i = 1; i < 32; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
-            sums.grow_to(max_of(across_halves(top)) * a.exponent);
-            const float base = sums.base();
-            f16x8 p[4];
+                for (int i = 0; i < kLoads; ++i) {
+                    u32x4* const at = reinterpret_cast<u32x4*>(here + kTileBytes) + threadIdx.x + 256 * i;
+                    const u32x4 x = *at;
+                    u32x4 fine;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], a.exponent, -base));
-                sums.l += e;
-                p[i >> 3][i & 7] = static_cast<_Float16>(e);
-            }
-            // V^T: dimensions 32 i + n, keys 16 c + {4 h .. 4 h + 3, 8 + 4 h ..}.
-#pragma unroll
-            for (int i = 0; i < DT; ++i)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint8_t* at = here + value_at[i] + 16 * CH * 16 * c;
-                    const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * CH * 16);
-                    sums.o[i] = mfma32(__builtin_bit_cast(f16x8, u32x4{lo.x, lo.y, hi.x, hi.y}), p[c], sums.o[i]);
+                    for (int w = 0; w < 4; ++w) fine[w] = finite_of(x[w]);
+                    if (fine[0] != x[0] || fine[1] != x[1] || fine[2] != x[2] || fine[3] != x[3]) {
+                        *at = fine;
+                        bad = true;
+                    }
                 }
-            if (careful && taken_out == tile + 1) {
+                if (bad) taken_out = tile + 1;
+                __syncthreads();
+            }
+            if (tile + 1 < tile1) load_tile(tile + 1, there);
+            if (!(a.causal && (j0 > wave_last || (window && j0 + KEYS - 1 <= wave_row + shift - window)))) {
+                f32x16 s[KEYS / 32];
+#pragma unroll
+                for (int t = 0; t < KEYS / 32; ++t)
+#pragma unroll
+                    for (int i = 0; i < KS; ++i)
+                        s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + key_at[i] + 32 * CH * 16 * t), qf[i],
+                                      i == 0 ? RowSums<DT>::zero() : s[t]);
+                if (j0 + KEYS > keys.n || (a.causal && j0 + KEYS - 1 > wave_row + shift) ||
+                    (window && j0 <= wave_last - window)) {
+                    const int from_last = last_seen - j0 - 4 * h;
+#pragma unroll
+                    for (int i = 0; i < KEYS / 2; ++i) {
+                        const int j = 32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3);
+                        if (static_cast<uint32_t>(from_last - j) >= seen) s[i >> 4][i & 15] = -infinity();
+                    }
+                }
+                float top = s[0][0];
+#pragma unroll
+                for (int i = 1; i < KEYS / 2; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
+                sums.grow_to(max_of(across_halves(top)) * a.exponent);
+                const float base = sums.base();
+                f16x8 p[KEYS / 16];
+#pragma unroll
+                for (int i = 0; i < KEYS / 2; ++i) {
+                    const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], a.exponent, -base));
+                    sums.l += e;
+                    p[i >> 3][i & 7] = static_cast<_Float16>(e);
+                }
+                // V^T: dimensions 32 i + n, keys 16 c + {4 h .. 4 h + 3, 8 + 4 h ..}.
+#pragma unroll
+                for (int i = 0; i < DT; ++i)
+#pragma unroll
+                    for (int c = 0; c < KEYS / 16; ++c) {
+                        const uint8_t* at = here + value_at[i] + 16 * CH * 16 * c;
+                        const u32x2 lo = read_transposed(at), hi = read_transposed(at + 8 * CH * 16);
+                        sums.o[i] = mfma32(__builtin_bit_cast(f16x8, u32x4{lo.x, lo.y, hi.x, hi.y}), p[c], sums.o[i]);
+                    }
+                if (careful && taken_out == tile + 1) {
 #pragma unroll 1
-                for (int j = j0; j < min(j0 + kTileKeys, keys.n); ++j) {
-                    const bool sees = static_cast<uint32_t>(last_seen - j) < seen;
-                    const _Float16* at = v + static_cast<uint64_t>(j) * a.v_stride + 4 * h;
+                    for (int j = j0; j < min(j0 + KEYS, keys.n); ++j) {
+                        const bool sees = static_cast<uint32_t>(last_seen - j) < seen;
+                        const _Float16* at = v + static_cast<uint64_t>(j) * a.v_stride + 4 * h;
 #pragma unroll
-                    for (int i = 0; i < DT; ++i) {
+                        for (int i = 0; i < DT; ++i) {
 #pragma unroll
-                        for (int r = 0; r < 16; r += 4) {
-                            const uint32_t d = 32 * i + 2 * r;
-                            if (!DIRECT && d >= a.head_dim) continue;
-                            const u32x2 four = *reinterpret_cast<const u32x2_a2*>(at + d);
-                            const float x[4] = {half_lo_to_float(four.x), half_hi_to_float(four.x),
-                                                half_lo_to_float(four.y), half_hi_to_float(four.y)};
+                            for (int r = 0; r < 16; r += 4) {
+                                const uint32_t d = 32 * i + 2 * r;
+                                if (!DIRECT && d >= a.head_dim) continue;
+                                const u32x2 four = *reinterpret_cast<const u32x2_a2*>(at + d);
+                                const float x[4] = {half_lo_to_float(four.x), half_hi_to_float(four.x),
+                                                    half_lo_to_float(four.y), half_hi_to_float(four.y)};
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                sums.o[i][r + e] += sees && !(fabsf(x[e]) < infinity()) ? x[e] : 0.0f;
+                                for (int e = 0; e < 4; ++e)
+                                    sums.o[i][r + e] += sees && !(fabsf(x[e]) < infinity()) ? x[e] : 0.0f;
+                            }
+                            order_fence();  // rare, and not to be paid for in registers
                         }
-                        order_fence();  // rare, and not to be paid for in registers
                     }
                 }
             }
+            if (tile + 1 < tile1) store_tile(there);
         }
-        if (tile + 1 < tile1) store_tile(there);
-    }
     };
     walk(std::false_type());
     if (wave_any(!sums.finite())) not_finite = 1;
@@ -356,7 +376,7 @@ struct PromptPlan {
 PromptPlan plan_prompt(uint64_t sequences, uint64_t tokens, uint64_t max_keys, uint64_t heads, uint64_t head_dim) {
     PromptPlan p{};
     p.tiles = units_of(kTileRows, 1, sequences, tokens);
-    p.parts = choose_parts(p.tiles * heads, (max_keys + kTileKeys - 1) / kTileKeys, tokens * heads, head_dim, 1.4, 2.0);
+    p.parts = choose_parts(p.tiles * heads, (max_keys + 63) / 64, tokens * heads, head_dim, 1.4, 2.0);
     return p;
 }
 
@@ -433,16 +453,18 @@ MOTE_EXPORT int mote_hip_prompt_attention_f16(const void* q, const void* k, cons
     a.exponent = exponent;
     const bool direct = !off_grid(k, 16) && !off_grid(v, 16) && k_stride % 8 == 0 && v_stride % 8 == 0 &&
                         k_stride < (uint64_t{1} << 24) && v_stride < (uint64_t{1} << 24);
-    const auto kernel = direct && head_dim == 64    ? prompt_attention_kernel<64, true>
-                        : direct && head_dim == 96  ? prompt_attention_kernel<96, true>
-                        : direct && head_dim == 128 ? prompt_attention_kernel<128, true>
-                        : direct && head_dim == 192 ? prompt_attention_kernel<192, true>
-                        : direct && head_dim == 256 ? prompt_attention_kernel<256, true>
-                        : head_dim <= 64            ? prompt_attention_kernel<64, false>
-                        : head_dim <= 96            ? prompt_attention_kernel<96, false>
-                        : head_dim <= 128           ? prompt_attention_kernel<128, false>
-                        : head_dim <= 192           ? prompt_attention_kernel<192, false>
-                                                    : prompt_attention_kernel<256, false>;
+    const bool many = p.tiles * q_heads >= 1024;
+    const auto kernel = direct && head_dim == 64            ? prompt_attention_kernel<64, true, 64>
+                        : direct && head_dim == 96          ? prompt_attention_kernel<96, true, 64>
+                        : direct && head_dim == 128 && many ? prompt_attention_kernel<128, true, 32>
+                        : direct && head_dim == 128         ? prompt_attention_kernel<128, true, 64>
+                        : direct && head_dim == 192         ? prompt_attention_kernel<192, true, 64>
+                        : direct && head_dim == 256         ? prompt_attention_kernel<256, true, 64>
+                        : head_dim <= 64                    ? prompt_attention_kernel<64, false, 64>
+                        : head_dim <= 96                    ? prompt_attention_kernel<96, false, 64>
+                        : head_dim <= 128                   ? prompt_attention_kernel<128, false, 64>
+                        : head_dim <= 192                   ? prompt_attention_kernel<192, false, 64>
+                                                            : prompt_attention_kernel<256, false, 64>;
     const auto s = static_cast<hipStream_t>(stream);
     constexpr uint64_t kMostZ = 65535;
     for (uint64_t first = 0; first < p.tiles * p.parts; first += kMostZ) {

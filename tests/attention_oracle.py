@@ -32,22 +32,23 @@ def attend(q, k, v, scale, causal=True, window=0):
         sees = j <= at
         if window:
             sees &= j > at - window
+    some = sees.any(1)
+    if not some.any():
+        return o, bound
+    mask = sees[some]
     for h in range(heads):
         kh, vh = k[:, h // group], v[:, h // group]
-        with np.errstate(all="ignore"):
-            s = (q[:, h] @ kh.T) * scale
-            size = (np.abs(q[:, h]) @ np.abs(kh).T) * scale
-            for i in range(n):
-                m = sees[i]
-                if not m.any():
-                    continue
-                x = s[i, m]
-                w = np.exp(x - x.max())
-                w /= w.sum()
-                o[i, h] = w @ vh[m]
-                reach = w @ np.abs(vh[m]) + 2.0**-33 * m.sum() * np.abs(vh[m]).max()
-                off = (d * size[i, m].max() + 3 * np.abs(x).max() + 3) * 2.0**-23
-                bound[i, h] = 2.0**-11 * np.abs(o[i, h]) + reach * (2.0**-11 + 2 * off + t * 2.0**-23) + 2.0**-24
+        s = np.where(mask, (q[some, h] @ kh.T) * scale, -np.inf)
+        size = np.where(mask, (np.abs(q[some, h]) @ np.abs(kh).T) * scale, 0.0).max(1)
+        most = np.abs(np.where(mask, s, 0.0)).max(1)
+        w = np.exp(s - s.max(1, keepdims=True))
+        w /= w.sum(1, keepdims=True)
+        o[some, h] = w @ vh
+        large = np.stack([np.abs(vh[m]).max() for m in mask]) if window else np.maximum.accumulate(
+            np.abs(vh).max(1))[mask.shape[1] - 1 - mask[:, ::-1].argmax(1)]
+        reach = w @ np.abs(vh) + (2.0**-33 * mask.sum(1) * large)[:, None]
+        off = ((d * size + 3 * most + 3) * 2.0**-23)[:, None]
+        bound[some, h] = 2.0**-11 * np.abs(o[some, h]) + reach * (2.0**-11 + 2 * off + t * 2.0**-23) + 2.0**-24
     return o, bound
 
 

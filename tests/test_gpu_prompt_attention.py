@@ -120,6 +120,31 @@ def test_packed(stream, queries, keys):
     check(stream, len(queries), queries, keys, 2, 1, 64)
 
 
+@pytest.mark.parametrize("how", [dict(), dict(causal=False), dict(window=1), dict(window=33), dict(window=64)])
+def test_many_workgroups(stream, how):
+    """More than a thousand, which take shorter tiles of keys."""
+    queries = [1, 31, 32, 33, 0, 64, 65, 130]
+    check(stream, 12, queries, [1, 40, 32, 95, 5, 64, 65, 200], 128, 4, 128, **how)
+
+
+def test_many_workgroups_not_finite_where_not_seen(stream):
+    queries = [130, 60, 60, 60, 60, 60, 60]
+    q, k, v = tensors(13, queries, queries, 128, 2, 128)
+    clean = Call(q, k, v, queries, queries)
+    clean.run(stream)
+    want = clean.result(stream)
+    k[100, 0], v[101, 0, 3], v[180, 1, 5] = np.nan, np.inf, np.nan
+    call = Call(q, k, v, queries, queries)
+    call.run(stream)
+    got = call.result(stream)
+    touched = np.zeros(got.shape, bool)
+    touched[100:130, :64] = True
+    touched[101:130, :64, 3] = True
+    touched[180:190, 64:, 5] = True
+    assert (got.view(np.uint16) == want.view(np.uint16))[~touched].all()
+    assert np.isnan(got[touched]).all()
+
+
 @pytest.mark.parametrize("count", [4097, 70000])
 def test_very_many_sequences(stream, count):
     """Of one token each (whose attention is its value) and now and then five: three
