@@ -419,9 +419,9 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
         if (j0 <= wave_last && !(window && j0 + 63 <= wave_first - window)) {
             f32x16 s[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int i = 0; i < KS; ++i)
 #pragma unroll
-                for (int i = 0; i < KS; ++i)
+                for (int t = 0; t < 2; ++t)
                     s[t] = mfma32(*reinterpret_cast<const f16x8*>(here + ((t * KS + i) * 64 + lane) * 16), qf[i],
                                   i == 0 ? RowSums<CT>::zero() : s[t]);
             // Exponents are s factor + more: see the few rows' kernel for the values' scale.
@@ -469,9 +469,9 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
                 sums.l = __builtin_fmaf(sum, less[t], sums.l);
             }
 #pragma unroll
-            for (int i = 0; i < CT; ++i)
+            for (int c = 0; c < 4; ++c)
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int i = 0; i < CT; ++i)
                     sums.o[i] = mfma32(*reinterpret_cast<const f16x8*>(here + kTileBytes +
                                                                        (((c >> 1) * KS + 2 * i + (c & 1)) * 64 + lane) * 16),
                                        p[c], sums.o[i]);
