@@ -435,3 +435,24 @@ def test_repeats_streams_and_graphs_agree(stream):
         call.run(stream)
         stream.synchronize()
     hip.destroy_graph(graph)
+
+
+def test_graph_replayed_with_other_lengths(stream):
+    """Only the sizes given by the host divide the work: what a graph holds stays
+    right as the lengths on the device change."""
+    hip = HipRuntime()
+    held, q = setup(18, [1, 1, 1], [2000, 1500, 700], 8, 2, 64)
+    call = Attend(held, q, [1, 1, 1], [2000, 1500, 700], single=True)
+    call.run(stream)
+    call.result(stream)
+    graph = hip.capture(stream, lambda: call.run(stream))
+    for lengths in ([2000, 1500, 700], [1, 33, 0], [64, 1999, 1000]):
+        call.lengths.upload(ints(lengths))
+        call.run(stream)
+        eager = call.result(stream).copy()
+        call.out.upload(np.full(call.out.nbytes // 2, 0x7A7A, np.uint16))
+        hip.launch_graph(graph, stream)
+        assert (call.result(stream).view(np.uint16) == eager.view(np.uint16)).all()
+        o, bound = expected(held, q, [1, 1, 1], lengths)
+        assert_within(eager, o, bound)
+    hip.destroy_graph(graph)
