@@ -11,13 +11,13 @@
 // V^T, comes out of the row-major tile through LDS transpose reads.
 //
 // 64 x 32 scores of 128 dimensions are 32 matrix instructions (1024 cycles) and
-// about 150 vector instructions, a fifth of them exponentials (1050 cycles); two
-// workgroups a compute unit run the one under the other.  1 x 8192 tokens, 32 heads
-// of 128, causal: 557 us, 990 TFLOP/s (a large library product here: 1175), the
-// matrix cores busy 54 % of the cycles at the 1.78 GHz that the card's power leaves;
-// two tiles of a compute unit take 3450 cycles, 2048 of them matrix instructions.
-// Short prompts wait for their starts: 6300 cycles before a workgroup's first
-// product, 24 prompts of up to 1000 tokens 123 us, 550 TFLOP/s.
+// about 150 vector instructions, a fifth of them exponentials (1050 cycles); the
+// workgroups of a compute unit run the one under the other.  1 x 8192 tokens, 32 heads
+// of 128, causal: 557 to 590 us by the card, 930 to 990 TFLOP/s (a large library
+// product: 1175).  Power bounds it: the matrix cores are busy 60 % of the cycles, of
+// which the card gives 1.5 GHz over the launch (1.9 in light ones).  Short prompts wait
+// for their starts: 6300 cycles before a workgroup's first product, 24 prompts of up to
+// 1000 tokens 126 us, 540 TFLOP/s.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
