@@ -297,8 +297,9 @@ cache_attention_kernel(CacheAttentionArgs a) {
 // 32 x 32 x 16 instruction; the planes' order makes both operands of a lane 16
 // consecutive bytes of LDS, key row 16 c + 8 b + 4 h + r of a tile being token
 // 16 b + 8 c + 4 h + r of the block.  512 queries of 32 heads over 8192 tokens of 8
-// key heads of 128: 96 us, 695 TFLOP/s (in 16-row tiles 243), 10 of them the join of
-// four parts; matrix cores busy 36 % and vector ALUs 49 % of the cycles.
+// key heads of 128: 95 us, 700 TFLOP/s (in 16-row tiles 243), 10 of them the join of
+// four parts; matrix cores busy 38 % and vector ALUs 51 % of the cycles.  (The next
+// tile's scores under this one's weights, with two tiles' in registers: 99.)
 // CT: 32-dimension groups there is room for.
 constexpr uint32_t kTileRows = 128;
 
