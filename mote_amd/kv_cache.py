@@ -12,6 +12,8 @@ or cannot wait keeps its own on the device and calls ``mote_amd.ops`` directly.
 
 from __future__ import annotations
 
+import operator
+
 import numpy as np
 
 from . import ops
@@ -21,6 +23,12 @@ from .device import DeviceBuffer
 
 class CacheFull(RuntimeError):
     """The pool has no block left, or a sequence no room in its table."""
+
+
+def _integers(values) -> list[int]:
+    """A call's numbers, in whatever form they come (numpy takes a tuple of two
+    indices for a row and a column)."""
+    return [operator.index(v) for v in values]
 
 
 class BlockTable:
@@ -103,6 +111,7 @@ class KVCacheQ8:
 
     ``k``, ``v``, ``q`` and ``out`` are device addresses of packed f16 rows: the
     rows of ``sequences[0]`` first, ``counts[0]`` of them, and so on.
+    ``sequences``, ``counts`` and ``first`` are integers in any iterable.
     """
 
     def __init__(self, blocks: int, kv_heads: int, head_dim: int, max_sequences: int, max_context: int) -> None:
@@ -132,16 +141,18 @@ class KVCacheQ8:
 
     def append(self, sequences, k: int, v: int, counts, stream, strides=None) -> None:
         """The next counts[i] tokens of sequences[i]."""
+        sequences, counts = _integers(sequences), _integers(counts)
         if len(sequences) != len(counts):
             raise ValueError("one count for each sequence")
         self.blocks.reserve(sequences, counts)
         self._upload(sequences, counts, self.blocks.lengths[sequences], stream)
         ops.kv_cache_append_q8(k, v, self._offsets.ptr, self._second.ptr, self._table.ptr, self.cache.ptr,
-                               self.scales.ptr, len(sequences), int(sum(counts)), *self._shape(), stream, strides)
+                               self.scales.ptr, len(sequences), sum(counts), *self._shape(), stream, strides)
         self.blocks.advance(sequences, counts)
 
     def read(self, sequences, k: int, v: int, counts, first, stream, strides=None) -> None:
         """counts[i] tokens of sequences[i] from first[i] on, in f16."""
+        sequences, counts, first = _integers(sequences), _integers(counts), _integers(first)
         if not len(sequences) == len(counts) == len(first):
             raise ValueError("one count and one first token for each sequence")
         self.blocks._known(sequences)
@@ -150,13 +161,14 @@ class KVCacheQ8:
                 raise ValueError(f"sequence {s} holds {self.blocks.lengths[s]} tokens")
         self._upload(sequences, counts, first, stream)
         ops.kv_cache_read_q8_f16(self.cache.ptr, self.scales.ptr, self._offsets.ptr, self._second.ptr,
-                                 self._table.ptr, k, v, len(sequences), int(sum(counts)), *self._shape(), stream,
+                                 self._table.ptr, k, v, len(sequences), sum(counts), *self._shape(), stream,
                                  strides)
 
     def attend(self, sequences, q: int, out: int, q_heads: int, counts, stream, scale=None, window: int = 0,
                strides=None) -> None:
         """Attention of the last counts[i] tokens of sequences[i], their own keys
         already appended.  `scale` None: 1 / sqrt(head_dim)."""
+        sequences, counts = _integers(sequences), _integers(counts)
         if len(sequences) != len(counts):
             raise ValueError("one count for each sequence")
         self.blocks._known(sequences)
@@ -167,7 +179,7 @@ class KVCacheQ8:
         if not len(sequences) or not sum(counts):
             return
         self._upload(sequences, counts, lengths, stream)
-        shape = (len(sequences), int(sum(counts)), int(max(counts)), int(lengths.max()), q_heads, self.kv_heads,
+        shape = (len(sequences), sum(counts), max(counts), int(lengths.max()), q_heads, self.kv_heads,
                  self.head_dim)
         need = ops.cache_attention_workspace(*shape)
         if need > self._workspace.nbytes:  # nothing uses the old one: the upload has waited
