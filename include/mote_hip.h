@@ -306,7 +306,8 @@ int mote_hip_rope_tables_f32(const void* positions, void* cos_out, void* sin_out
  * `workspace` (16-byte aligned, at least the bytes that
  * mote_hip_prompt_attention_workspace says for the same sizes, which may be 0);
  * it holds nothing between calls.  The output may be q itself (same stride), and
- * must not overlap k or v.  Offsets that run past the rows there are cut to them.
+ * must not overlap k or v.  Offsets that run past the rows there are cut to them;
+ * output rows that no sequence owns are left as they are.
  * Nothing is allocated, and a call can be captured.
  * Status: 0; -1 for a null pointer (key_offsets, and a workspace of which 0 bytes
  * are needed, excepted), an odd f16 or misaligned offsets address, head_dim not a
@@ -378,7 +379,8 @@ int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* scales, const v
  * strides, types, rows that see nothing, workspace and statuses as for the prompt
  * attention above, with the cache's values (u - 128) x scale for k and v; the
  * cache's own requirements as for append.  max_queries: at least the largest n
- * (rows past it are not computed); max_context: at least the largest length (it
+ * (the output rows of a sequence's queries past it, like those that no sequence
+ * owns, are left as they are); max_context: at least the largest length (it
  * only chooses how the work is divided).  query_offsets NULL needs query_tokens =
  * sequences and max_queries = 1.  Blocks whose number is not below cache_blocks
  * count as not there.  A plane whose scale is NaN makes every query NaN that

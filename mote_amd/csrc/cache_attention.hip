@@ -38,7 +38,8 @@ struct CacheAttentionArgs {
     float2* stats;  // null: one part, written to output
     float* sums;
     uint64_t q_stride, out_stride;
-    uint32_t sequences, tokens, row_tiles, heads, kv_heads, head_dim, table_blocks, cache_blocks, window, chunk, parts;
+    uint32_t sequences, tokens, max_queries, row_tiles, heads, kv_heads, head_dim;
+    uint32_t table_blocks, cache_blocks, window, chunk, parts;
     float exponent;  // scale log2(e)
 };
 
@@ -85,12 +86,14 @@ cache_attention_kernel(CacheAttentionArgs a) {
     const int n = lane & 15, g = lane >> 4;
     const uint32_t group = a.heads / a.kv_heads;
     Span rows = {static_cast<int>(seq), 1};
-    if (a.offsets != nullptr) rows = span_of(a.offsets, seq, a.tokens);
-    const uint32_t row0 = row_tile * kRows, all_rows = static_cast<uint32_t>(rows.n) * group;
+    if (a.offsets != nullptr) rows = scalar_span_of(a.offsets, seq, a.tokens);
+    if (a.stats != nullptr && part == 0 && row_tile == 0)
+        mark_not_computed(a.stats, rows, seq, a.sequences, a.tokens, a.max_queries, a.heads, kv_head * group, group);
+    const uint32_t row0 = row_tile * kRows, all_rows = min(static_cast<uint32_t>(rows.n), a.max_queries) * group;
     if (row0 >= all_rows) return;
     const uint32_t here = min(all_rows - row0, static_cast<uint32_t>(kRows));
     const int most_length = static_cast<int>(a.table_blocks * kBlockTokens);
-    const int length = min(max(a.lengths[seq], 0), most_length);
+    const int length = min(max(scalar_load(a.lengths + seq), 0), most_length);
     const int shift = length - rows.n;  // position of the first query; below 0: it sees nothing
     const int first_token = static_cast<int>(row0 / group), last_token = static_cast<int>((row0 + here - 1) / group);
     // Blocks that any of the rows sees: [b0, b1)
@@ -141,14 +144,14 @@ cache_attention_kernel(CacheAttentionArgs a) {
         float key_scale, value_scale;
         bool there;
     };
-    const auto number = [&](int b) { return b < b1 ? table[b] : -1; };
+    const auto number = [&](int b) { return b < b1 ? scalar_load(table + b) : -1; };
     const auto place_of = [&](int32_t block) {
         Place f;
         f.there = block >= 0 && static_cast<uint32_t>(block) < a.cache_blocks;
         const uint64_t at = static_cast<uint64_t>(f.there ? block : 0) * a.kv_heads + kv_head;
         f.planes = a.cache + at * (2 * kPlane) + lane * 16;
-        f.key_scale = a.scales[at * 2];
-        f.value_scale = a.scales[at * 2 + 1];
+        f.key_scale = scalar_load(a.scales + at * 2);
+        f.value_scale = scalar_load(a.scales + at * 2 + 1);
         return f;
     };
     u32x4 kb[C], vb[C];
@@ -322,10 +325,12 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
     const int n = lane & 31, h = lane >> 5;
     const uint32_t group = a.heads / a.kv_heads, groups = padded_dim(a.head_dim) / 32;
     Span rows = {static_cast<int>(seq), 1};
-    if (a.offsets != nullptr) rows = span_of(a.offsets, seq, a.tokens);
-    const uint32_t row0 = row_tile * kTileRows, all_rows = static_cast<uint32_t>(rows.n) * group;
+    if (a.offsets != nullptr) rows = scalar_span_of(a.offsets, seq, a.tokens);
+    if (a.stats != nullptr && part == 0 && row_tile == 0)
+        mark_not_computed(a.stats, rows, seq, a.sequences, a.tokens, a.max_queries, a.heads, kv_head * group, group);
+    const uint32_t row0 = row_tile * kTileRows, all_rows = min(static_cast<uint32_t>(rows.n), a.max_queries) * group;
     if (row0 >= all_rows) return;
-    const int length = min(max(a.lengths[seq], 0), static_cast<int>(a.table_blocks * kBlockTokens));
+    const int length = min(max(scalar_load(a.lengths + seq), 0), static_cast<int>(a.table_blocks * kBlockTokens));
     const int shift = length - rows.n;  // position of the first query
     const int window = static_cast<int>(a.window);
     const auto position = [&](uint32_t r) { return shift + static_cast<int>(min(r, all_rows - 1) / group); };
@@ -354,11 +359,11 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const int b = begin / 32 + 2 * tile + t;
-            const int32_t block = table[min(b, last_block)];
+            const int32_t block = scalar_load(table + min(b, last_block));
             f.there[t] = b <= last_block && block >= 0 && static_cast<uint32_t>(block) < a.cache_blocks;
             at[t] = static_cast<uint64_t>(f.there[t] ? block : 0) * a.kv_heads + kv_head;
-            f.key[t] = a.scales[at[t] * 2];
-            f.value[t] = a.scales[at[t] * 2 + 1];
+            f.key[t] = scalar_load(a.scales + at[t] * 2);
+            f.value[t] = scalar_load(a.scales + at[t] * 2 + 1);
         }
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
@@ -624,6 +629,7 @@ MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache
     a.out_stride = output_stride;
     a.sequences = static_cast<uint32_t>(sequences);
     a.tokens = static_cast<uint32_t>(query_tokens);
+    a.max_queries = static_cast<uint32_t>(max_queries);
     a.row_tiles = p.row_tiles;
     a.heads = static_cast<uint32_t>(q_heads);
     a.kv_heads = static_cast<uint32_t>(kv_heads);

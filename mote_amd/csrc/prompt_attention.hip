@@ -115,6 +115,8 @@ prompt_attention_kernel(PromptArgs a) {
     if (!u.found) return;
     queries = span_at(queries, u.lane);
     keys = span_at(keys, u.lane);
+    if (a.stats != nullptr && part == 0 && u.local == 0)
+        mark_not_computed(a.stats, queries, u.sequence, a.sequences, a.tokens, a.tokens, a.heads, head, 1);
     const uint32_t row_tiles = (static_cast<uint32_t>(queries.n) + kTileRows - 1) / kTileRows;
     if (u.local >= row_tiles) return;  // room that the sequence does not need
     const int row0 = static_cast<int>((row_tiles - 1 - u.local) * kTileRows);  // the longest walks first
