@@ -40,6 +40,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLeastFactor = 0x1p-100f;  // of scores: a masked one stays -inf, others vanish
 constexpr float kLeastScale = 0x1p-64f;  // of values: times 127 far below binary16, and its inverse in range
 
+// Between a wave's own writes to LDS and what its other lanes read there.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ float infinity() { return __builtin_inff(); }
 
@@ -197,6 +204,7 @@ struct RowSums {
                 *reinterpret_cast<u32x2*>(chunk(n, 4 * i + r / 4) + 8 * h) =
                     u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
             }
+        wave_lds_fence();
 #pragma unroll
         for (int j = 0; j < CH / 2; ++j) {
             const int row = (64 * j + lane) / CH, c = (64 * j + lane) % CH;
@@ -286,9 +294,7 @@ __global__ __launch_bounds__(256) void parts_join_kernel(const float2* __restric
     const float weight = ml.y == 0.0f ? 0.0f : ml.x == -infinity() ? ml.y : exp2_fast(ml.x - top);
     float l = wave_sum(weight * ml.y);
     weights[wave][lane] = weight;  // read by this wave alone
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    wave_lds_fence();
     f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
     for (uint32_t s0 = 0; s0 < mine; s0 += 4 * at_once) {
         if (s0 != 0) load(s0);
