@@ -384,7 +384,9 @@ int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* scales, const v
  * only chooses how the work is divided).  query_offsets NULL needs query_tokens =
  * sequences and max_queries = 1.  Blocks whose number is not below cache_blocks
  * count as not there.  A plane whose scale is NaN makes every query NaN that
- * sees one of its tokens.  Nothing is allocated, and a call can be captured. */
+ * sees one of its tokens.  Nothing is allocated, and a call can be captured.
+ * Status -1 also for more than 2^32 - 1 workgroups, of which a sequence takes at
+ * most one for each key head, 16 rows (queries x heads of the key head) and part. */
 int mote_hip_cache_attention_workspace(uint64_t sequences, uint64_t query_tokens, uint64_t max_queries,
                                        uint64_t max_context, uint64_t q_heads, uint64_t kv_heads,
                                        uint64_t head_dim, size_t* bytes);

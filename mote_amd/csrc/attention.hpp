@@ -22,7 +22,8 @@ constexpr int kInvalid = -1;
 constexpr uint32_t kBlockTokens = 32;             // tokens of a cache block
 constexpr uint64_t kMostTokens = uint64_t{1} << 30;  // int32 offsets, with room for a window's
 constexpr uint64_t kMostHeadDim = 256;
-constexpr uint64_t kMostGrid = (uint64_t{1} << 32) / 256 - 1;  // workgroups of 256 threads in one launch
+// Workgroups of so many threads in one launch, whose threads are counted in 32 bits.
+constexpr uint64_t most_groups(uint64_t threads) { return 0xFFFFFFFFu / threads; }
 
 __host__ __device__ constexpr uint32_t padded_dim(uint32_t d) { return (d + 31u) & ~31u; }
 
@@ -263,13 +264,14 @@ __device__ __forceinline__ void mark_not_computed(float2* stats, Span rows, uint
 template <int W>
 __global__ __launch_bounds__(256) void parts_join_kernel(const float2* __restrict__ stats,
                                                          const float* __restrict__ sums, _Float16* output,
-                                                         uint32_t rows, uint32_t parts, uint32_t heads,
-                                                         uint32_t head_dim, uint32_t lanes, uint64_t out_stride) {
+                                                         uint32_t rows, uint32_t first_row, uint32_t parts,
+                                                         uint32_t heads, uint32_t head_dim, uint32_t lanes,
+                                                         uint64_t out_stride) {
     __shared__ __align__(16) float joined[W == 1 ? 1 : 4][W == 1 ? 4 : 256];
     __shared__ float2 joined_stats[4];
     __shared__ float weights[4][64];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t row = W == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+    const uint32_t row = first_row + (W == 1 ? blockIdx.x * 4 + wave : blockIdx.x);
     if (row >= rows) return;
     const uint32_t share = (parts + W - 1) / W, first = W == 1 ? 0 : wave * share;
     const uint32_t mine = first < parts ? min(share, parts - first) : 0;
@@ -372,12 +374,18 @@ inline int join_parts(const void* workspace, void* output, uint64_t rows, uint32
     while (lanes * 4 < head_dim) lanes *= 2;
     const bool many = parts > 8;
     const auto kernel = many ? parts_join_kernel<4> : parts_join_kernel<1>;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(many ? rows : (rows + 3) / 4)), dim3(256), 0, stream,
-                       static_cast<const float2*>(workspace),
-                       reinterpret_cast<const float*>(static_cast<const char*>(workspace) + stats_bytes(rows, parts)),
-                       static_cast<_Float16*>(output), static_cast<uint32_t>(rows), parts,
-                       static_cast<uint32_t>(heads), static_cast<uint32_t>(head_dim), lanes, out_stride);
-    return static_cast<int>(hipGetLastError());
+    const uint64_t per = many ? 1 : 4, most = most_groups(256) * per;
+    for (uint64_t first = 0; first < rows; first += most) {
+        const uint64_t now = rows - first < most ? rows - first : most;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((now + per - 1) / per)), dim3(256), 0, stream,
+                           static_cast<const float2*>(workspace),
+                           reinterpret_cast<const float*>(static_cast<const char*>(workspace) + stats_bytes(rows, parts)),
+                           static_cast<_Float16*>(output), static_cast<uint32_t>(rows), static_cast<uint32_t>(first),
+                           parts, static_cast<uint32_t>(heads), static_cast<uint32_t>(head_dim), lanes, out_stride);
+        const int status = static_cast<int>(hipGetLastError());
+        if (status != 0) return status;
+    }
+    return 0;
 }
 
 inline bool odd_address(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 1) != 0; }

@@ -39,7 +39,7 @@ struct CacheAttentionArgs {
     float* sums;
     uint64_t q_stride, out_stride;
     uint32_t sequences, tokens, max_queries, row_tiles, heads, kv_heads, head_dim;
-    uint32_t table_blocks, cache_blocks, window, chunk, parts;
+    uint32_t table_blocks, cache_blocks, window, chunk, parts, first;
     float exponent;  // scale log2(e)
 };
 
@@ -75,7 +75,7 @@ cache_attention_kernel(CacheAttentionArgs a) {
     __shared__ __align__(16) float sums_of[WAVES][kRows][kRowFloats];
     __shared__ float2 stats_of[WAVES][kRows];
 
-    uint32_t id = blockIdx.x;
+    uint32_t id = a.first + blockIdx.x;
     const uint32_t part = id % a.parts;
     id /= a.parts;
     const uint32_t kv_head = id % a.kv_heads;
@@ -314,7 +314,7 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
     constexpr int kLoads = (2 * 64 * CT + 255) / 256;  // 16-byte chunks of a thread in two planes
     __shared__ __align__(1024) uint8_t lds[4 * kTileBytes];  // two of [keys | values]
 
-    uint32_t id = blockIdx.x;
+    uint32_t id = a.first + blockIdx.x;
     const uint32_t kv_head = id % a.kv_heads;
     id /= a.kv_heads;
     const uint32_t part = id % a.parts;
@@ -612,7 +612,7 @@ MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache
     const uint64_t rows = query_tokens * q_heads;
     const uint64_t need = parts_bytes(rows, p.parts, head_dim);
     if (need > 0 && (!workspace || off_grid(workspace, 16) || workspace_bytes < need)) return kInvalid;
-    if (sequences * p.row_tiles > kMostGrid / kv_heads / p.parts) return kInvalid;
+    if (sequences * p.row_tiles > 0xFFFFFFFFu / kv_heads / p.parts) return kInvalid;  // workgroups: 32 bits
     CacheAttentionArgs a{};
     a.q = static_cast<const _Float16*>(q);
     a.cache = static_cast<const uint8_t*>(cache);
@@ -642,9 +642,14 @@ MOTE_EXPORT int mote_hip_cache_attention_q8_f16(const void* q, const void* cache
     a.exponent = exponent;
     const auto kernel = kernel_of(p.tile_rows, padded_dim(a.head_dim) / 32);
     const auto s = static_cast<hipStream_t>(stream);
-    const uint64_t groups = sequences * p.row_tiles * kv_heads * p.parts;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(64 * p.waves), 0, s, a);
-    const int status = static_cast<int>(hipGetLastError());
-    if (status != 0 || p.parts <= 1) return status;
+    const uint64_t groups = sequences * p.row_tiles * kv_heads * p.parts, most = most_groups(64 * p.waves);
+    for (uint64_t first = 0; first < groups; first += most) {
+        a.first = static_cast<uint32_t>(first);
+        const uint64_t now = groups - first < most ? groups - first : most;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(now)), dim3(64 * p.waves), 0, s, a);
+        const int status = static_cast<int>(hipGetLastError());
+        if (status != 0) return status;
+    }
+    if (p.parts <= 1) return 0;
     return join_parts(workspace, output, rows, p.parts, q_heads, head_dim, output_stride, s);
 }

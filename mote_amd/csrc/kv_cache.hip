@@ -359,7 +359,7 @@ MOTE_EXPORT int mote_hip_kv_cache_append_q8(const void* k, const void* v, const 
                                     head_dim, table_blocks, cache_blocks, stream);
     if (go != 1) return go;
     const uint64_t pieces = units_of(kBlockTokens, 2, sequences, tokens);
-    if (pieces > kMostGrid) return kInvalid;
+    if (pieces > most_groups(256)) return kInvalid;
     const CacheArgs a{static_cast<const int32_t*>(offsets), static_cast<const int32_t*>(positions),
                       static_cast<const int32_t*>(block_table), static_cast<uint8_t*>(cache),
                       static_cast<float*>(scales), static_cast<_Float16*>(const_cast<void*>(k)),
@@ -384,7 +384,7 @@ MOTE_EXPORT int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* sca
     if (go != 1) return go;
     if (k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim) return kInvalid;
     const uint64_t pieces = units_of(kBlockTokens, 2, sequences, tokens);
-    if (pieces > kMostGrid) return kInvalid;
+    if (pieces > most_groups(256)) return kInvalid;
     const CacheArgs a{static_cast<const int32_t*>(offsets), static_cast<const int32_t*>(positions),
                       static_cast<const int32_t*>(block_table), static_cast<uint8_t*>(const_cast<void*>(cache)),
                       static_cast<float*>(const_cast<void*>(scales)), static_cast<_Float16*>(k),
