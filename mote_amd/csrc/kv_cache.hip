@@ -37,7 +37,7 @@ struct CacheArgs {
     _Float16* k;
     _Float16* v;
     uint64_t k_stride, v_stride;  // elements between packed rows
-    uint32_t sequences, tokens, heads, head_dim, table_blocks, cache_blocks;
+    uint32_t sequences, tokens, heads, head_dim, table_blocks, cache_blocks, first;  // first: unit of the launch
 };
 
 // The part of a sequence's rows that lies in one block.
@@ -223,7 +223,7 @@ __global__ __launch_bounds__(256) void append_kernel(CacheArgs a) {
     __shared__ __align__(16) uint8_t stage[kBlockTokens * stage_row(CHUNKS)];
     __shared__ uint32_t most_of[2][4];
     const uint32_t head = blockIdx.y;
-    const Piece p = piece_of(a, blockIdx.x, head);
+    const Piece p = piece_of(a, a.first + blockIdx.x, head);
     if (!p.found) return;
     const float old_k = p.from != 0 ? a.scales[p.planes] : 0.0f, old_v = p.from != 0 ? a.scales[p.planes + 1] : 0.0f;
     const uint32_t t = threadIdx.x >> 3, sub = threadIdx.x & 7, chunks = a.head_dim / 8;
@@ -272,7 +272,7 @@ __global__ __launch_bounds__(256) void read_kernel(CacheArgs a) {
     constexpr uint32_t kMostRow = kMostHeadDim + 8;  // rows 16 bytes past a multiple of the banks
     __shared__ __align__(16) _Float16 rows[kBlockTokens * kMostRow];
     const uint32_t head = blockIdx.y;
-    const Piece p = piece_of(a, blockIdx.x, head);
+    const Piece p = piece_of(a, a.first + blockIdx.x, head);
     if (!p.found) return;
     const uint32_t padded = padded_dim(a.head_dim), loads = kBlockTokens * padded / 16, row = padded + 8;
     const float scale_k = a.scales[p.planes], scale_v = a.scales[p.planes + 1];
@@ -346,6 +346,20 @@ int check_cache_call(const void* k, const void* v, const void* offsets, const vo
     return 1;
 }
 
+// A workgroup for each piece there is room for and each head.
+int launch_pieces(void (*kernel)(CacheArgs), CacheArgs a, void* stream) {
+    const uint64_t pieces = units_of(kBlockTokens, 2, a.sequences, a.tokens), most = most_groups(256);
+    for (uint64_t first = 0; first < pieces; first += most) {
+        a.first = static_cast<uint32_t>(first);
+        const uint64_t now = pieces - first < most ? pieces - first : most;
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(now), a.heads), dim3(256), 0,
+                           static_cast<hipStream_t>(stream), a);
+        const int status = static_cast<int>(hipGetLastError());
+        if (status != 0) return status;
+    }
+    return 0;
+}
+
 }  // namespace
 }  // namespace mote::attention
 
@@ -358,19 +372,15 @@ MOTE_EXPORT int mote_hip_kv_cache_append_q8(const void* k, const void* v, const 
     const int go = check_cache_call(k, v, offsets, positions, block_table, cache, scales, sequences, tokens, kv_heads,
                                     head_dim, table_blocks, cache_blocks, stream);
     if (go != 1) return go;
-    const uint64_t pieces = units_of(kBlockTokens, 2, sequences, tokens);
-    if (pieces > most_groups(256)) return kInvalid;
     const CacheArgs a{static_cast<const int32_t*>(offsets), static_cast<const int32_t*>(positions),
                       static_cast<const int32_t*>(block_table), static_cast<uint8_t*>(cache),
                       static_cast<float*>(scales), static_cast<_Float16*>(const_cast<void*>(k)),
                       static_cast<_Float16*>(const_cast<void*>(v)), k_stride, v_stride,
                       static_cast<uint32_t>(sequences), static_cast<uint32_t>(tokens), static_cast<uint32_t>(kv_heads),
                       static_cast<uint32_t>(head_dim), static_cast<uint32_t>(table_blocks),
-                      static_cast<uint32_t>(cache_blocks)};
+                      static_cast<uint32_t>(cache_blocks), 0};
     const auto kernel = head_dim <= 64 ? append_kernel<1> : head_dim <= 128 ? append_kernel<2> : append_kernel<4>;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(kv_heads)), dim3(256),
-                       0, static_cast<hipStream_t>(stream), a);
-    return static_cast<int>(hipGetLastError());
+    return launch_pieces(kernel, a, stream);
 }
 
 MOTE_EXPORT int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* scales, const void* offsets,
@@ -383,15 +393,11 @@ MOTE_EXPORT int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* sca
                                     head_dim, table_blocks, cache_blocks, stream);
     if (go != 1) return go;
     if (k_stride < kv_heads * head_dim || v_stride < kv_heads * head_dim) return kInvalid;
-    const uint64_t pieces = units_of(kBlockTokens, 2, sequences, tokens);
-    if (pieces > most_groups(256)) return kInvalid;
     const CacheArgs a{static_cast<const int32_t*>(offsets), static_cast<const int32_t*>(positions),
                       static_cast<const int32_t*>(block_table), static_cast<uint8_t*>(const_cast<void*>(cache)),
                       static_cast<float*>(const_cast<void*>(scales)), static_cast<_Float16*>(k),
                       static_cast<_Float16*>(v), k_stride, v_stride, static_cast<uint32_t>(sequences),
                       static_cast<uint32_t>(tokens), static_cast<uint32_t>(kv_heads), static_cast<uint32_t>(head_dim),
-                      static_cast<uint32_t>(table_blocks), static_cast<uint32_t>(cache_blocks)};
-    hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(pieces), static_cast<unsigned>(kv_heads)), dim3(256),
-                       0, static_cast<hipStream_t>(stream), a);
-    return static_cast<int>(hipGetLastError());
+                      static_cast<uint32_t>(table_blocks), static_cast<uint32_t>(cache_blocks), 0};
+    return launch_pieces(read_kernel, a, stream);
 }

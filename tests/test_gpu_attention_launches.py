@@ -38,3 +38,36 @@ def test_cache_attention_of_half_a_million_sequences(stream):
         k, v = (host.values(w, table[s], lengths[s]).astype(np.float64) for w in (0, 1))
         o, bound = attend(q[s:s + 1], k, v, d ** -0.5)
         assert_within(got[s:s + 1], o, bound, f"sequence {s}")
+
+
+def test_cache_writes_and_reads_of_eight_million_sequences(stream):
+    """One token each: more than the 16 777 215 workgroups of 256 threads a launch has
+    room for.  Blocks for the first, the last and some between; the others have none."""
+    rng = np.random.default_rng(2)
+    sequences, heads, d = (1 << 23) + 9, 1, 8
+    held = np.unique(np.concatenate([np.arange(20), sequences - 1 - np.arange(20), rng.integers(0, sequences, 60)]))
+    host = Cache(len(held), heads, d, rng)
+    table = np.full((sequences, 1), -1, np.int32)
+    table[held, 0] = rng.permutation(len(held))
+    positions = rng.integers(0, BLOCK, sequences).astype(np.int32)
+    k, v = (rng.standard_normal((sequences, heads, d), dtype=np.float32).astype(np.float16) for _ in range(2))
+    kb, vb, at, pos, tab, cache, scales = (DeviceBuffer.from_array(x) for x in (
+        k, v, np.arange(sequences + 1, dtype=np.int32), positions, table, host.bytes, host.scales))
+    ops.kv_cache_append_q8(kb.ptr, vb.ptr, at.ptr, pos.ptr, tab.ptr, cache.ptr, scales.ptr, sequences, sequences, heads,
+                           d, 1, len(held), stream)
+    back = [DeviceBuffer.from_array(np.full(k.size, SENTINEL, np.uint16)) for _ in range(2)]
+    ops.kv_cache_read_q8_f16(cache.ptr, scales.ptr, at.ptr, pos.ptr, tab.ptr, back[0].ptr, back[1].ptr, sequences,
+                             sequences, heads, d, 1, len(held), stream)
+    stream.synchronize()
+    for s in held:
+        for which, x in ((0, k), (1, v)):
+            host.append(x[s:s + 1], which, table[s], positions[s])
+    assert (cache.download(np.uint8).reshape(host.bytes.shape) == host.bytes).all()
+    assert (scales.download(np.float32).reshape(host.scales.shape) == host.scales).all()
+    for which in (0, 1):
+        got = back[which].download(np.uint16).reshape(k.shape)
+        for s in held:
+            want = host.values(which, table[s], positions[s] + 1)[-1:].astype(np.float16)
+            assert (got[s:s + 1] == want.view(np.uint16)).all()
+        got[held] = SENTINEL
+        assert (got == SENTINEL).all()
