@@ -2,7 +2,7 @@
 //
 // Attention of query i (position i + keys - queries in its sequence) over the
 // keys j it sees: o_i = sum_j p_ij v_j, p_ij = 2^(c q_i.k_j - m_i) / l_i, with
-// c = scale log2(e), m_i a bound near the row's largest exponent and l_i the sum
+// c = scale log2(e), m_i a reference near the row's largest exponent and l_i the sum
 // that makes the weights one.  One pass over the keys keeps (m, l, o) and
 // rescales l and o by 2^(m - m') when m grows to m'; parts of the keys computed
 // apart join the same way.  All of that is held in 32 bits.
@@ -31,12 +31,16 @@ __host__ __device__ constexpr uint32_t padded_dim(uint32_t d) { return (d + 31u)
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef uint32_t u32x2_a2 __attribute__((ext_vector_type(2), aligned(2)));
 
-// Rows whose largest exponent grows by no more than this keep their reference
-// m: weights then reach 2^(kGrowth + kShift) at most, within binary16 (2^16),
-// and those that matter stay above its subnormals: kShift places the weight of
-// the reference itself at 2^8, so weights down to 2^-22 of it keep all 11 bits.
-constexpr float kGrowth = 6.0f;
+// A row's reference m lies kShift under the largest exponent it had when it was
+// taken, so that the weight of that one is 2^8 and weights down to 2^-22 of it keep
+// all 11 bits of binary16.  It is kept until an exponent lies more than kReach over
+// it: weights stay within 2^14, and binary16 ends at 2^16.
 constexpr float kShift = 8.0f;
+constexpr float kReach = 14.0f;
+// Where exponents are this large, their roundings to 32 bits show in 2^(x - m): a
+// fused c s - m, next to an m taken from rounded products, would be off by as much.
+// x is then rounded by itself, as what m was taken from.
+constexpr float kLargeExponent = 0x1p22f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLeastFactor = 0x1p-100f;  // of scores: a masked one stays -inf, others vanish
 constexpr float kLeastScale = 0x1p-64f;  // of values: times 127 far below binary16, and its inverse in range
@@ -77,6 +81,17 @@ __device__ __forceinline__ float sum_of(Both v) { return v.a + v.b; }
 template <typename T>
 __device__ __forceinline__ T scalar_load(const T* p) {
     return *(const __attribute__((address_space(4))) T*)(p);
+}
+
+// The reference m where exponents reach up to `top` (-inf: none seen); no lower.
+__device__ __forceinline__ float reference(float m, float top) {
+    const float below = top - kShift;
+    return fmaxf(m, top - below > kReach ? top : below);  // where floats are 16 apart, top - 8 may be 16 below
+}
+// c s, rounded before anything is added to it.
+__device__ __forceinline__ float product(float s, float c) {
+#pragma clang fp contract(off)
+    return s * c;
 }
 
 // Packed sequences: tokens [at, at + n) of sequence s, from offsets held on the
@@ -156,6 +171,7 @@ template <int D>
 struct RowSums {
     f32x16 o[D];
     float m, l;  // l: of the lane's keys alone
+    bool large;  // some row's m is: exponents are rounded before m is taken off
 
     static __device__ __forceinline__ f32x16 zero() {
         return f32x16{0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
@@ -165,16 +181,18 @@ struct RowSums {
         for (int i = 0; i < D; ++i) o[i] = zero();
         m = -infinity();
         l = 0.0f;
+        large = false;
     }
     // Makes room for exponents up to `top` (of the row, the same in both halves).
     __device__ __forceinline__ void grow_to(float top) {
-        if (!wave_any(top > m + kGrowth)) return;
-        const float to = fmaxf(m, top);
+        if (!wave_any(top - m > kReach)) return;
+        const float to = reference(m, top);
         const float w = m == to ? 1.0f : exp2_fast(m - to);  // also where both are -inf
         m = to;
         l *= w;
 #pragma unroll
         for (int i = 0; i < D; ++i) o[i] *= w;
+        large = wave_any(fabsf(base()) > kLargeExponent);
     }
     __device__ __forceinline__ bool finite() const {
         float all = 0.0f;  // any that is not makes NaN
@@ -185,7 +203,7 @@ struct RowSums {
         return all == 0.0f;
     }
     // What exponents are taken less of.
-    __device__ __forceinline__ float base() const { return m == -infinity() ? 0.0f : m - kShift; }
+    __device__ __forceinline__ float base() const { return m == -infinity() ? 0.0f : m; }
     // The wave's results: through `stage`, 2 KB x D of LDS that is the wave's own, so
     // that whole rows leave in 16-byte chunks of neighbouring lanes (a lane's own
     // pieces are 8 bytes a row: 64 prompts of 128 tokens took 58 us so, 51 now).  row_at(i):
@@ -219,7 +237,7 @@ struct RowSums {
     __device__ __forceinline__ void write_part(float2* stats, float* sums, uint64_t at, uint32_t head_dim) const {
         const int h = (threadIdx.x >> 5) & 1;
         const float all = sum_of(across_halves(l));
-        if (h == 0) stats[at] = float2{m == -infinity() ? m : m - kShift, all};
+        if (h == 0) stats[at] = float2{m, all};
         if (all == 0.0f) return;  // saw nothing: not read
 #pragma unroll
         for (int i = 0; i < D; ++i)

@@ -207,15 +207,15 @@ cache_attention_kernel(CacheAttentionArgs a) {
             }
             float top = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
             top = max_of(across_halves(max_of(across_rows16(top))));
-            if (wave_any(top > m[t] + kGrowth)) {
-                const float to = fmaxf(m[t], top);
+            if (wave_any(top - m[t] > kReach)) {
+                const float to = reference(m[t], top);
                 const float w = m[t] == to ? 1.0f : exp2_fast(m[t] - to);  // also where both are -inf
                 m[t] = to;
                 l[t] *= w;
 #pragma unroll
                 for (int i = 0; i < 2 * C; ++i) o[t][i] *= w;
             }
-            const float base = m[t] == -infinity() ? 0.0f : m[t] - kShift;
+            const float base = m[t] == -infinity() ? 0.0f : m[t];
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -461,6 +461,14 @@ __global__ __launch_bounds__(256, CT <= 4 ? 2 : 1) void cache_tiles_kernel(Cache
             }
             sums.grow_to(max_of(across_halves(fmaxf(top[0], top[1]))));
             const float base = sums.base();
+            if (sums.large) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) s[t][i] = __builtin_fmaf(s[t][i], factor[t], more[t]);
+                    factor[t] = 1.0f, more[t] = 0.0f;
+                }
+            }
             f16x8 p[4];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {

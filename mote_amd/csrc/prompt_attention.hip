@@ -304,12 +304,18 @@ prompt_attention_kernel(PromptArgs a) {
                 float top = s[0][0];
 #pragma unroll
                 for (int i = 1; i < KEYS / 2; ++i) top = fmaxf(top, s[i >> 4][i & 15]);
-                sums.grow_to(max_of(across_halves(top)) * a.exponent);
+                sums.grow_to(product(max_of(across_halves(top)), a.exponent));
                 const float base = sums.base();
+                float exponent = a.exponent;
+                if (sums.large) {
+                    exponent = 1.0f;
+#pragma unroll
+                    for (int i = 0; i < KEYS / 2; ++i) s[i >> 4][i & 15] = product(s[i >> 4][i & 15], a.exponent);
+                }
                 f16x8 p[KEYS / 16];
 #pragma unroll
                 for (int i = 0; i < KEYS / 2; ++i) {
-                    const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], a.exponent, -base));
+                    const float e = exp2_fast(__builtin_fmaf(s[i >> 4][i & 15], exponent, -base));
                     sums.l += e;
                     p[i >> 3][i & 7] = static_cast<_Float16>(e);
                 }
