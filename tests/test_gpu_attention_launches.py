@@ -71,3 +71,52 @@ def test_cache_writes_and_reads_of_eight_million_sequences(stream):
             assert (got[s:s + 1] == want.view(np.uint16)).all()
         got[held] = SENTINEL
         assert (got == SENTINEL).all()
+
+
+def test_prompts_of_many_sequences_and_heads(stream):
+    """70000 sequences of one token, whose attention is its value, with 512 heads: more
+    than 2^32 threads in a launch's three directions together."""
+    rng = np.random.default_rng(3)
+    sequences, heads, d = 70000, 512, 8
+    v = rng.integers(0, 0x7C00, (sequences, heads, d), dtype=np.uint16)
+    q = rng.integers(0, 0x4000, v.shape, dtype=np.uint16)
+    qb, vb = DeviceBuffer.from_array(q), DeviceBuffer.from_array(v)
+    at = DeviceBuffer.from_array(np.arange(sequences + 1, dtype=np.int32))
+    out = DeviceBuffer(v.nbytes)
+    sizes = (sequences, sequences, sequences, 1, heads, heads, d)
+    assert ops.prompt_attention_workspace(*sizes) == 0
+    ops.prompt_attention_f16(qb.ptr, qb.ptr, vb.ptr, out.ptr, at.ptr, None, *sizes, d ** -0.5, 0, 0, stream)
+    stream.synchronize()
+    assert (out.download(np.uint16).reshape(v.shape) == v).all()
+
+
+def test_cache_writes_and_reads_of_many_sequences_and_heads(stream):
+    """As many workgroups, in two directions: 2^18 sequences of one token, 128 heads.
+    One sequence in 4096 has a block."""
+    rng = np.random.default_rng(4)
+    sequences, heads, d = 1 << 18, 128, 8
+    held = np.arange(4095, sequences, 4096)
+    host = Cache(len(held), heads, d, rng)
+    table = np.full((sequences, 1), -1, np.int32)
+    table[held, 0] = rng.permutation(len(held))
+    positions = rng.integers(0, BLOCK, sequences).astype(np.int32)
+    k, v = (rng.integers(0, 0x4000, (sequences, heads, d), dtype=np.uint16).view(np.float16) for _ in range(2))
+    kb, vb, at, pos, tab, cache, scales = (DeviceBuffer.from_array(x) for x in (
+        k, v, np.arange(sequences + 1, dtype=np.int32), positions, table, host.bytes, host.scales))
+    ops.kv_cache_append_q8(kb.ptr, vb.ptr, at.ptr, pos.ptr, tab.ptr, cache.ptr, scales.ptr, sequences, sequences, heads,
+                           d, 1, len(held), stream)
+    back = [DeviceBuffer.from_array(np.full(k.size, SENTINEL, np.uint16)) for _ in range(2)]
+    ops.kv_cache_read_q8_f16(cache.ptr, scales.ptr, at.ptr, pos.ptr, tab.ptr, back[0].ptr, back[1].ptr, sequences,
+                             sequences, heads, d, 1, len(held), stream)
+    stream.synchronize()
+    for s in held:
+        for which, x in ((0, k), (1, v)):
+            host.append(x[s:s + 1], which, table[s], positions[s])
+    assert (cache.download(np.uint8).reshape(host.bytes.shape) == host.bytes).all()
+    for which in (0, 1):
+        got = back[which].download(np.uint16).reshape(k.shape)
+        for s in held:
+            want = host.values(which, table[s], positions[s] + 1)[-1:].astype(np.float16)
+            assert (got[s:s + 1] == want.view(np.uint16)).all()
+        got[held] = SENTINEL
+        assert (got == SENTINEL).all()
