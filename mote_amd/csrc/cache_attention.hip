@@ -19,9 +19,10 @@
 // TB/s here.  The vector ALUs, which turn bytes into operands, are busy 40 % of it.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 
-#include "attention.hpp"
+#include "attention_sums.hpp"
 #include "tile_ops.hpp"
 
 namespace mote::attention {

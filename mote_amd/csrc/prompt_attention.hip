@@ -20,10 +20,11 @@
 // 1000 tokens 126 us, 540 TFLOP/s.
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdint>
 #include <type_traits>
 
-#include "attention.hpp"
+#include "attention_sums.hpp"
 #include "tile_ops.hpp"
 
 namespace mote::attention {
