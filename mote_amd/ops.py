@@ -137,6 +137,12 @@ def prompt_attention_workspace(sequences, query_tokens, key_tokens, max_keys, q_
     return need.value
 
 
+def _window(window: int) -> int:
+    if window < 0:
+        raise ValueError("a window of fewer than no tokens")
+    return window
+
+
 def prompt_attention_f16(q, k, v, out, query_offsets, key_offsets, sequences, query_tokens, key_tokens, max_keys,
                          q_heads, kv_heads, head_dim, scale, workspace, workspace_bytes, stream, causal=True,
                          window=0, strides=None) -> None:
@@ -147,7 +153,8 @@ def prompt_attention_f16(q, k, v, out, query_offsets, key_offsets, sequences, qu
     check(
         lib().mote_hip_prompt_attention_f16(
             q, k, v, out, query_offsets, key_offsets, sequences, query_tokens, key_tokens, max_keys, q_heads,
-            kv_heads, head_dim, sq, sk, sv, so, scale, int(causal), window, workspace, workspace_bytes, _s(stream)
+            kv_heads, head_dim, sq, sk, sv, so, scale, int(causal), _window(window), workspace, workspace_bytes,
+            _s(stream)
         ),
         "launch prompt attention kernel",
     )
@@ -201,8 +208,8 @@ def cache_attention_q8_f16(q, cache, scales, query_offsets, lengths, block_table
     check(
         lib().mote_hip_cache_attention_q8_f16(
             q, cache, scales, query_offsets, lengths, block_table, out, sequences, query_tokens, max_queries,
-            max_context, q_heads, kv_heads, head_dim, sq, so, table_blocks, cache_blocks, scale, window, workspace,
-            workspace_bytes, _s(stream)
+            max_context, q_heads, kv_heads, head_dim, sq, so, table_blocks, cache_blocks, scale, _window(window),
+            workspace, workspace_bytes, _s(stream)
         ),
         "launch cache attention kernel",
     )
