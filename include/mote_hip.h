@@ -299,8 +299,9 @@ int mote_hip_rope_tables_f32(const void* positions, void* cos_out, void* sin_out
  * with window > 0 only the last `window` of those; with causal = 0 all t keys
  * (window must be 0).  output = softmax(scale q k^T) v over the keys seen, in f32
  * with one f16 rounding (the weights of the second product are rounded to f16);
- * a query that sees none gets zeros.  Keys and values that a query does not see
- * do not touch its output, whatever they hold.  max_keys: at least the longest
+ * a query that sees none, or only scores of -infinity, gets zeros.  Keys and values
+ * that a query does not see do not touch its output, whatever they hold; of those it
+ * sees, a NaN shows as NaN and an infinity as an infinity or NaN.  max_keys: at least the longest
  * sequence's keys (it only chooses how the work is divided).
  * Few rows over many keys are computed in parts that a second launch joins, in
  * `workspace` (16-byte aligned, at least the bytes that
@@ -314,8 +315,8 @@ int mote_hip_rope_tables_f32(const void* positions, void* cos_out, void* sin_out
  * multiple of 8 or above 256, q_heads not a multiple of kv_heads or above 65535,
  * an output stride below q_heads x head_dim, a scale that is not finite and
  * positive, causal other than 0 or 1, a window without causal, key_offsets NULL
- * with key_tokens other than query_tokens, more than 2^30 rows, too small a
- * workspace; the launch status.  No sequence, query, head or dimension: 0 without
+ * with key_tokens other than query_tokens, more than 2^30 rows or sequences or
+ * 2^32 - 1 query rows x heads, too small a workspace; the launch status.  No sequence, query, head or dimension: 0 without
  * a launch. */
 int mote_hip_prompt_attention_workspace(uint64_t sequences, uint64_t query_tokens, uint64_t key_tokens,
                                         uint64_t max_keys, uint64_t q_heads, uint64_t kv_heads,
@@ -358,8 +359,8 @@ int mote_hip_prompt_attention_f16(const void* q, const void* k, const void* v, v
  * cache_blocks, are left out.  Nothing is allocated, and a call can be captured.
  * Status: 0; -1 for a null pointer, an odd f16 address, int32 or float arrays off
  * their alignment, a cache off the 16-byte grid, head_dim not a multiple of 8 or
- * above 256, more than 65535 heads, 2^30 tokens or 2^25 blocks of a sequence (for
- * read, a stride below kv_heads x head_dim); the launch status.  No sequence,
+ * above 256, more than 65535 heads, 2^30 tokens or sequences or 2^25 blocks of a
+ * sequence (for read, a stride below kv_heads x head_dim); the launch status.  No sequence,
  * token, head or dimension: 0 without a launch. */
 int mote_hip_kv_cache_append_q8(const void* k, const void* v, const void* offsets, const void* positions,
                                 const void* block_table, void* cache, void* scales, uint64_t sequences,
@@ -385,8 +386,9 @@ int mote_hip_kv_cache_read_q8_f16(const void* cache, const void* scales, const v
  * sequences and max_queries = 1.  Blocks whose number is not below cache_blocks
  * count as not there.  A plane whose scale is NaN makes every query NaN that
  * sees one of its tokens.  Nothing is allocated, and a call can be captured.
- * Status -1 also for more than 2^32 - 1 workgroups, of which a sequence takes at
- * most one for each key head, 16 rows (queries x heads of the key head) and part. */
+ * Status -1 also for max_queries x q_heads from 2^31 on and for more than 2^32 - 1
+ * workgroups, of which a sequence takes at most one for each key head, 16 rows
+ * (queries x heads of the key head) and part. */
 int mote_hip_cache_attention_workspace(uint64_t sequences, uint64_t query_tokens, uint64_t max_queries,
                                        uint64_t max_context, uint64_t q_heads, uint64_t kv_heads,
                                        uint64_t head_dim, size_t* bytes);

@@ -14,9 +14,12 @@
 // One pass is bound by the cache's bytes.  A workgroup takes `chunk` blocks of
 // one (sequence, rows, key head), its waves a block each in turn, and joins the
 // waves' sums through LDS; the chunks' sums join in a second launch.  With 8 key
-// heads of 128: 1 x 131 000 tokens 52 us (5.16 TB/s, the join included), 64 sequences
-// of up to 8192 tokens 106 us (4.83 TB/s), 1 x 600 tokens 6.9 us; a copy reaches 5.18
-// TB/s here.  The vector ALUs, which turn bytes into operands, are busy 40 % of it.
+// heads of 128: 1 x 131 000 tokens 52.5 us (5.11 TB/s, the join included), 64 sequences
+// of up to 8192 tokens 106.5 us (4.83 TB/s), 1 x 600 tokens 7.0 us; a copy reaches 5.05
+// to 5.18 TB/s here.  The vector ALUs, which turn bytes into operands, are busy 43 % of
+// the cycles.  Chunks are cut from max_context: with a window far shorter, or lengths
+// far below it, few of the workgroups have blocks (a window of 4096 over 131 072 tokens
+// 24 us, 4096 tokens without one 12).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -301,8 +304,8 @@ cache_attention_kernel(CacheAttentionArgs a) {
 // 32 x 32 x 16 instruction; the planes' order makes both operands of a lane 16
 // consecutive bytes of LDS, key row 16 c + 8 b + 4 h + r of a tile being token
 // 16 b + 8 c + 4 h + r of the block.  512 queries of 32 heads over 8192 tokens of 8
-// key heads of 128: 95 us, 700 TFLOP/s (in 16-row tiles 243), 10 of them the join of
-// four parts; matrix cores busy 38 % and vector ALUs 51 % of the cycles.  (The next
+// key heads of 128: 91 to 95 us, 700 to 730 TFLOP/s (in 16-row tiles 243), 10 of them the
+// join of four parts; matrix cores busy 38 % and vector ALUs 51 % of the cycles.  (The next
 // tile's scores under this one's weights, with two tiles' in registers: 99.)
 // CT: 32-dimension groups there is room for.
 constexpr uint32_t kTileRows = 128;

@@ -16,9 +16,10 @@
 // makes the plane's scale NaN until the block is begun again, so it shows in
 // every read and is never taken for a number.
 //
-// Both ways are bound by memory for prompts (8 of up to 2000 tokens, 8 heads of
-// 128, 42 MB each way: append 11.9 us, 3.6 TB/s; read 9.2 us, 4.6 TB/s) and by the
-// chain of loads for single tokens (64 sequences: 5.3 and 5.2 us).
+// Prompts (8 of up to 2000 tokens, 8 heads of 128, 42 MB each way): read 9.1 us, 4.6
+// TB/s; append 12.3 us, 3.4 TB/s, its waves waiting 56 % of their time (four barriers
+// between loads and stores) and the vector ALUs busy 59 % of the cycles.  Single tokens
+// are bound by the chain of loads offsets, table, rows (64 sequences: 5.4 and 5.3 us).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -214,9 +215,9 @@ __device__ __forceinline__ void write_plane(const CacheArgs& a, const Piece& p, 
 
 // One workgroup per (block piece, head): eight threads a token, which hold its
 // values of both planes, CHUNKS 16-byte chunks each, while the planes' scales are
-// found.  (8 prompts of 2000 tokens at most, 8 heads of 128: 13.5 us with room for
-// 256 dimensions in registers and LDS, which leaves four workgroups a compute
-// unit, 11.9 us with room for 128.)
+// found.  (8 prompts of 2000 tokens at most, 8 heads of 128: with room for 256
+// dimensions in registers and LDS, which leaves four workgroups a compute unit, 13 %
+// longer than with room for 128.)
 template <int CHUNKS>
 __global__ __launch_bounds__(256) void append_kernel(CacheArgs a) {
     __shared__ __align__(16) uint8_t image[2][kBlockTokens * 64 * CHUNKS];

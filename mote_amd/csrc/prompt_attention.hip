@@ -14,10 +14,10 @@
 // about 150 vector instructions, a fifth of them exponentials (1050 cycles); the
 // workgroups of a compute unit run the one under the other.  1 x 8192 tokens, 32 heads
 // of 128, causal: 557 to 590 us by the card, 930 to 990 TFLOP/s (a large library
-// product: 1175).  Power bounds it: the matrix cores are busy 60 % of the cycles, of
-// which the card gives 1.5 GHz over the launch (1.9 in light ones).  Short prompts wait
+// product: 1310 to 1325).  Power bounds it: the matrix cores are busy 60 % of the cycles,
+// of which the card gives 1.5 GHz over the launch (1.9 in light ones).  Short prompts wait
 // for their starts: 6300 cycles before a workgroup's first product, 24 prompts of up to
-// 1000 tokens 126 us, 540 TFLOP/s.
+// 1000 tokens 123 to 128 us, 530 to 550 TFLOP/s.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -57,10 +57,10 @@ __device__ __forceinline__ u32x2 read_transposed(const uint8_t* at) {
 
 // Position of 16-byte chunk c of row r in a tile of CH chunks a row: chunks of a
 // row are exchanged within aligned groups of G, a power of two, so that what is read
-// together lies in different banks, of which 16 chunks fill all: no conflict is
-// counted in the 8192-token case, where c ^ r for keys and c ^ 2 r for values made
-// conflicts a third of the LDS cycles.  16 / G neighbouring rows differ by their
-// place alone.
+// together lies in different banks, of which 16 chunks fill all: conflicts are 0.8 %
+// of the LDS cycles for 8192 tokens (a third with c ^ r for keys and c ^ 2 r for
+// values), 7 % for 24 packed prompts, 5 % for windows of 512 with heads of 64.
+// 16 / G neighbouring rows differ by their place alone.
 template <int CH>
 struct Swizzle {
     static constexpr int G = (CH & -CH) > 16 ? 16 : (CH & -CH);
@@ -83,8 +83,8 @@ __device__ __forceinline__ uint32_t finite_of(uint32_t pair) {
 
 // DP: the padded head size.  DIRECT: rows and addresses on the 16-byte grid and
 // head_dim = DP, so tiles go from memory to LDS without passing registers.  (Heads
-// of 64: four workgroups a compute unit, 95 us in the windowed case against 98 with
-// the three that fit without the bound.)
+// of 64: four workgroups a compute unit, for which three registers go to scratch, 95
+// us for windows of 512 against 98 with the three that fit without the bound.)
 //
 // KEYS: of a tile.  Tiles of 32 keys leave room for three workgroups of 128
 // dimensions a compute unit, which cover each other's starts where there are many:
@@ -253,7 +253,7 @@ prompt_attention_kernel(PromptArgs a) {
                 // The tile has come; what this wave read of the last one has arrived,
                 // since the others load over it once they are past the barrier.  (Said
                 // in assembly: after the builtin the compiler made the first LDS read
-                // wait for the loads of the next tile, 8192 tokens 584 us for 557.)
+                // wait for the loads of the next tile, 8192 tokens 5 % longer.)
                 asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
                 wait_counts<vm_wait(0)>();
                 group_barrier();

@@ -6,8 +6,10 @@ from one pool, and the calls that write and read them
 :class:`BlockTable` is the host's book-keeping alone; :class:`KVCacheQ8` adds the
 device memory.  The small arrays that describe a call (offsets, lengths, the
 block table) are uploaded by each call, which first waits for the stream of the
-call before (so calls may use different streams); a program that captures graphs
-or cannot wait keeps its own on the device and calls ``mote_amd.ops`` directly.
+call before (so calls may use different streams; one given by its handle must
+live until the next call).  That costs the host some 70 us a call: a program that
+captures graphs, cannot wait, or has the same sequences in many layers keeps its
+own on the device and calls ``mote_amd.ops`` directly.
 """
 
 from __future__ import annotations
@@ -88,7 +90,9 @@ class BlockTable:
             self.lengths[s] += n
 
     def truncate(self, sequence: int, length: int) -> None:
-        """Forgets the tokens from `length` on (drafts that were not taken)."""
+        """Forgets the tokens from `length` on (drafts that were not taken).  What
+        they made of the block that `length` lies in stays: its scales, which are
+        NaN where one of them was not finite."""
         self._known([sequence])
         if not 0 <= length <= self.lengths[sequence]:
             raise ValueError(f"sequence {sequence} holds {self.lengths[sequence]} tokens")
