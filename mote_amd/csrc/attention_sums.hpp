@@ -110,8 +110,8 @@ constexpr float kNotComputed = -1.0f;
 // Marks the rows of tokens [from, to) that belong to `count` heads from `head` on.
 __device__ inline void mark_rows(float2* stats, uint32_t from, uint32_t to, uint32_t heads, uint32_t head,
                                  uint32_t count) {
-    for (uint32_t t = from; t < to; ++t)
-        for (uint32_t i = threadIdx.x; i < count; i += blockDim.x)
+    for (uint32_t t = from + threadIdx.x; t < to; t += blockDim.x)
+        for (uint32_t i = 0; i < count; ++i)
             stats[static_cast<uint64_t>(t) * heads + head + i] = float2{-infinity(), kNotComputed};
 }
 // By one workgroup of a sequence and its heads: the sequence's rows past the first
