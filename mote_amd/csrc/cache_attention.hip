@@ -91,10 +91,12 @@ cache_attention_kernel(CacheAttentionArgs a) {
     const uint32_t group = a.heads / a.kv_heads;
     Span rows = {static_cast<int>(seq), 1};
     if (a.offsets != nullptr) rows = scalar_span_of(a.offsets, seq, a.tokens);
-    if (a.stats != nullptr && part == 0 && row_tile == 0)
-        mark_not_computed(a.stats, rows, seq, a.sequences, a.tokens, a.max_queries, a.heads, kv_head * group, group);
+    const auto mark = [&] {  // done last: before the walk, 80 rows of 16 x 8000 tokens took 110 us for 107
+        if (a.stats != nullptr && part == 0 && row_tile == 0)
+            mark_not_computed(a.stats, rows, seq, a.sequences, a.tokens, a.max_queries, a.heads, kv_head * group, group);
+    };
     const uint32_t row0 = row_tile * kRows, all_rows = min(static_cast<uint32_t>(rows.n), a.max_queries) * group;
-    if (row0 >= all_rows) return;
+    if (row0 >= all_rows) return mark();
     const uint32_t here = min(all_rows - row0, static_cast<uint32_t>(kRows));
     const int most_length = static_cast<int>(a.table_blocks * kBlockTokens);
     const int length = min(max(scalar_load(a.lengths + seq), 0), most_length);
@@ -296,6 +298,7 @@ cache_attention_kernel(CacheAttentionArgs a) {
             *reinterpret_cast<f32x4*>(out + 4) = hi;
         }
     }
+    mark();
 }
 
 // Many rows: 128 of a (sequence, key head), 32 a wave, over tiles of two blocks
