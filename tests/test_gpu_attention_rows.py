@@ -127,3 +127,40 @@ def test_prompt_rows_past_the_last_offset(stream, keys, in_parts, d, start):
                              need, stream)
     stream.synchronize()
     check_rows(out.download(np.float16).reshape(q.shape), want, bound, computed)
+
+
+@pytest.mark.parametrize("heads,kv_heads,d,most,lengths,parts", CACHE_FORMS)
+def test_cache_output_over_the_queries(stream, heads, kv_heads, d, most, lengths, parts):
+    rng = np.random.default_rng(7)
+    blocks = -(-max(lengths) // BLOCK)
+    host = Cache(2 * blocks, kv_heads, d, rng)
+    table = rng.permutation(2 * blocks).reshape(2, blocks).astype(np.int32)
+    q = rng.standard_normal((2 * most - 1, heads, d)).astype(np.float16)
+    qb, *bufs = (DeviceBuffer.from_array(x) for x in (q, host.bytes, host.scales, ints([0, most - 1, 2 * most - 1]),
+                                                      ints(lengths), table))
+    sizes = (2, len(q), most, max(lengths), heads, kv_heads, d)
+    need = ops.cache_attention_workspace(*sizes)
+    assert (need > 0) == parts
+    out, work = outputs(len(q), heads, d), workspace(need)
+    for to in (out, qb):
+        ops.cache_attention_q8_f16(qb.ptr, *(b.ptr for b in bufs), to.ptr, *sizes, blocks, len(host.bytes), d ** -0.5,
+                                   work.ptr, need, stream)
+    stream.synchronize()
+    assert (qb.download(np.uint16) == out.download(np.uint16)).all()
+
+
+@pytest.mark.parametrize("d", [40, 128, 256])
+def test_prompt_output_over_the_queries_in_parts(stream, d):
+    rng = np.random.default_rng(8)
+    q = rng.standard_normal((130, 4, d)).astype(np.float16)
+    k, v = (rng.standard_normal((3000, 2, d)).astype(np.float16) for _ in range(2))
+    qb, kb, vb, at, key_at = (DeviceBuffer.from_array(x) for x in (q, k, v, ints([0, 130]), ints([0, 3000])))
+    sizes = (1, 130, 3000, 3000, 4, 2, d)
+    need = ops.prompt_attention_workspace(*sizes)
+    assert need > 0
+    out, work = outputs(130, 4, d), workspace(need)
+    for to in (out, qb):
+        ops.prompt_attention_f16(qb.ptr, kb.ptr, vb.ptr, to.ptr, at.ptr, key_at.ptr, *sizes, d ** -0.5, work.ptr, need,
+                                 stream)
+    stream.synchronize()
+    assert (qb.download(np.uint16) == out.download(np.uint16)).all()
