@@ -9,7 +9,7 @@ operations) and through the library's entry points.
   their weights), and the plan of the products: the (token, choice) pairs in the
   order of their experts.  The last ``padded`` tokens have no expert.
 * ``quantize``: rows to microscaled ``bits`` and back to their own type.
-* ``linear``: y = x W^T, W in microscaled 4 bits, x in 4 or 8.
+* ``linear``: y = x W^T, W in microscaled 4 bits, x in 4 or 6.
 * ``gate_up``: for every pair, silu(x Wg^T) (x Wu^T) with its expert's weights;
   rows in the plan's order.
 * ``down``: for every token the weighted sum of its pairs' products with their
@@ -17,8 +17,11 @@ operations) and through the library's entry points.
 
 The microscaled formats: blocks of 32 elements along a row, each with a scale
 byte b that stands for 2^(b - 127).  4 bits: sign, 2 bits of exponent, 1 of
-mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6), element 2 i in the low half of byte i.  8
-bits: sign, 4, 3 (largest 448).
+mantissa (0, 0.5, 1, 1.5, 2, 3, 4, 6), element 2 i of a block in the low half of
+its byte i.  6 bits: sign, 2, 3 (0 to 2 in eighths, to 4 in quarters, to 7.5 in
+halves), element i in bits 6 i to 6 i + 5 of 24 bytes; the first 16 bytes of all
+of a row's blocks lie before the last 8 of all.  Rows are padded with zero bytes
+to a multiple of four blocks, values and scales.
 """
 
 import functools
@@ -31,6 +34,7 @@ import torch
 own = False  # whether run() calls the library
 
 BLOCK = 32  # elements of a scale
+PADDED = 128  # a row's elements are stored in multiples of these
 
 
 def _route(name, tokens, experts, top, score, type, bias=False, groups=1, top_groups=1, best=1, renormalize=True,
@@ -64,23 +68,23 @@ def listed():
         # the activations of 64 sequences' tokens before a product
         _quantize("quantize_batch", 64, 4096, 4, "f16"),
         # a prompt's activations before a down projection
-        _quantize("quantize_prompt", 4000, 14336, 8, "f16"),
+        _quantize("quantize_prompt", 4000, 14336, 6, "f16"),
         # one token through an up projection: the latency of a weight-streaming call
-        _linear("linear_one", 1, 14336, 4096, 8, "f16"),
+        _linear("linear_one", 1, 14336, 4096, 6, "f16"),
         # 48 sequences through a down projection
         _linear("linear_batch", 48, 4096, 14336, 4, "f32"),
         # a chunk of prompts through an up projection (the most operations)
         _linear("linear_prompt", 4096, 14336, 4096, 4, "f16"),
         # one token's eight experts, small ones
-        _experts("gate_up_one", "gate_up", 1, 8, 128, 2048, 768, 8, 1),
+        _experts("gate_up_one", "gate_up", 1, 8, 128, 2048, 768, 6, 1),
         # 64 sequences over 32 experts, widths that are not multiples of 128
-        _experts("gate_up_batch", "gate_up", 64, 4, 32, 2880, 2880, 8, 2),
+        _experts("gate_up_batch", "gate_up", 64, 4, 32, 2880, 2880, 6, 2),
         # a chunk of prompts over many small experts, its end padded
         _experts("gate_up_prompt", "gate_up", 4096, 8, 128, 2048, 768, 4, 3, padded=60),
         # 48 sequences, the weighted sum of six experts each
         _experts("down_batch", "down", 48, 6, 64, 4096, 1408, 4, 4),
         # a chunk of prompts over few experts of unequal use
-        _experts("down_prompt", "down", 5000, 4, 32, 2880, 2880, 8, 5, skew=1.0),
+        _experts("down_prompt", "down", 5000, 4, 32, 2880, 2880, 6, 5, skew=1.0),
     ]
 
 
@@ -122,7 +126,7 @@ def draw(rng):
 def _draw(rng):
     kind = rng.choice(["route", "quantize", "linear", "linear", "gate_up", "gate_up", "down", "down"])
     tokens = rng.choice([1, _log_int(rng, 1, 8), _log_int(rng, 2, 64), _log_int(rng, 16, 8192), _log_int(rng, 64, 8192)])
-    bits = rng.choice([4, 8])
+    bits = rng.choice([4, 6])
     type = rng.choice(["f16", "f32"])
     if kind == "quantize":
         return _unnamed(_quantize("", tokens, _width(rng, 64, 32768), bits, type))
@@ -178,6 +182,10 @@ def _in_experts_order(ids, experts):
     return offsets, rows
 
 
+def _padded(features):
+    return -(-features // PADDED) * PADDED
+
+
 def _bytes(g, *shape):
     return torch.randint(0, 256, shape, dtype=torch.uint8, device="cuda", generator=g)
 
@@ -185,9 +193,13 @@ def _bytes(g, *shape):
 def _weights(g, experts, outputs, features):
     """Values and scales whose products of unit inputs are about one."""
     middle = 127 - int(round(math.log2(2.5 * math.sqrt(features))))
-    scales = torch.randint(middle - 1, middle + 2, (experts, outputs, features // BLOCK), dtype=torch.uint8,
+    width = _padded(features)
+    scales = torch.randint(middle - 1, middle + 2, (experts, outputs, width // BLOCK), dtype=torch.uint8,
                            device="cuda", generator=g)
-    return _bytes(g, experts, outputs, features // 2), scales
+    scales[..., features // BLOCK:] = 0
+    values = _bytes(g, experts, outputs, width // 2)
+    values[..., features // 2:] = 0
+    return values, scales
 
 
 def _activations(g, rows, features):
@@ -253,8 +265,9 @@ def _prepare_route(s, case, g):
 
 
 def _quantized_room(s, rows, features, bits):
-    s["values"] = torch.empty(rows, features * bits // 8, dtype=torch.uint8, device="cuda")
-    s["scales"] = torch.empty(rows, features // BLOCK, dtype=torch.uint8, device="cuda")
+    width = _padded(features)
+    s["values"] = torch.empty(rows, width * bits // 8, dtype=torch.uint8, device="cuda")
+    s["scales"] = torch.empty(rows, width // BLOCK, dtype=torch.uint8, device="cuda")
 
 
 # --- one pass -------------------------------------------------------------
@@ -382,8 +395,7 @@ def _plain_plan(ids, experts):
     return offsets, torch.where(expert == experts, -1, rows).to(torch.int32)
 
 
-_E2M1 = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)
-_SIZE = {4: (2, 6.0), 8: (8, 448.0)}  # exponent of the largest element, and it
+_SIZE = {4: (2, 6.0, 1), 6: (2, 7.5, 3)}  # exponent of the largest element, it, bits of mantissa
 
 
 def _powers(device):
@@ -393,10 +405,10 @@ def _powers(device):
 
 def _to_element(y, bits):
     """y to the nearest element, halves to the even one."""
-    emax, most = _SIZE[bits]
+    _, most, mantissa = _SIZE[bits]
     y = y.clamp(-most, most)
-    exponent = (torch.frexp(y)[1] - 1).clamp_min(0 if bits == 4 else -6)
-    step = torch.exp2((exponent - (1 if bits == 4 else 3)).float())
+    exponent = (torch.frexp(y)[1] - 1).clamp_min(0)
+    step = torch.exp2((exponent - mantissa).float())
     return torch.round(y / step) * step
 
 
@@ -412,28 +424,43 @@ def _plain_values(x, bits):
     return _to_element(y, bits), shared
 
 
+def _elements(bits, device):
+    """What each code stands for."""
+    mantissa = _SIZE[bits][2]
+    code = torch.arange(1 << (bits - 1), device=device)
+    exponent, part = code >> mantissa, (code & ((1 << mantissa) - 1)).float() / (1 << mantissa)
+    size = torch.where(exponent > 0, (1 + part) * torch.exp2((exponent - 1).float()), part)
+    return torch.cat([size, -size])
+
+
 def _plain_quantize(x, bits):
-    """The bytes that stand for x: values [rows, features bits / 8] and scales."""
+    """The bytes that stand for x: values [rows, padded features bits / 8] and scales."""
+    rows, features = x.shape
     y, shared = _plain_values(x, bits)
-    scales = (shared + 127).to(torch.uint8).squeeze(2)
-    y = y.view(x.shape)
-    if bits == 8:
-        return y.to(torch.float8_e4m3fn).view(torch.uint8), scales
-    table = torch.tensor(_E2M1, device=x.device)
-    code = torch.bucketize(y.abs(), table).to(torch.uint8) | (y < 0).to(torch.uint8) << 3
-    return code[:, ::2] | code[:, 1::2] << 4, scales
+    more = (0, 0, 0, (_padded(features) - features) // BLOCK)
+    scales = torch.nn.functional.pad((shared + 127).to(torch.uint8), more).squeeze(2)
+    y = torch.nn.functional.pad(y, more)
+    size = _elements(bits, x.device)[:1 << (bits - 1)]
+    code = torch.bucketize(y.abs(), size).to(torch.uint8) | (y < 0).to(torch.uint8) << (bits - 1)
+    if bits == 4:
+        return (code[..., ::2] | code[..., 1::2] << 4).view(rows, -1), scales
+    a, b, c, d = (code[..., i::4] for i in range(4))
+    block = torch.stack([a | b << 6, b >> 2 | c << 4, c >> 4 | d << 2], -1).view(rows, -1, 24)
+    return torch.cat([block[..., :16].reshape(rows, -1), block[..., 16:].reshape(rows, -1)], 1), scales
 
 
 def _plain_read(values, scales, bits):
-    """What bytes [..., features bits / 8] and scales [..., features / 32] stand
-    for, in 32 bits."""
-    if bits == 8:
-        y = values.view(torch.float8_e4m3fn).float()
+    """What values [..., padded features bits / 8] and scales [..., padded
+    features / 32] stand for, in 32 bits."""
+    if bits == 4:
+        code = torch.stack([values & 15, values >> 4], -1).flatten(-2)
     else:
-        table = torch.tensor(_E2M1 + tuple(-v for v in _E2M1), device=values.device)
-        y = torch.stack([table[(values & 15).int()], table[(values >> 4).int()]], -1).flatten(-2)
+        at = values.shape[-1] // 24 * 16
+        block = torch.cat([values[..., :at].unflatten(-1, (-1, 16)), values[..., at:].unflatten(-1, (-1, 8))], -1)
+        p, q, r = (block[..., i::3] for i in range(3))
+        code = torch.stack([p & 63, p >> 6 | (q & 15) << 2, q >> 4 | (r & 3) << 4, r >> 2], -1).flatten(-3)
     of = _powers(values.device)[scales.int()]
-    return (y.unflatten(-1, (-1, BLOCK)) * of[..., None]).flatten(-2)
+    return (_elements(bits, values.device)[code.int()].unflatten(-1, (-1, BLOCK)) * of[..., None]).flatten(-2)
 
 
 def _plain_quantize_pass(s, case):
@@ -561,17 +588,10 @@ def _exact_route(s, case):
 def _elements64(bits):
     """Every value that an element's code can stand for, by its code."""
     if bits == 4:
-        exponent_bits, mantissa_bits, bias = 2, 1, 1
+        up = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
     else:
-        exponent_bits, mantissa_bits, bias = 4, 3, 7
-    values = []
-    for code in range(1 << (exponent_bits + mantissa_bits)):
-        e, m = code >> mantissa_bits, code % (1 << mantissa_bits)
-        part = m / (1 << mantissa_bits)
-        values.append((1 + part) * 2.0 ** (e - bias) if e else part * 2.0 ** (1 - bias))
-    if bits == 8:
-        values[-1] = math.nan
-    return torch.tensor(values + [-v for v in values], dtype=torch.float64, device="cuda")
+        up = [i / 8 for i in range(16)] + [2 + i / 4 for i in range(8)] + [4 + i / 2 for i in range(8)]
+    return torch.tensor(up + [-v for v in up], dtype=torch.float64, device="cuda")
 
 
 def _exact_quantize(s, case):
@@ -579,7 +599,6 @@ def _exact_quantize(s, case):
     bits = case["bits"]
     elements = _elements64(bits)
     up = elements[:len(elements) // 2]
-    up = up[torch.isfinite(up)]
     x = s["x"].double().view(case["rows"], -1, BLOCK)
     out = torch.empty_like(x)
     for a in range(0, case["rows"], 512):  # a part at a time: 64 bits of everything is much
@@ -595,10 +614,21 @@ def _exact_quantize(s, case):
 
 
 def _read64(values, scales, bits):
+    blocks = scales.shape[-1]
     if bits == 4:
-        values = torch.stack([values % 16, values // 16], -1).flatten(-2)
-    y = _elements64(bits)[values.long()]
-    return y * torch.exp2(scales.double() - 127).repeat_interleave(BLOCK, -1)
+        stream = values.view(*scales.shape, 16)
+    else:
+        stream = torch.cat([values[..., :16 * blocks].view(*scales.shape, 16),
+                            values[..., 16 * blocks:].view(*scales.shape, 8)], -1)
+    out = torch.empty(*scales.shape, BLOCK, dtype=torch.float64, device="cuda")
+    elements = _elements64(bits)
+    for i in range(BLOCK):  # the bits of element i, in one byte or two
+        byte, shift = bits * i // 8, bits * i % 8
+        word = stream[..., byte].long()
+        if shift + bits > 8:
+            word = word + 256 * stream[..., byte + 1].long()
+        out[..., i] = elements[torch.div(word, 1 << shift, rounding_mode="floor") % (1 << bits)]
+    return (out * torch.exp2(scales.double() - 127)[..., None]).flatten(-2)
 
 
 def _exact_linear(s, case):
