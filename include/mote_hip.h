@@ -1,7 +1,7 @@
 /*
  * mote_hip.h: C ABI of libmote_hip.so, the MI355X (gfx950) implementation of
- * Mote's Q4_0 quantized-linear path, RMSNorm and RoPE, and of the attention
- * between them.
+ * Mote's Q4_0 quantized-linear path, RMSNorm and RoPE, of the attention between
+ * them, and of the MLP of a mixture of experts.
  *
  * Conventions (all of them those of the reference's Rust FFI,
  * crates/mote-backend-hip/src/ffi.rs:8-13): pointers are untyped device
@@ -400,6 +400,119 @@ int mote_hip_cache_attention_q8_f16(const void* q, const void* cache, const void
                                     uint64_t output_stride, uint64_t table_blocks, uint64_t cache_blocks,
                                     float scale, uint64_t window, void* workspace, size_t workspace_bytes,
                                     void* stream);
+
+/* ---- Microscaled formats ----------------------------------------------------- */
+/* [new] No counterpart in the reference.  Rows of `features` elements (a multiple of
+ * 32) in blocks of 32 with a scale each.  With Kp = features rounded up to a multiple
+ * of 128, `values` is uint8 [rows][Kp bits / 8] (16-byte aligned) and `scales` uint8
+ * [rows][Kp / 32]; what of a row lies past `features` is zeros.  A scale byte b
+ * stands for 2^(b - 127), 255 for not a number.  bits = 4: E2M1, code c (its top bit
+ * the sign) for 0, 0.5, 1, 1.5, 2, 3, 4, 6; bits = 6: E2M3, 0 to 1.875 in eighths, to
+ * 3.75 in quarters, to 7.5 in halves.  Element i of a block is bits (bits x i) up to (bits x
+ * (i + 1)) of its 4 x bits bytes, lowest first.  Block n's first 16 bytes are at 16 n of its
+ * row, its other 8 (bits = 6) at Kp / 2 + 8 n.  (4-bit rows of a multiple of 128
+ * elements are those of the published MXFP4 format, two elements a byte, the first in the
+ * low half.)
+ *
+ * quantize: rows `input_stride` elements apart.  Scale 2^(floor(log2 m) - 2), m the
+ * block's largest magnitude, at least 2^-127; elements rounded to the nearest, ties to
+ * the even code, held to +-6 or +-7.5.  A block of zeros has scale byte 0; one with an infinity or
+ * NaN has 255 and zeros.  Writes the padding too.
+ * dequantize: element x 2^(b - 127) rounded once to the output's type, to rows
+ * `output_stride` apart; what lies between the rows is left as it is.
+ * Status: 0; -1 for a null pointer, bits other than 4 or 6, features not a multiple of
+ * 32 or above 2^24, a stride below features or above 2^40, more than 2^31 rows or 2^32 - 257 blocks
+ * (padding included), values off the 16-byte grid, f16 or f32 off their alignment; the
+ * launch status.  No row or feature: 0 without a launch. */
+int mote_hip_mx_quantize_f16(const void* input, void* values, void* scales, uint64_t rows, uint64_t features,
+                             uint64_t input_stride, int bits, void* stream);
+int mote_hip_mx_quantize_f32(const void* input, void* values, void* scales, uint64_t rows, uint64_t features,
+                             uint64_t input_stride, int bits, void* stream);
+int mote_hip_mx_dequantize_f16(const void* values, const void* scales, void* output, uint64_t rows,
+                               uint64_t features, uint64_t output_stride, int bits, void* stream);
+int mote_hip_mx_dequantize_f32(const void* values, const void* scales, void* output, uint64_t rows,
+                               uint64_t features, uint64_t output_stride, int bits, void* stream);
+
+/* [new] output[rows, N] = input[rows, K] x weights[N, K]^T, the weights in 4 bits, the
+ * input in input_bits (4 or 6), f32 accumulation, one rounding to the output's type.  A
+ * scale that is not a number shows as NaN in the outputs of its row.
+ * Status: 0; -1 for a null pointer, input_bits other than 4 or 6, K not a multiple of
+ * 32, K or N above 2^24, more than 2^30 rows, values off the 16-byte grid or scales off the 4-byte
+ * one, an output off its alignment, more work than one launch holds (rows / 64 x N / 16 of
+ * 2^23 - 1); the launch status.  rows == 0 or N == 0: 0 without a launch; K == 0 writes
+ * zeros.  Output must not alias the inputs.  Nothing is allocated, and a call can be captured. */
+int mote_hip_mx_linear_f16(const void* input_values, const void* input_scales, const void* weight_values,
+                           const void* weight_scales, void* output, uint64_t rows, uint64_t output_features,
+                           uint64_t input_features, int input_bits, void* stream);
+int mote_hip_mx_linear_f32(const void* input_values, const void* input_scales, const void* weight_values,
+                           const void* weight_scales, void* output, uint64_t rows, uint64_t output_features,
+                           uint64_t input_features, int input_bits, void* stream);
+
+/* ---- Experts -------------------------------------------------------------------- */
+/* [new] No counterpart in the reference.  The `top` experts of each token: logits
+ * [tokens, experts] -> ids (int32) and weights (float), [tokens, top] each, the best first.
+ * score 0: softmax over the experts; 1: sigmoid.  The choice is by score + bias[expert]
+ * (float, NULL: none), the lowest index first among equals; the bias is not in the weights.
+ * With top_groups < groups the experts are `groups` runs of experts / groups; a group's
+ * worth is the sum of its group_best (1 or 2) best choices, as many as it has, and only the experts of
+ * the top_groups best groups are chosen.  weights = scale x score, divided by the chosen
+ * scores' sum with renormalize = 1 (0 where that is 0).  An expert whose logit, or whose score +
+ * bias, is infinite or NaN takes no part (a logit that is, not in the softmax either);
+ * where fewer than `top` are left the ids are -1 and the weights 0, so a row of
+ * -infinity is a token without experts.  Scores are held in 64 bits.
+ * Status: 0; -1 for a null pointer (bias excepted), logits, bias, ids or weights off
+ * their alignment, score or renormalize other than 0 or 1, group_best other than 1 or 2, a scale that is
+ * not finite, more than 1024 experts, top above 64 or above the experts that the groups leave, groups that do not
+ * divide the experts or top_groups not in 1 .. groups, more than 2^26 - 1 tokens
+ * or 2^30 pairs; the launch status.  No token, expert or top: 0 without a launch. */
+int mote_hip_route_experts_f16(const void* logits, const void* bias, void* ids, void* weights, uint64_t tokens,
+                               uint64_t experts, uint64_t top, int score, uint64_t groups, uint64_t top_groups,
+                               int group_best, int renormalize, float scale, void* stream);
+int mote_hip_route_experts_f32(const void* logits, const void* bias, void* ids, void* weights, uint64_t tokens,
+                               uint64_t experts, uint64_t top, int score, uint64_t groups, uint64_t top_groups,
+                               int group_best, int renormalize, float scale, void* stream);
+
+/* [new] The plan of the experts' products: the pairs (token t, choice j), numbered
+ * top x t + j, in the order of their experts and within one of their numbers.  rows (int32
+ * [tokens x top]): the pairs; expert e has rows offsets[e] up to offsets[e + 1] (int32
+ * [experts + 1]).  A pair whose id is not in 0 .. experts - 1 has no row; the rows
+ * past offsets[experts] are -1.
+ * Status: 0; -1 for a null pointer, int32 arrays off their alignment, more than 1024
+ * experts, top above 64, 2^30 pairs or tokens; the launch status.  No expert: 0 without a launch. */
+int mote_hip_plan_experts(const void* ids, void* offsets, void* rows, uint64_t tokens, uint64_t top,
+                          uint64_t experts, void* stream);
+
+/* [new] The experts' gate and up projections: row i of output (f16 [tokens x top, inner]) is,
+ * for the pair rows[i] of token t and expert e, silu(x_t Wg_e^T) (x_t Wu_e^T), in f32 with one
+ * rounding; x [tokens, hidden] in input_bits, weights 4-bit rows [experts][2 inner] of
+ * `hidden`, an expert's gate rows first.  Rows past offsets[experts] are left as they are.
+ *
+ * The down projection: output[t] (f16 [tokens, hidden]) = the sum over j of pair_weights[t, j]
+ * h_(t, j) W_e^T, in the order of j in f32 (a pair that the plan leaves out adds nothing; a
+ * token with none gets zeros); row i of the input (h, `inner` elements in input_bits) is that of pair
+ * rows[i], weights 4-bit rows [experts][hidden] of `inner`.  The pairs' products meet in `workspace`
+ * (16-byte aligned, at least the bytes that mote_hip_experts_down_workspace says for the same
+ * sizes); it holds nothing between calls, and calls that overlap need their own.  ids and
+ * plan must belong together.
+ *
+ * Offsets that run past the pairs are cut to them, and a row that names no pair reads
+ * token 0 or is left out.  Nothing is allocated, and a call can be captured.
+ * Status: 0; -1 for a null pointer (a workspace of which 0 bytes are needed excepted), operands as for
+ * mx_linear, int32 or float arrays off their alignment, hidden or inner not a multiple of 32 or
+ * above 2^24, more than 1024 experts, top above 64, 2^30 pairs or tokens, too small a
+ * workspace, more work than one launch holds; the launch status.  No output: 0 without a launch. */
+int mote_hip_experts_gate_up_silu_mx_f16(const void* input_values, const void* input_scales,
+                                         const void* weight_values, const void* weight_scales, const void* offsets,
+                                         const void* rows, void* output, uint64_t tokens, uint64_t top,
+                                         uint64_t experts, uint64_t hidden, uint64_t inner, int input_bits,
+                                         void* stream);
+int mote_hip_experts_down_workspace(uint64_t tokens, uint64_t top, uint64_t experts, uint64_t hidden, uint64_t inner,
+                                    size_t* bytes);
+int mote_hip_experts_down_mx_f16(const void* input_values, const void* input_scales, const void* weight_values,
+                                 const void* weight_scales, const void* ids, const void* offsets, const void* rows,
+                                 const void* pair_weights, void* output, uint64_t tokens, uint64_t top,
+                                 uint64_t experts, uint64_t hidden, uint64_t inner, int input_bits, void* workspace,
+                                 size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

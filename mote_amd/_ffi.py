@@ -98,6 +98,24 @@ SIGNATURES = {
         _I,
         [_P] * 7 + [_U64] * 11 + [ctypes.c_float, _U64, _P, _SZ, _P],
     ),
+    "mote_hip_mx_quantize_f16": (_I, [_P] * 3 + [_U64] * 3 + [_I, _P]),
+    "mote_hip_mx_quantize_f32": (_I, [_P] * 3 + [_U64] * 3 + [_I, _P]),
+    "mote_hip_mx_dequantize_f16": (_I, [_P] * 3 + [_U64] * 3 + [_I, _P]),
+    "mote_hip_mx_dequantize_f32": (_I, [_P] * 3 + [_U64] * 3 + [_I, _P]),
+    "mote_hip_mx_linear_f16": (_I, [_P] * 5 + [_U64] * 3 + [_I, _P]),
+    "mote_hip_mx_linear_f32": (_I, [_P] * 5 + [_U64] * 3 + [_I, _P]),
+    "mote_hip_route_experts_f16": (
+        _I,
+        [_P] * 4 + [_U64] * 3 + [_I, _U64, _U64, _I, _I, ctypes.c_float, _P],
+    ),
+    "mote_hip_route_experts_f32": (
+        _I,
+        [_P] * 4 + [_U64] * 3 + [_I, _U64, _U64, _I, _I, ctypes.c_float, _P],
+    ),
+    "mote_hip_plan_experts": (_I, [_P] * 3 + [_U64] * 3 + [_P]),
+    "mote_hip_experts_gate_up_silu_mx_f16": (_I, [_P] * 7 + [_U64] * 5 + [_I, _P]),
+    "mote_hip_experts_down_workspace": (_I, [_U64] * 5 + [ctypes.POINTER(_SZ)]),
+    "mote_hip_experts_down_mx_f16": (_I, [_P] * 9 + [_U64] * 5 + [_I, _P, _SZ, _P]),
 }
 
 _lib: ctypes.CDLL | None = None

@@ -1,0 +1,107 @@
+// What the products of microscaled rows share: their arguments, and how an experts'
+// product finds its rows.
+#pragma once
+
+#include "mx.hpp"
+
+namespace mote::mx {
+namespace {
+
+
+// What a product's outputs become.
+enum class Result {
+    kF16,     // rows x outputs, binary16 (a linear)
+    kF32,     // the same in 32 bits
+    kGateUp,  // silu(gate) up of an expert's 2 outputs weight rows, binary16, row i of the plan
+    kPairs,   // row i of the plan to the row of its pair, 32 bits (an expert's down projection)
+};
+template <Result R>
+constexpr bool kOfExperts = R == Result::kGateUp || R == Result::kPairs;
+
+struct ProductArgs {
+    const uint8_t* x;        // values of the rows
+    const uint8_t* x_scales;
+    const uint8_t* w;        // values of the weights' rows, expert after expert
+    const uint8_t* w_scales;
+    void* output;
+    const int32_t* offsets;  // [experts + 1] first row of the plan of each expert
+    const int32_t* plan;     // the pair of each row of the plan
+    uint32_t rows;           // of a linear's x; pairs of the experts'
+    uint32_t outputs;        // columns of the output
+    uint32_t kp;
+    uint32_t experts, top;
+};
+
+// The rows of one tile: an expert's, `count` of them (0: no such tile) from row `first` of the
+// plan, or a linear's.
+struct Tile {
+    uint32_t expert, first, count;
+};
+
+// Tile `unit` of the experts' tiles of PER rows: each expert has its rows / PER of
+// them, rounded up.  Every wave looks it up by itself: lane l counts those of its run
+// of experts, a prefix sum over the lanes finds the run, and the run is walked.
+template <uint32_t PER>
+__device__ __forceinline__ Tile expert_tile(const ProductArgs& a, uint32_t unit) {
+    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t run = (a.experts + 63) / 64;
+    const auto at = [&](uint32_t e) {  // kept inside the rows there are, whatever the offsets hold
+        return static_cast<uint32_t>(min(max(a.offsets[e], 0), static_cast<int32_t>(a.rows)));
+    };
+    uint32_t mine = 0;
+    const uint32_t e0 = min(lane * run, a.experts), e1 = min(e0 + run, a.experts);
+    if (e0 < e1) {
+        uint32_t from = at(e0);
+        for (uint32_t e = e0; e < e1; ++e) {
+            const uint32_t to = at(e + 1);
+            mine += to > from ? (to - from + PER - 1) / PER : 0;
+            from = to;
+        }
+    }
+    uint32_t upto = mine;  // tiles of this lane's experts and the lanes' before
+#pragma unroll
+    for (int by = 1; by < 64; by *= 2) {
+        const uint32_t other = __shfl_up(upto, by, 64);
+        if (lane >= static_cast<uint32_t>(by)) upto += other;
+    }
+    const uint64_t before = __builtin_amdgcn_ballot_w64(upto <= unit);
+    const uint32_t owner = __builtin_popcountll(before);
+    if (owner == 64) return {0, 0, 0};
+    uint32_t left = unit;
+    if (owner > 0) left -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), owner - 1));
+    for (uint32_t e = owner * run; e < a.experts; ++e) {
+        const uint32_t from = at(e), to = at(e + 1);
+        const uint32_t n = to > from ? to - from : 0, tiles = (n + PER - 1) / PER;
+        if (left < tiles) return {e, from + left * PER, min(n - left * PER, PER)};
+        left -= tiles;
+    }
+    return {0, 0, 0};
+}
+
+// As many tiles as there may be.
+inline uint64_t most_expert_tiles(uint64_t pairs, uint64_t experts, uint64_t per) {
+    const uint64_t used = pairs < experts ? pairs : experts;
+    const uint64_t tiles = pairs / per + used;
+    return tiles < pairs ? tiles : pairs;
+}
+
+template <Result R, uint32_t PER>
+__device__ __forceinline__ Tile find_tile(const ProductArgs& a, uint32_t unit) {
+    if constexpr (kOfExperts<R>) return expert_tile<PER>(a, unit);
+    const uint32_t first = unit * PER;
+    return {0, first, min(a.rows - first, PER)};
+}
+
+// The row of x that row `first + i` of a tile multiplies.
+template <Result R>
+__device__ __forceinline__ uint32_t input_row(const ProductArgs& a, uint32_t row) {
+    if constexpr (R == Result::kGateUp) {
+        // An entry that names no pair reads row 0, in place of memory that is not x.
+        const uint32_t pair = static_cast<uint32_t>(a.plan[row]);
+        return pair < a.rows ? pair / a.top : 0;
+    }
+    return row;
+}
+
+}  // namespace
+}  // namespace mote::mx

@@ -11,6 +11,9 @@ from ._ffi import HipError, check, lib
 HALF_SPLIT = 0
 INTERLEAVED = 1
 
+SOFTMAX = 0
+SIGMOID = 1
+
 
 def _s(stream) -> int:
     return stream.handle if hasattr(stream, "handle") else int(stream)
@@ -212,6 +215,117 @@ def cache_attention_q8_f16(q, cache, scales, query_offsets, lengths, block_table
             workspace, workspace_bytes, _s(stream)
         ),
         "launch cache attention kernel",
+    )
+
+
+def _stride(stride, features):
+    if stride is None:
+        return features
+    if stride < 0:
+        raise ValueError("a negative stride")
+    return stride
+
+
+def mx_value_bytes(features, bits) -> int:
+    """Bytes of a row of microscaled values, padded to four blocks."""
+    return -(-features // 128) * 128 * bits // 8
+
+
+def mx_scale_bytes(features) -> int:
+    """Bytes of a row's scales."""
+    return -(-features // 128) * 4
+
+
+def mx_quantize_f16(x, values, scales, rows, features, bits, stream, stride=None) -> None:
+    """Rows to microscaled 4 or 6 bits.  `stride`: elements between the rows of x."""
+    check(lib().mote_hip_mx_quantize_f16(x, values, scales, rows, features, _stride(stride, features), bits,
+                                         _s(stream)), "launch quantization kernel")
+
+
+def mx_quantize_f32(x, values, scales, rows, features, bits, stream, stride=None) -> None:
+    check(lib().mote_hip_mx_quantize_f32(x, values, scales, rows, features, _stride(stride, features), bits,
+                                         _s(stream)), "launch quantization kernel")
+
+
+def mx_dequantize_f16(values, scales, out, rows, features, bits, stream, stride=None) -> None:
+    """Microscaled rows back.  `stride`: elements between the rows of out."""
+    check(lib().mote_hip_mx_dequantize_f16(values, scales, out, rows, features, _stride(stride, features), bits,
+                                           _s(stream)), "launch microscaled decode kernel")
+
+
+def mx_dequantize_f32(values, scales, out, rows, features, bits, stream, stride=None) -> None:
+    check(lib().mote_hip_mx_dequantize_f32(values, scales, out, rows, features, _stride(stride, features), bits,
+                                           _s(stream)), "launch microscaled decode kernel")
+
+
+def mx_linear_f16(x, x_scales, w, w_scales, y, rows, n, k, x_bits, stream) -> None:
+    """y = x w^T, w in microscaled 4 bits, x in x_bits (4 or 6)."""
+    check(lib().mote_hip_mx_linear_f16(x, x_scales, w, w_scales, y, rows, n, k, x_bits, _s(stream)),
+          "launch microscaled linear kernel")
+
+
+def mx_linear_f32(x, x_scales, w, w_scales, y, rows, n, k, x_bits, stream) -> None:
+    check(lib().mote_hip_mx_linear_f32(x, x_scales, w, w_scales, y, rows, n, k, x_bits, _s(stream)),
+          "launch microscaled linear kernel")
+
+
+def route_experts_f16(logits, bias, ids, weights, tokens, experts, top, stream, score=SOFTMAX, groups=1, top_groups=1,
+                      group_best=2, renormalize=True, scale=1.0) -> None:
+    """The `top` experts of each token and their weights.  `bias` None: none."""
+    check(
+        lib().mote_hip_route_experts_f16(
+            logits, bias, ids, weights, tokens, experts, top, score, groups, top_groups, group_best,
+            int(renormalize), scale, _s(stream)
+        ),
+        "launch expert routing kernel",
+    )
+
+
+def route_experts_f32(logits, bias, ids, weights, tokens, experts, top, stream, score=SOFTMAX, groups=1, top_groups=1,
+                      group_best=2, renormalize=True, scale=1.0) -> None:
+    check(
+        lib().mote_hip_route_experts_f32(
+            logits, bias, ids, weights, tokens, experts, top, score, groups, top_groups, group_best,
+            int(renormalize), scale, _s(stream)
+        ),
+        "launch expert routing kernel",
+    )
+
+
+def plan_experts(ids, offsets, rows, tokens, top, experts, stream) -> None:
+    """The (token, choice) pairs in the order of their experts."""
+    check(lib().mote_hip_plan_experts(ids, offsets, rows, tokens, top, experts, _s(stream)),
+          "launch expert plan kernel")
+
+
+def experts_gate_up_silu_mx_f16(x, x_scales, w, w_scales, offsets, rows, h, tokens, top, experts, hidden, inner,
+                                x_bits, stream) -> None:
+    """silu(x gate^T) (x up^T) of every row of the plan with its expert's weights."""
+    check(
+        lib().mote_hip_experts_gate_up_silu_mx_f16(
+            x, x_scales, w, w_scales, offsets, rows, h, tokens, top, experts, hidden, inner, x_bits, _s(stream)
+        ),
+        "launch experts' gate/up kernel",
+    )
+
+
+def experts_down_workspace(tokens, top, experts, hidden, inner) -> int:
+    """Bytes of workspace that experts_down_mx_f16 needs for these sizes."""
+    need = ctypes.c_size_t(0)
+    check(lib().mote_hip_experts_down_workspace(tokens, top, experts, hidden, inner, ctypes.byref(need)),
+          "size experts' down workspace")
+    return need.value
+
+
+def experts_down_mx_f16(h, h_scales, w, w_scales, ids, offsets, rows, pair_weights, y, tokens, top, experts, hidden,
+                        inner, h_bits, workspace, workspace_bytes, stream) -> None:
+    """The weighted sum of each token's experts' down projections."""
+    check(
+        lib().mote_hip_experts_down_mx_f16(
+            h, h_scales, w, w_scales, ids, offsets, rows, pair_weights, y, tokens, top, experts, hidden, inner,
+            h_bits, workspace, workspace_bytes, _s(stream)
+        ),
+        "launch experts' down kernel",
     )
 
 
