@@ -52,6 +52,16 @@ __device__ __forceinline__ uint32_t scale_of(uint32_t most) {
     return e > 2 ? e - 2 : 0;
 }
 
+// The conversions of a whole block write their result in several passes while they still read, and the
+// compiler gives result and operand the same registers where it can: elements then came out
+// as others' bits.  So their operands are said to be in use a little longer.
+template <typename V>
+__device__ __forceinline__ void still_used(const V& v) {
+#ifdef __HIP_DEVICE_COMPILE__
+    asm volatile("" ::"v"(v));
+#endif
+}
+
 template <int BITS>
 __device__ __forceinline__ Block<BITS> convert(const _Float16 (&x)[32], float scale) {
     Block<BITS> b;
@@ -71,6 +81,8 @@ __device__ __forceinline__ Block<BITS> convert(const _Float16 (&x)[32], float sc
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = x[i];
         const u32x6 w = __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(v, scale);
+        still_used(v);
+        still_used(scale);
         b.low = u32x4{w[0], w[1], w[2], w[3]};
         b.high = u32x2{w[4], w[5]};
     }
@@ -98,6 +110,9 @@ __device__ __forceinline__ Block<BITS> convert(const float (&x)[32], float scale
             odd[i] = x[2 * i + 1];
         }
         const u32x6 w = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale);
+        still_used(even);
+        still_used(odd);
+        still_used(scale);
         b.low = u32x4{w[0], w[1], w[2], w[3]};
         b.high = u32x2{w[4], w[5]};
     }
@@ -160,39 +175,58 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
     return byte == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, bits);
 }
 
+// The blocks leave through LDS, so that a wave's stores are each 1024 bytes in a row.
 template <typename T, int BITS>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(RowArgs a) {
+    constexpr int kPer = 16 / sizeof(T), kPieces = 32 / kPer;  // 16-byte pieces of a block
+    constexpr int kRoom = kPieces * 16 + 16;                   // 16 bytes more: 8 lanes touch all banks
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kThreads / 64][64 * kRoom];
     uint64_t row;
     uint32_t block;
-    if (!block_of(a, row, block) || block >= a.blocks) return;
-    const Block<BITS> b = load_block<BITS>(a.values_in + row * value_bytes(a.kp, BITS), a.kp, block);
-    const float scale = scale_value(a.scales[row * scale_bytes(a.kp) + block]);
-    float v[32];
-    if constexpr (BITS == 4) {
+    const bool there = block_of(a, row, block) && block < a.blocks;
+    const uint32_t lane = threadIdx.x & 63;
+    uint8_t* const turn = lds[threadIdx.x >> 6];
+    uint64_t to = 0;  // where the block goes; 0: nowhere
+    if (there) {
+        const Block<BITS> b = load_block<BITS>(a.values_in + row * value_bytes(a.kp, BITS), a.kp, block);
+        const float scale = scale_value(a.scales[row * scale_bytes(a.kp) + block]);
+        float v[32];
+        if constexpr (BITS == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const auto pair = [&](int at, f32x2 p) { v[8 * i + 2 * at] = p.x, v[8 * i + 2 * at + 1] = p.y; };
-            pair(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 0));
-            pair(1, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 1));
-            pair(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 2));
-            pair(3, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 3));
+            for (int i = 0; i < 4; ++i) {
+                const auto pair = [&](int at, f32x2 p) { v[8 * i + 2 * at] = p.x, v[8 * i + 2 * at + 1] = p.y; };
+                pair(0, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 0));
+                pair(1, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 1));
+                pair(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 2));
+                pair(3, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(b.low[i], 1.0f, 3));
+            }
+        } else {
+            const u32x6 codes = {b.low.x, b.low.y, b.low.z, b.low.w, b.high.x, b.high.y};
+            const f32x32 w = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(codes, 1.0f);
+            still_used(codes);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = w[i];
         }
-    } else {
-        const f32x32 w = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(
-            u32x6{b.low.x, b.low.y, b.low.z, b.low.w, b.high.x, b.high.y}, 1.0f);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = w[i];
+        for (int i = 0; i < kPieces; ++i) {
+            T part[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) part[j] = to_out<T>(v[i * kPer + j] * scale);
+            u32x4 word;
+            __builtin_memcpy(&word, part, 16);
+            *reinterpret_cast<u32x4*>(turn + lane * kRoom + 16 * i) = word;
+        }
+        to = reinterpret_cast<uint64_t>(static_cast<T*>(a.output) + row * a.stride + block * kBlock);
     }
-    T* out = static_cast<T*>(a.output) + row * a.stride + block * kBlock;
-    constexpr int kPer = 16 / sizeof(T);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int i = 0; i < 32 / kPer; ++i) {
-        T part[kPer];
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) part[j] = to_out<T>(v[i * kPer + j] * scale);
-        u32x4 word;
-        __builtin_memcpy(&word, part, 16);
-        *reinterpret_cast<u32x4_a2*>(out + i * kPer) = word;
+    for (int i = 0; i < kPieces; ++i) {
+        const uint32_t piece = i * 64 + lane, of = piece / kPieces;
+        const uint64_t begin = __shfl(to, of, 64);
+        if (begin == 0) continue;
+        *reinterpret_cast<u32x4_a2*>(begin + piece % kPieces * 16) =
+            *reinterpret_cast<const u32x4*>(turn + of * kRoom + piece % kPieces * 16);
     }
 }
 
