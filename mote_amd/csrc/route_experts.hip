@@ -17,7 +17,7 @@
 #include <cstdint>
 #include <cmath>
 
-#include "mx.hpp"
+#include "mx_products.hpp"
 
 namespace mote::mx {
 namespace {
@@ -118,20 +118,32 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     if constexpr (GROUPED) {
 #pragma unroll
         for (int v = 0; v < SLOTS; ++v) choices[wave][v * 64 + lane] = choice[v];
-        // (One wave's LDS operations keep their order.)
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        for (uint32_t g = lane; g < a.groups; g += 64) {
+        __builtin_amdgcn_wave_barrier();
+        // `part` lanes share a group: its choices in turn, then their bests across the lanes.
+        uint32_t part = 1;
+        while (part * 2 * a.groups <= 64) part *= 2;
+        for (uint32_t first_group = 0; first_group < a.groups; first_group += 64 / part) {
+            const uint32_t g = first_group + lane / part;
             uint64_t first = 0, second = 0;
-            for (uint32_t i = 0; i < a.size; ++i) {
-                const uint64_t c = choices[wave][g * a.size + i];
-                second = max(second, min(first, c));
+            if (g < a.groups) {
+                for (uint32_t i = lane % part; i < a.size; i += part) {
+                    const uint64_t c = choices[wave][g * a.size + i];
+                    second = max(second, min(first, c));
+                    first = max(first, c);
+                }
+            }
+            for (uint32_t by = 1; by < part; by *= 2) {
+                const uint64_t c = __shfl_xor(first, by, 64), d = __shfl_xor(second, by, 64);
+                second = max(max(second, d), min(first, c));
                 first = max(first, c);
             }
             double worth = first ? value_of(first) : 0.0;
             if (a.best == 2 && second) worth += value_of(second);
-            worths[wave][g] = first ? order_of(worth) : 0;
+            if (g < a.groups && lane % part == 0) worths[wave][g] = first ? order_of(worth) : 0;
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
         // Groups that fewer than top_groups others come before.
 #pragma unroll
         for (int v = 0; v < SLOTS; ++v) {
@@ -201,49 +213,88 @@ struct PlanArgs {
 };
 
 // A workgroup for each expert: it counts the pairs of lower experts, which is where its own
-// begin, and its own, wave by wave over runs of the pairs, then writes its own in their order.
-// No counter is shared, so the order is always the same.
+// begin, and its own, then writes its own in their order.  No counter is shared, so the order is
+// always the same.  A thread has a run of neighbouring pairs, up to kRun of them in its registers
+// (so up to 32768 pairs are read once); more go by in rounds that are counted first.
 constexpr uint32_t kPlanThreads = 1024;
+constexpr uint32_t kRun = 32;
 
-__device__ __forceinline__ uint32_t expert_of(const PlanArgs& a, uint32_t p) {  // kMostExperts on: none
-    return p < a.pairs ? min(static_cast<uint32_t>(a.ids[p]), kMostExperts) : kMostExperts;
+struct Run {
+    uint32_t expert[kRun];
+};
+__device__ __forceinline__ void load_run(const PlanArgs& a, uint32_t first, uint32_t per, Run& run) {
+    typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+    for (uint32_t i = 0; i < kRun; i += 4) {
+        if (i < per && first + i + 4 <= a.pairs) {
+            const i32x4_a4 four = *reinterpret_cast<const i32x4_a4*>(a.ids + first + i);
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) run.expert[i + j] = static_cast<uint32_t>(four[j]);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                run.expert[i + j] = i < per && first + i + j < a.pairs ? static_cast<uint32_t>(a.ids[first + i + j]) : ~0u;
+        }
+    }
 }
 
-__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a) {
-    constexpr uint32_t kWaves = kPlanThreads / 64;
-    __shared__ uint32_t lower_of[kWaves], own_of[kWaves];
+// per: pairs of a thread's run in a round, a multiple of 4 up to kRun.
+__global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a, uint32_t per) {
+    __shared__ uint32_t lower_of[kPlanThreads / 64], own_of[kPlanThreads / 64];
     const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
     const uint32_t expert = blockIdx.x;
-    const uint32_t run = ((a.pairs + waves - 1) / waves + 63) & ~63u;  // pairs of a wave
-    const uint32_t first = min(wave * run, a.pairs), last = min(first + run, a.pairs);
-    uint32_t lower = 0, own = 0;
-    for (uint32_t p = first; p < last; p += 64) {
-        const uint32_t e = p + lane < last ? expert_of(a, p + lane) : kMostExperts;
-        lower += __builtin_popcountll(__builtin_amdgcn_ballot_w64(e < expert));
-        own += __builtin_popcountll(__builtin_amdgcn_ballot_w64(e == expert));
+    const uint32_t round = blockDim.x * per, rounds = max((a.pairs + round - 1) / round, 1u);
+    const uint32_t mine = threadIdx.x * per;
+    Run run;
+    uint32_t lower = 0, all = 0;  // of this thread, all rounds
+    for (uint32_t r = 0; r < rounds; ++r) {
+        load_run(a, r * round + mine, per, run);
+#pragma unroll
+        for (uint32_t i = 0; i < kRun; ++i) {
+            lower += run.expert[i] < expert ? 1 : 0;
+            all += run.expert[i] == expert ? 1 : 0;
+        }
     }
-    if (lane == 0) {
-        lower_of[wave] = lower;
-        own_of[wave] = own;
+    // Those of the workgroup, and in one round those of the threads before.
+    const uint32_t lower_before = lanes_before(lower), own_before = lanes_before(all);
+    if (lane == 63) {
+        lower_of[wave] = lower_before + lower;
+        own_of[wave] = own_before + all;
     }
     __syncthreads();
-    uint32_t begin = 0, all = 0, before = 0;
+    uint32_t begin = 0, total = 0, before = own_before;
     for (uint32_t w = 0; w < waves; ++w) {
         begin += lower_of[w];
-        all += own_of[w];
+        total += own_of[w];
         if (w < wave) before += own_of[w];
     }
-    uint32_t at = begin + before;
-    for (uint32_t p = first; p < last && own > 0; p += 64) {
-        const uint32_t e = p + lane < last ? expert_of(a, p + lane) : kMostExperts;
-        const uint64_t mine = __builtin_amdgcn_ballot_w64(e == expert);
-        const uint32_t under = __builtin_popcountll(mine & ((uint64_t{1} << lane) - 1));
-        if (e == expert) a.rows[at + under] = static_cast<int32_t>(p + lane);
-        at += __builtin_popcountll(mine);
+    uint32_t at = begin;
+    for (uint32_t r = 0; r < rounds && total > 0; ++r) {
+        uint32_t own = all, own_total = total;
+        if (rounds > 1) {
+            load_run(a, r * round + mine, per, run);
+            own = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kRun; ++i) own += run.expert[i] == expert ? 1 : 0;
+            before = lanes_before(own);
+            __syncthreads();  // the sums of the round before have been read
+            if (lane == 63) own_of[wave] = before + own;
+            __syncthreads();
+            own_total = 0;
+            for (uint32_t w = 0; w < waves; ++w) {
+                own_total += own_of[w];
+                if (w < wave) before += own_of[w];
+            }
+        }
+        uint32_t to = at + before;
+#pragma unroll
+        for (uint32_t i = 0; i < kRun; ++i)
+            if (run.expert[i] == expert) a.rows[to++] = static_cast<int32_t>(r * round + mine + i);
+        at += own_total;
     }
     if (threadIdx.x == 0) a.offsets[expert] = static_cast<int32_t>(begin);
     if (expert + 1 == a.experts) {
-        const uint32_t end = begin + all;
+        const uint32_t end = begin + total;
         if (threadIdx.x == 0) a.offsets[a.experts] = static_cast<int32_t>(end);
         for (uint32_t p = end + threadIdx.x; p < a.pairs; p += blockDim.x) a.rows[p] = -1;
     }
@@ -329,9 +380,10 @@ MOTE_EXPORT int mote_hip_plan_experts(const void* ids, void* offsets, void* rows
     if (experts == 0) return 0;
     const PlanArgs a{static_cast<const int32_t*>(ids), static_cast<int32_t*>(offsets), static_cast<int32_t*>(rows),
                      static_cast<uint32_t>(tokens * top), static_cast<uint32_t>(experts)};
-    // A wave for each 64 pairs, sixteen at most.
-    const uint32_t waves = a.pairs >= kPlanThreads ? kPlanThreads / 64 : (a.pairs + 63) / 64;
-    hipLaunchKernelGGL(plan_kernel, dim3(a.experts), dim3((waves ? waves : 1) * 64), 0,
-                       static_cast<hipStream_t>(stream), a);
+    // Four pairs a thread, more where a thousand threads do not take them all.
+    const uint32_t waves = a.pairs >= kPlanThreads * 4 ? kPlanThreads / 64 : max((a.pairs + 255) / 256, 1u);
+    const uint32_t each = (a.pairs + waves * 64 - 1) / (waves * 64);
+    const uint32_t per = min((max(each, 1u) + 3) & ~3u, kRun);
+    hipLaunchKernelGGL(plan_kernel, dim3(a.experts), dim3(waves * 64), 0, static_cast<hipStream_t>(stream), a, per);
     return static_cast<int>(hipGetLastError());
 }
