@@ -82,9 +82,8 @@ __device__ __forceinline__ Block<BITS> load_block(const uint8_t* row, uint32_t k
 // l holds block l / 16 of rows l % 16, and of D column j = l % 16, rows 4 (l / 16) + r.
 // Scales are the lanes' low bytes.
 template <int BITS>
-__device__ __forceinline__ f32x4 multiply16(const Block<4>& w, uint32_t w_scale, const Block<BITS>& x, uint32_t x_scale,
-                                            f32x4 d) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.operand(), x.operand(), d, kFormat<4>, kFormat<BITS>, 0,
+__device__ __forceinline__ f32x4 multiply16(i32x8 w, uint32_t w_scale, i32x8 x, uint32_t x_scale, f32x4 d) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, d, kFormat<4>, kFormat<BITS>, 0,
                                                             static_cast<int>(w_scale), 0, static_cast<int>(x_scale));
 }
 

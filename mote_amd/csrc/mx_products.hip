@@ -2,94 +2,134 @@
 // weights and rows.
 #include <hip/hip_runtime.h>
 
-#include <cmath>
+#include <algorithm>
 #include <cstdint>
+#include <utility>
 
 #include "mx_products.hpp"
 
 namespace mote::mx {
 namespace {
 
-// Few rows: HBM-bound on the weights.  A workgroup has 16 of the outputs (of gate and of
-// up each) and up to 64 rows in 16-row fragments, of which only those that hold rows are
-// multiplied; its waves divide the steps of K among them, two at a time, and add
-// their sums through LDS, in the waves' order.  A lane's operand is a 16-byte piece of
-// a weights' row as it is stored, so nothing is unpacked; the activations come from L2.
-constexpr uint32_t kFewRows = 64;
+// Few rows: HBM-bound on the weights.  A workgroup has one tile of up to 16 rows and the
+// columns part, part + parts, ... of 16 outputs (of gate and of up each).  A wave has
+// STEPS steps of K, the same for every column, and the waves' sums meet in LDS, in their order.
+//
+// A lane's operand is a 16-byte piece of a weights' row as it is stored, so nothing is
+// unpacked; what costs time beside the memory is the number of load instructions (14336 x 4096,
+// 31 MB that are read in 6.1 us at best: weights alone 6.9 us, with their scales a word at a
+// time and x at each step 11.5).  So scales are loaded four steps at a time, x once for all
+// of the workgroup's columns, and a step's weights for the next column as soon as they
+// have been multiplied.
+constexpr uint32_t kFewRows = 16;
 
-template <int BITS, Result R, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs a, uint32_t column_tiles) {
-    constexpr int kFragments = kFewRows / 16;
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+
+template <int BITS, Result R, int STEPS, int MOST_WAVES>
+__global__ __launch_bounds__(MOST_WAVES * 64) void few_rows_kernel(ProductArgs a, uint32_t parts) {
     constexpr int kSides = R == Result::kGateUp ? 2 : 1;
-    __shared__ f32x4 sums[WAVES][kSides][kFragments][64];
-    const uint32_t unit = blockIdx.x / column_tiles, column = blockIdx.x % column_tiles * 16;
+    typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+    extern __shared__ f32x4 sums[];  // [2][waves][kSides][64]
+    const uint32_t unit = blockIdx.x / parts, part = blockIdx.x % parts;
     const Tile tile = find_tile<R, kFewRows>(a, unit);
     if (tile.count == 0) return;
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, of16 = lane & 15, group = lane >> 4;
-    const uint32_t steps = a.kp / kStep;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const uint32_t lane = threadIdx.x & 63, of16 = lane & 15, group = lane >> 4;
+    const uint32_t columns = (a.outputs + 15) / 16;
+    const uint32_t steps = a.kp / kStep, first = wave * STEPS;
+    const uint32_t mine = first < steps ? min(steps - first, uint32_t{STEPS}) : 0;
+    const auto step_at = [&](int i) { return min(first + i, steps - 1); };  // past the end the last again, unused
+    const auto each_step = [](auto does) { each_of(does, std::make_integer_sequence<int, STEPS>{}); };
 
+    u32x4 w[STEPS][kSides];
+    uint32_t ws[STEPS][kSides];
     const uint8_t* w_row[kSides];
-    const uint8_t* w_scale[kSides];
-#pragma unroll
-    for (int side = 0; side < kSides; ++side) {
-        const uint64_t row = (static_cast<uint64_t>(tile.expert) * kSides + side) * a.outputs +
-                             min(column + of16, a.outputs - 1);
-        w_row[side] = a.w + row * value_bytes(a.kp, 4);
-        w_scale[side] = a.w_scales + row * scale_bytes(a.kp);
-    }
-    const uint8_t* x_row[kFragments];
-    const uint8_t* x_scale[kFragments];
-    const uint32_t fragments = (tile.count + 15) / 16;
-#pragma unroll
-    for (int f = 0; f < kFragments; ++f) {
-        const uint64_t row = input_row<R>(a, tile.first + min(f * 16 + of16, tile.count - 1));
-        x_row[f] = a.x + row * value_bytes(a.kp, BITS);
-        x_scale[f] = a.x_scales + row * scale_bytes(a.kp);
-    }
-
-    f32x4 d[kSides][kFragments] = {};
-    for (uint32_t first = wave * 2; first < steps; first += WAVES * 2) {
-#pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) {
-            const uint32_t step = first + j;
-            if (step >= steps) break;
-            const uint32_t block = step * 4 + group;
-            Block<4> w[kSides];
-            uint32_t ws[kSides];
-#pragma unroll
-            for (int side = 0; side < kSides; ++side) {
-                w[side] = load_block<4>(w_row[side], a.kp, block);
-                ws[side] = reinterpret_cast<const uint32_t*>(w_scale[side])[step] >> (8 * group);
-            }
-#pragma unroll
-            for (int f = 0; f < kFragments; ++f) {
-                if (static_cast<uint32_t>(f) >= fragments) break;
-                const Block<BITS> x = load_block<BITS>(x_row[f], a.kp, block);
-                const uint32_t xs = reinterpret_cast<const uint32_t*>(x_scale[f])[step] >> (8 * group);
-#pragma unroll
-                for (int side = 0; side < kSides; ++side)
-                    d[side][f] = multiply16<BITS>(w[side], ws[side], x, xs, d[side][f]);
-            }
-        }
-    }
-#pragma unroll
-    for (int side = 0; side < kSides; ++side)
-#pragma unroll
-        for (int f = 0; f < kFragments; ++f)
-            if (static_cast<uint32_t>(f) < fragments) sums[wave][side][f][lane] = d[side][f];
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < fragments * 64; i += WAVES * 64) {
-        const uint32_t f = i / 64, l = i % 64;
-        const uint32_t row = f * 16 + (l & 15), n = column + 4 * (l >> 4);
-        if (row >= tile.count || n >= a.outputs) continue;
-        f32x4 total[kSides];
+    const auto to_column = [&](uint32_t column) {  // and its scales
 #pragma unroll
         for (int side = 0; side < kSides; ++side) {
-            total[side] = sums[0][side][f][l];
+            const uint64_t row = (static_cast<uint64_t>(tile.expert) * kSides + side) * a.outputs +
+                                 min(column * 16 + of16, a.outputs - 1);
+            w_row[side] = a.w + row * value_bytes(a.kp, 4);
+            const uint32_t* scales = reinterpret_cast<const uint32_t*>(a.w_scales + row * scale_bytes(a.kp));
+            if (mine == STEPS) {
 #pragma unroll
-            for (int v = 1; v < WAVES; ++v) total[side] += sums[v][side][f][l];
+                for (int i = 0; i < STEPS; i += 4) {
+                    const u32x4 four = *reinterpret_cast<const u32x4_a4*>(scales + first + i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) ws[i + j][side] = four[j];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < STEPS; ++i) ws[i][side] = scales[step_at(i)];
+            }
         }
-        uint64_t to = tile.first + row;
+    };
+    const auto load_w = [&](auto at) {
+        constexpr int I = decltype(at)::value;
+#pragma unroll
+        for (int side = 0; side < kSides; ++side)
+            w[I][side] = *reinterpret_cast<const u32x4*>(w_row[side] + step_at(I) * 64 + group * 16);
+    };
+    i32x8 x[STEPS];
+    uint32_t xs[STEPS];
+    if (mine > 0) {
+        to_column(part);
+        each_step(load_w);
+        const uint64_t row = input_row<R>(a, tile.first + min(of16, tile.count - 1));
+        const uint8_t* const values = a.x + row * value_bytes(a.kp, BITS);
+        const uint32_t* const scales = reinterpret_cast<const uint32_t*>(a.x_scales + row * scale_bytes(a.kp));
+        each_step([&](auto at) {
+            constexpr int I = decltype(at)::value;
+            x[I] = load_block<BITS>(values, a.kp, step_at(I) * 4 + group).operand();
+            xs[I] = scales[step_at(I)] >> (8 * group);
+        });
+    }
+    uint32_t buffer = 0, turn = 0;
+    for (uint32_t column = part; column < columns; column += parts, buffer ^= 1) {
+        f32x4 d[kSides] = {};
+        if (mine > 0) {
+            uint32_t now[STEPS][kSides];
+#pragma unroll
+            for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+                for (int side = 0; side < kSides; ++side) now[i][side] = ws[i][side] >> (8 * group);
+            const auto multiply = [&](auto at) {
+                constexpr int I = decltype(at)::value;
+                if (static_cast<uint32_t>(I) < mine) {
+#pragma unroll
+                    for (int side = 0; side < kSides; ++side)
+                        d[side] = multiply16<BITS>(Block<4>{w[I][side]}.operand(), now[I][side], x[I], xs[I], d[side]);
+                }
+            };
+            if (column + parts < columns) {
+                to_column(column + parts);
+                each_step([&](auto at) {
+                    multiply(at);
+                    load_w(at);
+                });
+            } else {
+                each_step(multiply);
+            }
+        }
+        f32x4* const of_buffer = sums + buffer * waves * (kSides * 64);
+#pragma unroll
+        for (int side = 0; side < kSides; ++side) of_buffer[(wave * kSides + side) * 64 + lane] = d[side];
+        __syncthreads();  // (Two buffers: the one before has been read by all who are past this.)
+        // The waves take turns, so that one adds while the others go on.
+        const bool this_wave = turn == wave;
+        turn = turn + 1 == waves ? 0 : turn + 1;
+        if (!this_wave) continue;
+        const uint32_t n = column * 16 + 4 * group;
+        f32x4 total[kSides] = {};
+        for (uint32_t v = 0; v < waves; ++v) {
+#pragma unroll
+            for (int side = 0; side < kSides; ++side) total[side] += of_buffer[(v * kSides + side) * 64 + lane];
+        }
+        if (of16 >= tile.count || n >= a.outputs) continue;
+        uint64_t to = tile.first + of16;
         if constexpr (R == Result::kPairs) {
             to = static_cast<uint32_t>(a.plan[to]);
             if (to >= a.rows) continue;
@@ -99,7 +139,8 @@ __global__ __launch_bounds__(WAVES * 64) void few_rows_kernel(ProductArgs a, uin
         for (uint32_t r = 0; r < 4; ++r) {
             if (n + r >= a.outputs) break;
             if constexpr (R == Result::kGateUp)
-                static_cast<_Float16*>(a.output)[to + r] = static_cast<_Float16>(silu(total[0][r]) * total[kSides - 1][r]);
+                static_cast<_Float16*>(a.output)[to + r] =
+                    static_cast<_Float16>(silu(total[0][r]) * total[kSides - 1][r]);
             else if constexpr (R == Result::kF16)
                 static_cast<_Float16*>(a.output)[to + r] = static_cast<_Float16>(total[0][r]);
             else
@@ -119,30 +160,61 @@ struct CombineArgs {
 };
 __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
     const uint32_t token = blockIdx.x / a.parts;
-    const uint32_t n = (blockIdx.x % a.parts) * 256 + threadIdx.x;
+    const uint32_t n = ((blockIdx.x % a.parts) * 256 + threadIdx.x) * 4;  // four outputs: hidden is whole blocks
     if (n >= a.hidden) return;
-    float y = 0.0f;
+    f32x4 y = {};
     for (uint32_t j = 0; j < a.top; ++j) {
         const uint64_t pair = static_cast<uint64_t>(token) * a.top + j;
         if (static_cast<uint32_t>(a.ids[pair]) >= a.experts) continue;
-        y = __builtin_fmaf(a.weights[pair], a.products[pair * a.hidden + n], y);
+        const f32x4 product = *reinterpret_cast<const f32x4*>(a.products + pair * a.hidden + n);
+        const float weight = a.weights[pair];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[r] = __builtin_fmaf(weight, product[r], y[r]);
     }
-    a.output[static_cast<uint64_t>(token) * a.hidden + n] = static_cast<_Float16>(y);
+    typedef _Float16 f16x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
+    *reinterpret_cast<f16x4_a2*>(a.output + static_cast<uint64_t>(token) * a.hidden + n) =
+        f16x4_a2{static_cast<_Float16>(y[0]), static_cast<_Float16>(y[1]), static_cast<_Float16>(y[2]),
+                 static_cast<_Float16>(y[3])};
+}
+
+// Columns of a workgroup: more of them share the loads of x, but there have to be workgroups
+// enough (one row, 14336 x 4096: 10.3 us with one, 9.0 with two, 9.6 with four of 224
+// workgroups; 4096 x 4096, 256 columns: 4.2 with one, 5.2 with two).
+constexpr uint64_t kWorkgroups = 448, kMostColumns = 4;
+
+template <int BITS, Result R, int STEPS, int MOST_WAVES>
+int launch_few(const ProductArgs& a, hipStream_t stream) {
+    constexpr uint32_t kSides = R == Result::kGateUp ? 2 : 1;
+    const uint32_t columns = (a.outputs + 15) / 16, steps = a.kp / kStep;
+    const uint64_t units = kOfExperts<R> ? most_expert_tiles(a.rows, a.experts, kFewRows)
+                                         : (uint64_t{a.rows} + kFewRows - 1) / kFewRows;
+    const uint64_t each = std::min(std::max(units * columns / kWorkgroups, uint64_t{1}), kMostColumns);
+    const uint32_t parts = static_cast<uint32_t>((columns + each - 1) / each);
+    const uint32_t waves = steps > STEPS ? (steps + STEPS - 1) / STEPS : 1;
+    if (units * parts > kMostThreads / (waves * 64)) return kInvalid;
+    hipLaunchKernelGGL((few_rows_kernel<BITS, R, STEPS, MOST_WAVES>), dim3(static_cast<uint32_t>(units * parts)),
+                       dim3(waves * 64), 2 * waves * kSides * 1024, stream, a, parts);
+    return static_cast<int>(hipGetLastError());
+}
+
+// Few rows up to 16, or fewer than 8 of an expert in the mean (32 experts of 2880 x 2880, gate/up: 2
+// rows each 45 us and 51 in tiles, 8 rows 63 and 66, 16 rows 88 and 83); where K is too long for the
+// waves of a workgroup, or too short for the tiles' four steps, the other kernel has them.
+template <int BITS, Result R>
+int launch_bits(const ProductArgs& a, hipStream_t stream) {
+    constexpr bool kTwo = R == Result::kGateUp;  // twice the registers: no eight steps of K a wave
+    const uint32_t steps = a.kp / kStep;
+    const bool few = kOfExperts<R> ? a.rows < 8 * uint64_t{a.experts} : a.rows <= kFewRows;
+    if (steps >= 4 && (!few || steps > (kTwo ? 64 : 128))) return launch_tiles(R, a, BITS, stream);
+    if constexpr (!kTwo) {
+        if (steps > 64) return launch_few<BITS, R, 8, 16>(a, stream);
+    }
+    return launch_few<BITS, R, 4, 16>(a, stream);
 }
 
 template <Result R>
 int launch(const ProductArgs& a, int bits, hipStream_t stream) {
-    const uint32_t column_tiles = (a.outputs + 15) / 16;
-    const uint64_t units = kOfExperts<R> ? most_expert_tiles(a.rows, a.experts, kFewRows)
-                                         : (uint64_t{a.rows} + kFewRows - 1) / kFewRows;
-    constexpr uint32_t kWaves = 8;
-    if (units * column_tiles > kMostThreads / (kWaves * 64)) return kInvalid;
-    const auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(units * column_tiles)), dim3(kWaves * 64), 0, stream, a,
-                           column_tiles);
-    };
-    bits == 4 ? go(few_rows_kernel<4, R, kWaves>) : go(few_rows_kernel<6, R, kWaves>);
-    return static_cast<int>(hipGetLastError());
+    return bits == 4 ? launch_bits<4, R>(a, stream) : launch_bits<6, R>(a, stream);
 }
 
 // Sizes and addresses that every product needs.
@@ -246,7 +318,7 @@ MOTE_EXPORT int mote_hip_experts_down_mx_f16(const void* input_values, const voi
     if (tokens == 0 || hidden == 0) return 0;
     const uint64_t need = down_bytes(tokens * top, hidden);
     if (need > 0 && (!workspace || off_grid(workspace, 16) || workspace_bytes < need)) return kInvalid;
-    const uint32_t parts = static_cast<uint32_t>((hidden + 255) / 256);
+    const uint32_t parts = static_cast<uint32_t>((hidden + 1023) / 1024);
     if (tokens * parts > kMostThreads / 256) return kInvalid;
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (top > 0 && experts > 0) {

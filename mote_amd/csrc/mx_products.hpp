@@ -5,8 +5,6 @@
 #include "mx.hpp"
 
 namespace mote::mx {
-namespace {
-
 
 // What a product's outputs become.
 enum class Result {
@@ -15,9 +13,6 @@ enum class Result {
     kGateUp,  // silu(gate) up of an expert's 2 outputs weight rows, binary16, row i of the plan
     kPairs,   // row i of the plan to the row of its pair, 32 bits (an expert's down projection)
 };
-template <Result R>
-constexpr bool kOfExperts = R == Result::kGateUp || R == Result::kPairs;
-
 struct ProductArgs {
     const uint8_t* x;        // values of the rows
     const uint8_t* x_scales;
@@ -32,11 +27,34 @@ struct ProductArgs {
     uint32_t experts, top;
 };
 
+// Products of many rows (mx_tiles.hip).
+int launch_tiles(Result result, const ProductArgs& a, int bits, hipStream_t stream);
+
+namespace {
+
+template <Result R>
+constexpr bool kOfExperts = R == Result::kGateUp || R == Result::kPairs;
+
 // The rows of one tile: an expert's, `count` of them (0: no such tile) from row `first` of the
 // plan, or a linear's.
 struct Tile {
     uint32_t expert, first, count;
 };
+
+// The sum of v over the lanes before.
+template <int Ctrl, int RowMask>
+__device__ __forceinline__ uint32_t add_dpp(uint32_t v) {
+    return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), Ctrl, RowMask, 0xF, false));
+}
+__device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
+    uint32_t sum = add_dpp<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    sum = add_dpp<0x112, 0xF>(sum);
+    sum = add_dpp<0x114, 0xF>(sum);
+    sum = add_dpp<0x118, 0xF>(sum);
+    sum = add_dpp<0x142, 0xA>(sum);  // row_bcast:15 into rows 1 and 3
+    sum = add_dpp<0x143, 0xC>(sum);  // row_bcast:31 into rows 2 and 3
+    return sum - v;
+}
 
 // Tile `unit` of the experts' tiles of PER rows: each expert has its rows / PER of
 // them, rounded up.  Every wave looks it up by itself: lane l counts those of its run
@@ -58,12 +76,7 @@ __device__ __forceinline__ Tile expert_tile(const ProductArgs& a, uint32_t unit)
             from = to;
         }
     }
-    uint32_t upto = mine;  // tiles of this lane's experts and the lanes' before
-#pragma unroll
-    for (int by = 1; by < 64; by *= 2) {
-        const uint32_t other = __shfl_up(upto, by, 64);
-        if (lane >= static_cast<uint32_t>(by)) upto += other;
-    }
+    const uint32_t upto = lanes_before(mine) + mine;  // tiles of this lane's experts and the lanes' before
     const uint64_t before = __builtin_amdgcn_ballot_w64(upto <= unit);
     const uint32_t owner = __builtin_popcountll(before);
     if (owner == 64) return {0, 0, 0};
