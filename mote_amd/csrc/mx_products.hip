@@ -34,7 +34,7 @@ __global__ __launch_bounds__(MOST_WAVES * 64) void few_rows_kernel(ProductArgs a
     typedef uint32_t u32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
     extern __shared__ f32x4 sums[];  // [2][waves][kSides][64]
     const uint32_t unit = blockIdx.x / parts, part = blockIdx.x % parts;
-    const Tile tile = find_tile<R, kFewRows>(a, unit);
+    const Tile tile = Tiles<R, kFewRows>(a).at(a, unit);
     if (tile.count == 0) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const uint32_t lane = threadIdx.x & 63, of16 = lane & 15, group = lane >> 4;
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(MOST_WAVES * 64) void few_rows_kernel(ProductArgs a
             if (n + r >= a.outputs) break;
             if constexpr (R == Result::kGateUp)
                 static_cast<_Float16*>(a.output)[to + r] =
-                    static_cast<_Float16>(silu(total[0][r]) * total[kSides - 1][r]);
+                    static_cast<_Float16>(silu_product(total[0][r], total[kSides - 1][r]));
             else if constexpr (R == Result::kF16)
                 static_cast<_Float16*>(a.output)[to + r] = static_cast<_Float16>(total[0][r]);
             else
@@ -197,14 +197,14 @@ int launch_few(const ProductArgs& a, hipStream_t stream) {
     return static_cast<int>(hipGetLastError());
 }
 
-// Few rows up to 16, or fewer than 8 of an expert in the mean (32 experts of 2880 x 2880, gate/up: 2
+// Few rows up to 16, or 8 of an expert in the mean (32 experts of 2880 x 2880, gate/up: 2
 // rows each 45 us and 51 in tiles, 8 rows 63 and 66, 16 rows 88 and 83); where K is too long for the
 // waves of a workgroup, or too short for the tiles' four steps, the other kernel has them.
 template <int BITS, Result R>
 int launch_bits(const ProductArgs& a, hipStream_t stream) {
     constexpr bool kTwo = R == Result::kGateUp;  // twice the registers: no eight steps of K a wave
     const uint32_t steps = a.kp / kStep;
-    const bool few = kOfExperts<R> ? a.rows < 8 * uint64_t{a.experts} : a.rows <= kFewRows;
+    const bool few = kOfExperts<R> ? a.rows <= 8 * uint64_t{a.experts} : a.rows <= kFewRows;
     if (steps >= 4 && (!few || steps > (kTwo ? 64 : 128))) return launch_tiles(R, a, BITS, stream);
     if constexpr (!kTwo) {
         if (steps > 64) return launch_few<BITS, R, 8, 16>(a, stream);

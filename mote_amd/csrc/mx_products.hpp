@@ -2,6 +2,8 @@
 // product finds its rows.
 #pragma once
 
+#include <type_traits>
+
 #include "mx.hpp"
 
 namespace mote::mx {
@@ -56,40 +58,61 @@ __device__ __forceinline__ uint32_t lanes_before(uint32_t v) {
     return sum - v;
 }
 
-// Tile `unit` of the experts' tiles of PER rows: each expert has its rows / PER of
-// them, rounded up.  Every wave looks it up by itself: lane l counts those of its run
-// of experts, a prefix sum over the lanes finds the run, and the run is walked.
+// The tiles of PER rows of the experts: each has its rows / PER of them, rounded up.
+// Every wave counts them by itself: lane l those of its run of experts, and a prefix sum over the
+// lanes; a tile's run is found in that and walked.
 template <uint32_t PER>
-__device__ __forceinline__ Tile expert_tile(const ProductArgs& a, uint32_t unit) {
-    const uint32_t lane = threadIdx.x & 63;
-    const uint32_t run = (a.experts + 63) / 64;
-    const auto at = [&](uint32_t e) {  // kept inside the rows there are, whatever the offsets hold
+struct ExpertTiles {
+    uint32_t upto;  // tiles of this lane's experts and the lanes' before
+
+    // Kept inside the rows there are, whatever the offsets hold.
+    __device__ __forceinline__ static uint32_t offset(const ProductArgs& a, uint32_t e) {
         return static_cast<uint32_t>(min(max(a.offsets[e], 0), static_cast<int32_t>(a.rows)));
-    };
-    uint32_t mine = 0;
-    const uint32_t e0 = min(lane * run, a.experts), e1 = min(e0 + run, a.experts);
-    if (e0 < e1) {
-        uint32_t from = at(e0);
-        for (uint32_t e = e0; e < e1; ++e) {
-            const uint32_t to = at(e + 1);
-            mine += to > from ? (to - from + PER - 1) / PER : 0;
-            from = to;
+    }
+    __device__ __forceinline__ explicit ExpertTiles(const ProductArgs& a) {
+        const uint32_t lane = threadIdx.x & 63, run = (a.experts + 63) / 64;
+        const uint32_t e0 = min(lane * run, a.experts), e1 = min(e0 + run, a.experts);
+        uint32_t mine = 0;
+        if (e0 < e1) {
+            uint32_t from = offset(a, e0);
+            for (uint32_t e = e0; e < e1; ++e) {
+                const uint32_t to = offset(a, e + 1);
+                mine += to > from ? (to - from + PER - 1) / PER : 0;
+                from = to;
+            }
         }
+        upto = lanes_before(mine) + mine;
     }
-    const uint32_t upto = lanes_before(mine) + mine;  // tiles of this lane's experts and the lanes' before
-    const uint64_t before = __builtin_amdgcn_ballot_w64(upto <= unit);
-    const uint32_t owner = __builtin_popcountll(before);
-    if (owner == 64) return {0, 0, 0};
-    uint32_t left = unit;
-    if (owner > 0) left -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), owner - 1));
-    for (uint32_t e = owner * run; e < a.experts; ++e) {
-        const uint32_t from = at(e), to = at(e + 1);
-        const uint32_t n = to > from ? to - from : 0, tiles = (n + PER - 1) / PER;
-        if (left < tiles) return {e, from + left * PER, min(n - left * PER, PER)};
-        left -= tiles;
+    __device__ __forceinline__ uint32_t total() const {
+        return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), 63));
     }
-    return {0, 0, 0};
-}
+    __device__ __forceinline__ Tile at(const ProductArgs& a, uint32_t unit) const {
+        const uint32_t run = (a.experts + 63) / 64;
+        const uint32_t owner = __builtin_popcountll(__builtin_amdgcn_ballot_w64(upto <= unit));
+        if (owner == 64) return {0, 0, 0};
+        uint32_t left = unit;
+        if (owner > 0) left -= static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(upto), owner - 1));
+        for (uint32_t e = owner * run; e < a.experts; ++e) {
+            const uint32_t from = offset(a, e), to = offset(a, e + 1);
+            const uint32_t n = to > from ? to - from : 0, tiles = (n + PER - 1) / PER;
+            if (left < tiles) return {e, from + left * PER, min(n - left * PER, PER)};
+            left -= tiles;
+        }
+        return {0, 0, 0};
+    }
+};
+// A linear's, all of one matrix.
+template <uint32_t PER>
+struct RowTiles {
+    uint32_t rows;
+    __device__ __forceinline__ explicit RowTiles(const ProductArgs& a) : rows(a.rows) {}
+    __device__ __forceinline__ uint32_t total() const { return (rows + PER - 1) / PER; }
+    __device__ __forceinline__ Tile at(const ProductArgs&, uint32_t unit) const {
+        return {0, unit * PER, min(rows - unit * PER, PER)};
+    }
+};
+template <Result R, uint32_t PER>
+using Tiles = std::conditional_t<kOfExperts<R>, ExpertTiles<PER>, RowTiles<PER>>;
 
 // As many tiles as there may be.
 inline uint64_t most_expert_tiles(uint64_t pairs, uint64_t experts, uint64_t per) {
@@ -98,11 +121,10 @@ inline uint64_t most_expert_tiles(uint64_t pairs, uint64_t experts, uint64_t per
     return tiles < pairs ? tiles : pairs;
 }
 
-template <Result R, uint32_t PER>
-__device__ __forceinline__ Tile find_tile(const ProductArgs& a, uint32_t unit) {
-    if constexpr (kOfExperts<R>) return expert_tile<PER>(a, unit);
-    const uint32_t first = unit * PER;
-    return {0, first, min(a.rows - first, PER)};
+// silu(gate) up, the quotient by a reciprocal (good to 2^-23): gate / (1 + e^-gate) exactly
+// rounded is a third of what a tile of outputs costs.
+__device__ __forceinline__ float silu_product(float gate, float up) {
+    return gate * __builtin_amdgcn_rcpf(1.0f + __expf(-gate)) * up;
 }
 
 // The row of x that row `first + i` of a tile multiplies.

@@ -57,7 +57,7 @@ __device__ __forceinline__ Place place_of(uint32_t at, uint32_t units, uint32_t 
 // WN x WM waves divide a tile; WK such groups divide a stage's WK x 128 elements of K among them
 // and add their sums at the end, in their order.
 template <int BITS, Result R, int BN, int BM, int WN, int WM, int WK, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a, uint32_t units, uint32_t columns) {
+__global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a, uint32_t columns) {
     constexpr int kThreads = 64 * WN * WM * WK;
     constexpr int NF = BN / WN / 32, MF = BM / WM / 32;  // 32 x 32 products of a wave
     constexpr bool kGate = R == Result::kGateUp;
@@ -77,14 +77,19 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     constexpr int kWLoads = loads_of(kW, 16), kXLoads = loads_of(kX, 16), kHighLoads = loads_of(kHigh, 16);
     constexpr int kScaleLoads = (kScaleRows + kThreads - 1) / kThreads;
     constexpr int kLoads = kWLoads + kXLoads + kHighLoads + (kEvery == 1 ? kScaleLoads : 0);
-    constexpr int kRing = STAGES * kStage, kLds = kRing + kScaleSlots * kScales;
+    constexpr int kRing = STAGES * kStage, kPairsAt = kRing + kScaleSlots * kScales;
+    constexpr int kLds = kPairsAt + (R == Result::kPairs ? BM * 4 : 0);
     static_assert(kStepBytes % 64 == 0 && kLds <= 160 * 1024 && (STAGES - 2) * kLoads + kScaleLoads < 64, "LDS and waits");
     static_assert(kW / 16 % 64 == 0 && kX / 16 % 64 == 0 && kHigh / 16 % 64 == 0, "whole loads of a wave");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
 
+    // (The grid has room for the most tiles that the experts may have: those there are
+    // go to all XCDs alike.)
+    const Tiles<R, BM> tiles(a);
+    const uint32_t units = tiles.total();
+    if (blockIdx.x >= units * columns) return;
     const Place place = place_of(blockIdx.x, units, columns);
-    const Tile tile = find_tile<R, BM>(a, place.unit);
-    if (tile.count == 0) return;
+    const Tile tile = tiles.at(a, place.unit);
     const uint32_t column = place.column * kColumns;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -102,6 +107,11 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     const auto x_row = [&](uint32_t row) -> uint64_t {
         return input_row<R>(a, tile.first + min(row, tile.count - 1));
     };
+    if constexpr (R == Result::kPairs) {  // where the rows of the results go, at hand when they do
+        for (uint32_t row = threadIdx.x; row < BM; row += kThreads)
+            reinterpret_cast<uint32_t*>(lds + kPairsAt)[row] =
+                row < tile.count ? static_cast<uint32_t>(a.plan[tile.first + row]) : ~0u;
+    }
     // What this thread loads: the row's first step, and the step of the stage.  (A load's place
     // in the part is the wave's; `piece` is the lane's own.)
     const auto piece_of = [&](int i, int pieces) { return (i * kThreads + wave * 64) % (WK * pieces) + lane; };
@@ -322,7 +332,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     __syncthreads();  // the last stage has been read
     if constexpr (WK > 1) {
         constexpr int kGroup = WN * WM * NF * MF;  // products of a group of waves
-        static_assert((WK - 1) * kGroup * 4096 <= kLds, "LDS");
+        static_assert((WK - 1) * kGroup * 4096 <= kPairsAt, "LDS");
         f32x4* const sums = reinterpret_cast<f32x4*>(lds) + lane;
         const int of_wave = wn + WN * wm;
         const auto place_in = [&](int group, int f, int g, int q) {
@@ -360,7 +370,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     constexpr int kOut = kGate ? NF / 2 : NF;                         // 32-column products of the wave
     constexpr int kPass = kOut < 8 / kSize ? kOut : 8 / kSize;        // of them, those turned together
     constexpr int kRowBytes = kPass * 32 * kSize, kRowRoom = kRowBytes + 16;
-    static_assert((WK - 1) * WN * WM * NF * MF * 4096 + WN * WM * 32 * kRowRoom <= kLds && kOut % kPass == 0, "LDS");
+    static_assert((WK - 1) * WN * WM * NF * MF * 4096 + WN * WM * 32 * kRowRoom <= kPairsAt && kOut % kPass == 0, "LDS");
     constexpr int kRowLanes = kRowBytes / 16, kPer = 16 / kSize;
     uint8_t* const turn = lds + (WK > 1 ? (WK - 1) * WN * WM * NF * MF * 4096 : 0) + wave * (32 * kRowRoom);
 #pragma unroll
@@ -376,7 +386,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         y[r] = d[pass + f][g][4 * q + r];
-                        if constexpr (kGate) y[r] = silu(y[r]) * d[pass + f + NF / 2][g][4 * q + r];
+                        if constexpr (kGate) y[r] = silu_product(y[r], d[pass + f + NF / 2][g][4 * q + r]);
                     }
                     uint8_t* const at = turn + of32 * kRowRoom + (f * 32 + 8 * q + 4 * half) * kSize;
                     if constexpr (kHalf)
@@ -396,7 +406,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
                     *reinterpret_cast<const u32x4*>(turn + in_product * kRowRoom + lane % kRowLanes * 16);
                 uint64_t to = tile.first + row;
                 if constexpr (R == Result::kPairs) {
-                    to = static_cast<uint32_t>(a.plan[to]);
+                    to = reinterpret_cast<const uint32_t*>(lds + kPairsAt)[row];
                     if (to >= a.rows) continue;
                 }
                 uint8_t* const out = static_cast<uint8_t*>(a.output) + (to * a.outputs + n) * kSize;
@@ -433,8 +443,7 @@ int launch(const ProductArgs& a, hipStream_t stream) {
     const uint64_t units = row_tiles<R>(a, BM);
     if (units * columns > kMostThreads / kThreads) return kInvalid;
     hipLaunchKernelGGL((tiles_kernel<BITS, R, BN, BM, WN, WM, WK, STAGES>),
-                       dim3(static_cast<uint32_t>(units * columns)), dim3(kThreads), 0, stream, a,
-                       static_cast<uint32_t>(units), columns);
+                       dim3(static_cast<uint32_t>(units * columns)), dim3(kThreads), 0, stream, a, columns);
     return static_cast<int>(hipGetLastError());
 }
 
