@@ -14,8 +14,9 @@
 // lanes share it.
 #include <hip/hip_runtime.h>
 
-#include <cstdint>
+#include <algorithm>
 #include <cmath>
+#include <cstdint>
 
 #include "mx_products.hpp"
 
@@ -53,10 +54,27 @@ __device__ __forceinline__ double lane_value(double v, int lane) {
     const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
+template <int Ctrl, int RowMask = 0xF>
+__device__ __forceinline__ double add_dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), Ctrl, RowMask, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), Ctrl, RowMask, 0xF, false);
+    return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum64(double v) {
-#pragma unroll
-    for (int by = 1; by < 64; by *= 2) v += __shfl_xor(v, by, 64);
-    return v;
+    v = add_dpp64<0xB1>(v);        // as wave_max; a lane that a step leaves out adds 0
+    v = add_dpp64<0x4E>(v);
+    v = add_dpp64<0x141>(v);
+    v = add_dpp64<0x140>(v);
+    v = add_dpp64<0x142, 0xA>(v);
+    v = add_dpp64<0x143, 0xC>(v);
+    return lane_value(v, 63);
+}
+// The largest of finite numbers and -infinity.
+__device__ __forceinline__ float wave_max_float(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const uint32_t most = wave_max(b >> 31 ? ~b : b | 0x80000000u);
+    return __builtin_bit_cast(float, most >> 31 ? most & 0x7FFFFFFFu : ~most);
 }
 
 // Orders as the number does, above 0; 0 is for what takes no part.
@@ -94,8 +112,7 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
         float most = x[0];
 #pragma unroll
         for (int v = 1; v < SLOTS; ++v) most = fmaxf(most, x[v]);
-#pragma unroll
-        for (int by = 1; by < 64; by *= 2) most = fmaxf(most, __shfl_xor(most, by, 64));
+        most = wave_max_float(most);
         double sum = 0.0;
 #pragma unroll
         for (int v = 0; v < SLOTS; ++v) {
@@ -144,53 +161,78 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        // Groups that fewer than top_groups others come before.
-#pragma unroll
-        for (int v = 0; v < SLOTS; ++v) {
-            const uint32_t e = v * 64 + lane;
-            if (e >= a.experts) continue;
-            const uint32_t mine = e / a.size;
-            const uint64_t worth = worths[wave][mine];
+        // Groups that fewer than top_groups others come before stay.
+        const float part_of = 1.0f / static_cast<float>(a.size);  // e / size: e + 1/2 is 2^-11 away from the next
+        if (a.groups <= 64) {
+            const uint64_t worth = lane < a.groups ? worths[wave][lane] : 0;
             uint32_t before = 0;
             for (uint32_t g = 0; g < a.groups; ++g) {
-                const uint64_t other = worths[wave][g];
-                before += other > worth || (other == worth && g < mine) ? 1 : 0;
+                const uint64_t other =
+                    static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(worth >> 32, g))) << 32 |
+                    static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(worth), g));
+                before += other > worth || (other == worth && g < lane) ? 1 : 0;
             }
-            if (before >= a.top_groups) choice[v] = 0;
+            const uint64_t kept = __builtin_amdgcn_ballot_w64(before < a.top_groups);
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) {
+                const uint32_t g = static_cast<uint32_t>((static_cast<float>(v * 64 + lane) + 0.5f) * part_of);
+                if (!(kept >> (g & 63) & 1)) choice[v] = 0;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) {
+                const uint32_t mine = min((v * 64 + lane) / a.size, a.groups - 1);
+                const uint64_t worth = worths[wave][mine];
+                uint32_t before = 0;
+                for (uint32_t g = 0; g < a.groups; ++g) {
+                    const uint64_t other = worths[wave][g];
+                    before += other > worth || (other == worth && g < mine) ? 1 : 0;
+                }
+                if (before >= a.top_groups) choice[v] = 0;
+            }
         }
     }
-    // The largest, `top` times; lane j keeps the j-th.
+    // The largest, `top` times; lane j keeps the j-th.  The upper halves decide unless two are equal.
     int32_t id = -1;
     double weight = 0.0, total = 0.0;
-    for (uint32_t j = 0; j < a.top; ++j) {
-        uint64_t best = choice[0];
-        uint32_t at = 0;
+    uint32_t high[SLOTS];
 #pragma unroll
-        for (int v = 1; v < SLOTS; ++v) {
-            at = choice[v] > best ? v : at;
-            best = max(best, choice[v]);
+    for (int v = 0; v < SLOTS; ++v) high[v] = static_cast<uint32_t>(choice[v] >> 32);
+    for (uint32_t j = 0; j < a.top; ++j) {
+        uint32_t mine = high[0];
+#pragma unroll
+        for (int v = 1; v < SLOTS; ++v) mine = max(mine, high[v]);
+        const uint32_t most = wave_max(mine);
+        if (most == 0) break;  // nothing left: an order of 0 alone has an upper half of 0
+        uint64_t holders[SLOTS];
+        uint32_t count = 0, slot = 0;
+#pragma unroll
+        for (int v = SLOTS - 1; v >= 0; --v) {
+            holders[v] = __builtin_amdgcn_ballot_w64(high[v] == most);
+            count += __builtin_popcountll(holders[v]);
+            slot = holders[v] ? v : slot;  // the lowest
         }
-        const uint32_t high = wave_max(static_cast<uint32_t>(best >> 32));
-        if (high == 0) break;  // an order of 0 alone has an upper half of 0
-        uint64_t holders = __builtin_amdgcn_ballot_w64(static_cast<uint32_t>(best >> 32) == high);
-        if (holders & (holders - 1)) {
-            const bool tied = static_cast<uint32_t>(best >> 32) == high;
-            const uint32_t low = wave_max(tied ? static_cast<uint32_t>(best) : 0);
-            const bool equal = tied && static_cast<uint32_t>(best) == low;
-            holders = __builtin_amdgcn_ballot_w64(equal);
-            const uint32_t least = ~wave_max(equal ? ~at : 0);  // the lowest slot, then the lowest lane
-            holders = __builtin_amdgcn_ballot_w64(equal && at == least);
+        if (count > 1) {
+            uint32_t low = 0;
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) low = max(low, high[v] == most ? static_cast<uint32_t>(choice[v]) : 0);
+            low = wave_max(low);
+#pragma unroll
+            for (int v = SLOTS - 1; v >= 0; --v) {
+                holders[v] = __builtin_amdgcn_ballot_w64(high[v] == most && static_cast<uint32_t>(choice[v]) == low);
+                slot = holders[v] ? v : slot;
+            }
         }
-        const int winner = __builtin_ctzll(holders);
-        const uint32_t slot = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(at), winner));
-        double s = score[0];
+        int winner = 0;
+        double s = 0.0;
 #pragma unroll
         for (int v = 0; v < SLOTS; ++v) {
-            const bool this_slot = static_cast<uint32_t>(v) == slot;
-            s = this_slot ? score[v] : s;
-            if (this_slot && lane == static_cast<uint32_t>(winner)) choice[v] = 0;
+            if (static_cast<uint32_t>(v) == slot) {  // the same in all lanes
+                winner = __builtin_ctzll(holders[v]);
+                s = lane_value(score[v], winner);
+                high[v] = lane == static_cast<uint32_t>(winner) ? 0 : high[v];
+            }
         }
-        s = lane_value(s, winner);
         total += s;
         if (lane == j) {
             id = static_cast<int32_t>(slot * 64 + winner);
@@ -214,89 +256,97 @@ struct PlanArgs {
 
 // A workgroup for each expert: it counts the pairs of lower experts, which is where its own
 // begin, and its own, then writes its own in their order.  No counter is shared, so the order is
-// always the same.  A thread has a run of neighbouring pairs, up to kRun of them in its registers
-// (so up to 32768 pairs are read once); more go by in rounds that are counted first.
-constexpr uint32_t kPlanThreads = 1024;
-constexpr uint32_t kRun = 32;
+// always the same.  A thread has four neighbouring pairs in each of up to kTurns turns, all
+// in its registers (so up to 32768 pairs are read once, with whole lines to a wave); a wave's own are bits of
+// ballots, and where they go is a prefix sum over turns and waves.  More pairs go by in rounds that are
+// counted first.
+constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kMostTurns = 8;
 
-struct Run {
-    uint32_t expert[kRun];
-};
-__device__ __forceinline__ void load_run(const PlanArgs& a, uint32_t first, uint32_t per, Run& run) {
-    typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
-#pragma unroll
-    for (uint32_t i = 0; i < kRun; i += 4) {
-        if (i < per && first + i + 4 <= a.pairs) {
-            const i32x4_a4 four = *reinterpret_cast<const i32x4_a4*>(a.ids + first + i);
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j) run.expert[i + j] = static_cast<uint32_t>(four[j]);
-        } else {
-#pragma unroll
-            for (uint32_t j = 0; j < 4; ++j)
-                run.expert[i + j] = i < per && first + i + j < a.pairs ? static_cast<uint32_t>(a.ids[first + i + j]) : ~0u;
-        }
-    }
-}
-
-// per: pairs of a thread's run in a round, a multiple of 4 up to kRun.
+// per: turns of a round, up to TURNS (one, where that is all: a single token's plan is bound by
+// the reading of the code).
+template <uint32_t TURNS>
 __global__ __launch_bounds__(kPlanThreads) void plan_kernel(PlanArgs a, uint32_t per) {
-    __shared__ uint32_t lower_of[kPlanThreads / 64], own_of[kPlanThreads / 64];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, waves = blockDim.x >> 6;
-    const uint32_t expert = blockIdx.x;
-    const uint32_t round = blockDim.x * per, rounds = max((a.pairs + round - 1) / round, 1u);
-    const uint32_t mine = threadIdx.x * per;
-    Run run;
-    uint32_t lower = 0, all = 0;  // of this thread, all rounds
-    for (uint32_t r = 0; r < rounds; ++r) {
-        load_run(a, r * round + mine, per, run);
+    __shared__ uint32_t lower_of[kPlanWaves], own_of[TURNS * kPlanWaves];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const uint32_t waves = blockDim.x >> 6, expert = blockIdx.x;
+    const uint32_t round = blockDim.x * 4 * per, rounds = max((a.pairs + round - 1) / round, 1u);
+    typedef int32_t i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+    uint32_t of[TURNS][4];
+    const auto first_of = [&](uint32_t r, uint32_t turn) { return r * round + (turn * blockDim.x + threadIdx.x) * 4; };
+    const auto load = [&](uint32_t r) {
 #pragma unroll
-        for (uint32_t i = 0; i < kRun; ++i) {
-            lower += run.expert[i] < expert ? 1 : 0;
-            all += run.expert[i] == expert ? 1 : 0;
-        }
-    }
-    // Those of the workgroup, and in one round those of the threads before.
-    const uint32_t lower_before = lanes_before(lower), own_before = lanes_before(all);
-    if (lane == 63) {
-        lower_of[wave] = lower_before + lower;
-        own_of[wave] = own_before + all;
-    }
-    __syncthreads();
-    uint32_t begin = 0, total = 0, before = own_before;
-    for (uint32_t w = 0; w < waves; ++w) {
-        begin += lower_of[w];
-        total += own_of[w];
-        if (w < wave) before += own_of[w];
-    }
-    uint32_t at = begin;
-    for (uint32_t r = 0; r < rounds && total > 0; ++r) {
-        uint32_t own = all, own_total = total;
-        if (rounds > 1) {
-            load_run(a, r * round + mine, per, run);
-            own = 0;
+        for (uint32_t t = 0; t < TURNS; ++t) {
+            const uint32_t first = first_of(r, t);
+            if (t < per && first + 4 <= a.pairs) {
+                const i32x4_a4 four = *reinterpret_cast<const i32x4_a4*>(a.ids + first);
 #pragma unroll
-            for (uint32_t i = 0; i < kRun; ++i) own += run.expert[i] == expert ? 1 : 0;
-            before = lanes_before(own);
-            __syncthreads();  // the sums of the round before have been read
-            if (lane == 63) own_of[wave] = before + own;
-            __syncthreads();
-            own_total = 0;
-            for (uint32_t w = 0; w < waves; ++w) {
-                own_total += own_of[w];
-                if (w < wave) before += own_of[w];
+                for (uint32_t j = 0; j < 4; ++j) of[t][j] = static_cast<uint32_t>(four[j]);
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j)
+                    of[t][j] = t < per && first + j < a.pairs ? static_cast<uint32_t>(a.ids[first + j]) : ~0u;
             }
         }
-        uint32_t to = at + before;
+    };
+    const auto own_bits = [&](uint32_t t, uint32_t j) { return __builtin_amdgcn_ballot_w64(of[t][j] == expert); };
+    const auto count_turns = [&] {  // each turn's own of the wave, to own_of
 #pragma unroll
-        for (uint32_t i = 0; i < kRun; ++i)
-            if (run.expert[i] == expert) a.rows[to++] = static_cast<int32_t>(r * round + mine + i);
-        at += own_total;
+        for (uint32_t t = 0; t < TURNS; ++t) {
+            uint32_t own = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) own += __builtin_popcountll(own_bits(t, j));
+            if (lane == 0 && t < per) own_of[t * waves + wave] = own;
+        }
+    };
+    uint32_t lower = 0;
+    for (uint32_t r = 0; r < rounds; ++r) {
+        load(r);
+#pragma unroll
+        for (uint32_t t = 0; t < TURNS; ++t)
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) lower += __builtin_popcountll(__builtin_amdgcn_ballot_w64(of[t][j] < expert));
+    }
+    if (rounds == 1) count_turns();
+    if (lane == 0) lower_of[wave] = lower;
+    __syncthreads();
+    uint32_t at = 0;
+    for (uint32_t w = 0; w < waves; ++w) at += lower_of[w];
+    const uint32_t begin = at;
+    for (uint32_t r = 0; r < rounds; ++r) {
+        if (rounds > 1) {
+            load(r);
+            __syncthreads();  // the turns of the round before have been read
+            count_turns();
+            __syncthreads();
+        }
+        // Turn t of wave w is entry t waves + w: lane l adds up entries 2 l and 2 l + 1.
+        const uint32_t entries = per * waves;
+        const uint32_t a0 = 2 * lane < entries ? own_of[2 * lane] : 0;
+        const uint32_t a1 = 2 * lane + 1 < entries ? own_of[2 * lane + 1] : 0;
+        const uint32_t before = lanes_before(a0 + a1);
+        const uint32_t all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before + a0 + a1), 63));
+#pragma unroll
+        for (uint32_t t = 0; t < TURNS; ++t) {
+            uint64_t bits[4], any = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j) any |= bits[j] = own_bits(t, j);
+            if (any == 0) continue;
+            const uint32_t entry = t * waves + wave;
+            uint32_t to = at + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before), entry / 2));
+            if (entry & 1) to += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(a0), entry / 2));
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                to += __builtin_popcountll(bits[j] & ((uint64_t{1} << lane) - 1));
+#pragma unroll
+            for (uint32_t j = 0; j < 4; ++j)
+                if (of[t][j] == expert) a.rows[to++] = static_cast<int32_t>(first_of(r, t) + j);
+        }
+        at += all;
     }
     if (threadIdx.x == 0) a.offsets[expert] = static_cast<int32_t>(begin);
     if (expert + 1 == a.experts) {
-        const uint32_t end = begin + total;
-        if (threadIdx.x == 0) a.offsets[a.experts] = static_cast<int32_t>(end);
-        for (uint32_t p = end + threadIdx.x; p < a.pairs; p += blockDim.x) a.rows[p] = -1;
+        if (threadIdx.x == 0) a.offsets[a.experts] = static_cast<int32_t>(at);
+        for (uint32_t p = at + threadIdx.x; p < a.pairs; p += blockDim.x) a.rows[p] = -1;
     }
 }
 
@@ -380,10 +430,13 @@ MOTE_EXPORT int mote_hip_plan_experts(const void* ids, void* offsets, void* rows
     if (experts == 0) return 0;
     const PlanArgs a{static_cast<const int32_t*>(ids), static_cast<int32_t*>(offsets), static_cast<int32_t*>(rows),
                      static_cast<uint32_t>(tokens * top), static_cast<uint32_t>(experts)};
-    // Four pairs a thread, more where a thousand threads do not take them all.
-    const uint32_t waves = a.pairs >= kPlanThreads * 4 ? kPlanThreads / 64 : max((a.pairs + 255) / 256, 1u);
-    const uint32_t each = (a.pairs + waves * 64 - 1) / (waves * 64);
-    const uint32_t per = min((max(each, 1u) + 3) & ~3u, kRun);
-    hipLaunchKernelGGL(plan_kernel, dim3(a.experts), dim3(waves * 64), 0, static_cast<hipStream_t>(stream), a, per);
+    // Four pairs a thread, more turns where a thousand threads do not take them all.
+    const uint32_t waves = a.pairs >= kPlanThreads * 4 ? kPlanWaves : std::max((a.pairs + 255) / 256, 1u);
+    const uint32_t turns = (a.pairs + waves * 256 - 1) / (waves * 256);
+    const uint32_t per = std::min(std::max(turns, 1u), kMostTurns);
+    const auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(a.experts), dim3(waves * 64), 0, static_cast<hipStream_t>(stream), a, per);
+    };
+    per == 1 ? go(plan_kernel<1>) : go(plan_kernel<kMostTurns>);
     return static_cast<int>(hipGetLastError());
 }
