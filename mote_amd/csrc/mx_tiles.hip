@@ -54,8 +54,7 @@ __device__ __forceinline__ Place place_of(uint32_t at, uint32_t units, uint32_t 
     return {band * kBand + in_band % height, in_band / height};
 }
 
-// WN x WM waves divide a tile; WK such groups divide a stage's WK x 128 elements of K among them
-// and add their sums at the end, in their order.
+// WN x WM waves divide a tile, or WK waves divide K and add their sums at the end, in their order.
 template <int BITS, Result R, int BN, int BM, int WN, int WM, int WK, int STAGES>
 __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a, uint32_t columns) {
     constexpr int kThreads = 64 * WN * WM * WK;
@@ -63,23 +62,25 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     constexpr bool kGate = R == Result::kGateUp;
     constexpr int kColumns = kGate ? BN / 2 : BN;  // outputs of a tile
     static_assert(!kGate || NF % 2 == 0, "a wave has a gate and its up");
-    // The parts of a step of a stage, and the loads of a stage that a thread issues for each.
-    // Where a part has fewer pieces than there are threads, some are loaded twice, to the same
-    // place: every wave then waits for the same number.
-    constexpr int kW = BN * 64, kX = BM * 64, kHigh = BITS == 6 ? BM * 32 : 0;
-    constexpr int kStepBytes = kW + kX + kHigh, kStage = WK * kStepBytes;
+    // Waves that divide K have a whole tile each, with rings and loads of their own: nothing of theirs
+    // meets before the end, so there is no barrier to wait at.
+    constexpr bool kAlone = WK > 1;
+    static_assert(!kAlone || WN * WM == 1, "waves divide the tile or K");
+    constexpr int kLoaders = kAlone ? 64 : kThreads;  // threads that load a stage, a step of K
+    // The parts of a stage, and the loads that a thread issues for each.  Where a part has fewer
+    // pieces than there are threads, some are loaded twice, to the same place: every wave then
+    // waits for the same number.
+    constexpr int kW = BN * 64, kX = BM * 64, kHigh = BITS == 6 ? BM * 32 : 0, kStage = kW + kX + kHigh;
     // Scales come four steps at a time, 16 bytes of a row (a word of each row at every step was half
-    // of all requests to the L2), to a ring of their own: kEvery stages take one piece of it.
+    // of all requests to the L2), to a ring of their own.
     constexpr int kScaleRows = (BN + BM + 63) / 64 * 64;  // whole loads of a wave
-    constexpr int kScales = kScaleRows * 16, kEvery = 4 / WK, kScaleSlots = WK == 4 ? STAGES : 2;
-    static_assert(4 % WK == 0, "a stage has the scales of one piece");
-    constexpr auto loads_of = [](int bytes, int each) { return (WK * bytes / each + kThreads - 1) / kThreads; };
-    constexpr int kWLoads = loads_of(kW, 16), kXLoads = loads_of(kX, 16), kHighLoads = loads_of(kHigh, 16);
-    constexpr int kScaleLoads = (kScaleRows + kThreads - 1) / kThreads;
-    constexpr int kLoads = kWLoads + kXLoads + kHighLoads + (kEvery == 1 ? kScaleLoads : 0);
-    constexpr int kRing = STAGES * kStage, kPairsAt = kRing + kScaleSlots * kScales;
+    constexpr int kScales = kScaleRows * 16;
+    constexpr auto loads_of = [](int pieces) { return (pieces + kLoaders - 1) / kLoaders; };
+    constexpr int kWLoads = loads_of(kW / 16), kXLoads = loads_of(kX / 16), kHighLoads = loads_of(kHigh / 16);
+    constexpr int kScaleLoads = loads_of(kScaleRows), kLoads = kWLoads + kXLoads + kHighLoads;
+    constexpr int kRing = STAGES * kStage, kOwn = kRing + 2 * kScales, kPairsAt = WK * kOwn;
     constexpr int kLds = kPairsAt + (R == Result::kPairs ? BM * 4 : 0);
-    static_assert(kStepBytes % 64 == 0 && kLds <= 160 * 1024 && (STAGES - 2) * kLoads + kScaleLoads < 64, "LDS and waits");
+    static_assert(kLds <= 160 * 1024 && (STAGES - 2) * kLoads + kScaleLoads < 64, "LDS and waits");
     static_assert(kW / 16 % 64 == 0 && kX / 16 % 64 == 0 && kHigh / 16 % 64 == 0, "whole loads of a wave");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
 
@@ -94,7 +95,9 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int wn = wave % WN, wm = wave / WN % WM, wk = wave / (WN * WM);
-    const uint32_t steps = a.kp / kStep, stages = (steps + WK - 1) / WK;
+    const uint32_t steps = a.kp / kStep, each = (steps + WK - 1) / WK;
+    const uint32_t first_step = min(wk * each, steps), stages = min(each, steps - first_step);
+    uint8_t* const own = lds + wk * kOwn;
 
     // Row `row` of the tile's weights, rows past the last being the last again.
     const auto w_row = [&](uint32_t row) -> uint64_t {
@@ -114,63 +117,58 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     }
     // What this thread loads: the row's first step, and the step of the stage.  (A load's place
     // in the part is the wave's; `piece` is the lane's own.)
-    const auto piece_of = [&](int i, int pieces) { return (i * kThreads + wave * 64) % (WK * pieces) + lane; };
+    const int loader = kAlone ? 0 : wave;
+    const auto piece_of = [&](int i, int pieces) { return (i * kLoaders + loader * 64) % pieces + lane; };
     const uint8_t* w_from[kWLoads];
     const uint8_t* x_from[kXLoads];
     const uint8_t* high_from[kHighLoads > 0 ? kHighLoads : 1];
     const uint8_t* scale_from[kScaleLoads];
 #pragma unroll
     for (int i = 0; i < kWLoads; ++i) {
-        const uint32_t at = piece_of(i, kW / 16) % (kW / 16), row = at / 4, block = (at % 4) ^ (row / 4 % 4);
+        const uint32_t at = piece_of(i, kW / 16), row = at / 4, block = (at % 4) ^ (row / 4 % 4);
         w_from[i] = a.w + w_row(row) * value_bytes(a.kp, 4) + block * 16;
     }
 #pragma unroll
     for (int i = 0; i < kXLoads; ++i) {
-        const uint32_t at = piece_of(i, kX / 16) % (kX / 16), row = at / 4, block = (at % 4) ^ (row / 4 % 4);
+        const uint32_t at = piece_of(i, kX / 16), row = at / 4, block = (at % 4) ^ (row / 4 % 4);
         x_from[i] = a.x + x_row(row) * value_bytes(a.kp, BITS) + block * 16;
     }
     if constexpr (BITS == 6) {
 #pragma unroll
         for (int i = 0; i < kHighLoads; ++i) {  // two blocks' 8 bytes, at pair ^ (row / 8 % 2)
-            const uint32_t at = piece_of(i, kHigh / 16) % (kHigh / 16), row = at / 2, pair = (at % 2) ^ (row / 8 % 2);
+            const uint32_t at = piece_of(i, kHigh / 16), row = at / 2, pair = (at % 2) ^ (row / 8 % 2);
             high_from[i] = a.x + x_row(row) * value_bytes(a.kp, BITS) + a.kp / 2 + pair * 16;
         }
     }
 #pragma unroll
     for (int i = 0; i < kScaleLoads; ++i) {
-        const uint32_t row = min((i * kThreads + wave * 64) % kScaleRows + lane, BN + BM - 1);
+        const uint32_t row = min(piece_of(i, kScaleRows), BN + BM - 1);
         scale_from[i] = row < BN ? a.w_scales + w_row(row) * scale_bytes(a.kp)
                                  : a.x_scales + x_row(row - BN) * scale_bytes(a.kp);
     }
-    // The scales of steps 4 group .. 4 group + 3; of the last four where that passes the end.
-    const auto first_of = [&](uint32_t group) { return min(4 * group, steps - 4); };
+    // The scales of the group of four steps; of the last four of all where that passes the end.
+    const auto first_of = [&](uint32_t group) { return min(first_step + 4 * group, steps - 4); };
     const auto load_scales = [&](uint32_t group) {
-        uint8_t* const to = lds + kRing + group % kScaleSlots * kScales;
+        uint8_t* const to = own + kRing + group % 2 * kScales;
 #pragma unroll
         for (int i = 0; i < kScaleLoads; ++i)
-            load_lds16(scale_from[i] + first_of(group) * 4, to + (i * kThreads + wave * 64) % kScaleRows * 16);
+            load_lds16(scale_from[i] + first_of(group) * 4, to + (piece_of(i, kScaleRows) - lane) * 16);
     };
-    // Load `i` of stage `stage`, to a slot; steps past the end are the last again, unused.
+    // Load `i` of stage `stage`, to a slot.
     const auto load_one = [&](uint32_t stage, uint32_t slot, int i) {
-        uint8_t* const to = lds + slot * kStage;
-        const auto load = [&](int at, int pieces, const uint8_t* from, uint32_t part, uint32_t bytes) {
-            const uint32_t first = piece_of(at, pieces) - lane;
-            const uint32_t step = WK == 1 ? stage : min(stage * WK + first / pieces, steps - 1);
-            load_lds16(from + step * bytes,
-                       to + (WK == 1 ? 0 : first / pieces * kStepBytes) + part + first % pieces * 16);
-        };
+        uint8_t* const to = own + slot * kStage;
+        const uint32_t step = first_step + stage;
         if (i < kWLoads)
-            load(i, kW / 16, w_from[i], 0, 64);
+            load_lds16(w_from[i] + step * 64, to + (piece_of(i, kW / 16) - lane) * 16);
         else if (i < kWLoads + kXLoads)
-            load(i - kWLoads, kX / 16, x_from[i - kWLoads], kW, 64);
-        else
-            load(i - kWLoads - kXLoads, kHigh > 0 ? kHigh / 16 : 64, high_from[i - kWLoads - kXLoads], kW + kX, 32);
+            load_lds16(x_from[i - kWLoads] + step * 64, to + kW + (piece_of(i - kWLoads, kX / 16) - lane) * 16);
+        else if constexpr (BITS == 6)
+            load_lds16(high_from[i - kWLoads - kXLoads] + step * 32,
+                       to + kW + kX + (piece_of(i - kWLoads - kXLoads, kHigh / 16) - lane) * 16);
     };
-    constexpr int kStageLoads = kWLoads + kXLoads + kHighLoads;
     const auto load_stage = [&](uint32_t stage, uint32_t slot) {
 #pragma unroll
-        for (int i = 0; i < kStageLoads; ++i) load_one(stage, slot, i);
-        if constexpr (kEvery == 1) load_scales(stage);
+        for (int i = 0; i < kLoads; ++i) load_one(stage, slot, i);
     };
 
     // This lane's rows of the wave's products, in the tile.
@@ -188,9 +186,9 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     u32x2 x_high[2][MF];  // (of 6 bits)
     uint32_t w_words[NF], x_words[MF], ws[NF], xs[MF];
     const auto read_scales = [&](uint32_t stage) {
-        const uint32_t group = stage / kEvery;
-        const uint32_t* const scales = reinterpret_cast<const uint32_t*>(lds + kRing + group % kScaleSlots * kScales) +
-                                       (stage * WK + wk - first_of(group));
+        const uint32_t group = stage / 4;
+        const uint32_t* const scales = reinterpret_cast<const uint32_t*>(own + kRing + group % 2 * kScales) +
+                                       (first_step + stage - first_of(group));
 #pragma unroll
         for (int f = 0; f < NF; ++f) w_words[f] = scales[(w_in_tile(f) + of32) * 4];
 #pragma unroll
@@ -204,7 +202,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     };
     const auto read_half = [&](uint32_t slot, auto which) {
         constexpr int S = decltype(which)::value;
-        const uint8_t* const at = lds + slot * kStage + wk * kStepBytes;
+        const uint8_t* const at = own + slot * kStage;
         const uint32_t block = 2 * S + half;
 #pragma unroll
         for (int f = 0; f < MF; ++f) {
@@ -239,63 +237,65 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
 
     const auto next = [](uint32_t slot) { return slot + 1 == STAGES ? 0 : slot + 1; };
     uint32_t loading = 0, reading = 0;
-    if constexpr (kEvery > 1) load_scales(0);
-#pragma unroll
-    for (uint32_t s = 0; s < STAGES - 1; ++s)
-        if (s < stages) load_stage(s, loading), loading = next(loading);
-    // Until all but `later` loads have landed, for all waves.
+    // Until all but `later` of the loads have landed, for all waves that share them.
     const auto arrive = [&](auto later) {
         wait_counts<vm_wait(decltype(later)::value) & kLgkmWait>();
         order_fence();
-        group_barrier();
+        if constexpr (!kAlone) group_barrier();
         order_fence();
     };
-    if constexpr (WK == 1) {
-        // While one half of a step is multiplied the next one is read: behind the first of its
-        // products, so that the wait for what that one needs is not for these too.  (steps is at least 4.)
-        static_assert(STAGES == 3, "the last two stages");
-        const auto run_stage = [&](uint32_t stage, auto loads, auto later) {
-            constexpr int kLater = decltype(later)::value;  // loads under way when the next stage has landed
-            take_scales();
-            multiply_half(k0, 0, 1);
-            order_fence();
-            read_half(reading, k1);
-            order_fence();
-            // The loads of a later stage between the products: one after the other they would hold up
-            // the wave, and the others at the barrier, for longer than the products take.
-            constexpr int kProducts = NF * MF;
+    // While one half of a step is multiplied the next one is read: behind the first of its
+    // products, so that the wait for what that one needs is not for these too.
+    const auto run_stage = [&](uint32_t stage, auto loads, auto later) {
+        constexpr int kLater = decltype(later)::value;  // loads under way when the next stage has landed; -1: none
+        take_scales();
+        multiply_half(k0, 0, 1);
+        order_fence();
+        read_half(reading, k1);
+        order_fence();
+        // The loads of a later stage between the products: one after the other they would hold up
+        // the wave, and the others at the barrier, for longer than the products take.
+        constexpr int kProducts = NF * MF, kGaps = kProducts > 1 ? kProducts - 1 : 1;
 #pragma unroll
-            for (int i = 1; i < kProducts; ++i) {
-                multiply_half(k0, i, i + 1);
-                order_fence();
-                if constexpr (decltype(loads)::value) {
-                    const int from = (i - 1) * kStageLoads / (kProducts - 1), to = i * kStageLoads / (kProducts - 1);
-#pragma unroll
-                    for (int l = from; l < to; ++l) load_one(stage + STAGES - 1, loading, l);
-                    order_fence();
-                }
-            }
-            if constexpr (decltype(loads)::value) loading = next(loading);
-            reading = next(reading);
-            if constexpr (kLater >= 0) arrive(later);
-            multiply_half(k1, 0, 1);
+        for (int i = 0; i < kGaps; ++i) {
+            multiply_half(k0, i + 1, i + 2);
             order_fence();
-            if constexpr (kLater >= 0) {
-                read_scales(stage + 1);
-                read_half(reading, k0);
+            if constexpr (decltype(loads)::value) {
+#pragma unroll
+                for (int l = i * kLoads / kGaps; l < (i + 1) * kLoads / kGaps; ++l)
+                    load_one(stage + STAGES - 1, loading, l);
                 order_fence();
             }
-            multiply_half(k1, 1, NF * MF);
+        }
+        if constexpr (decltype(loads)::value) loading = next(loading);
+        reading = next(reading);
+        if constexpr (kLater >= 0) arrive(later);
+        multiply_half(k1, 0, 1);
+        order_fence();
+        if constexpr (kLater >= 0) {
+            read_scales(stage + 1);
+            read_half(reading, k0);
             order_fence();
-        };
-        constexpr std::integral_constant<int, kLoads> kSteady;
-        arrive(kSteady);
+        }
+        multiply_half(k1, 1, kProducts);
+        order_fence();
+    };
+    if (stages > 0) {
+        load_scales(0);
+#pragma unroll
+        for (uint32_t s = 0; s < STAGES - 1; ++s)
+            if (s < stages) load_stage(s, loading), loading = next(loading);
+        constexpr std::integral_constant<int, (STAGES - 2) * kLoads> kSteady;
+        if (stages >= STAGES - 1)
+            arrive(kSteady);
+        else
+            arrive(k0);
         read_scales(0);
         read_half(0, k0);
         uint32_t stage = 0;
-        for (; stage + 4 + STAGES - 2 < stages; stage += 4) {  // in fours: straight code with the scales' loads
+        for (; stage + STAGES + 2 < stages; stage += 4) {  // in fours: straight code with the scales' loads
             load_scales(stage / 4 + 1);
-            run_stage(stage, std::true_type{}, std::integral_constant<int, kLoads + kScaleLoads>{});
+            run_stage(stage, std::true_type{}, std::integral_constant<int, (STAGES - 2) * kLoads + kScaleLoads>{});
             run_stage(stage + 1, std::true_type{}, kSteady);
             run_stage(stage + 2, std::true_type{}, kSteady);
             run_stage(stage + 3, std::true_type{}, kSteady);
@@ -304,30 +304,11 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
             if (stage % 4 == 0) load_scales(stage / 4 + 1);
             run_stage(stage, std::true_type{}, kSteady);
         }
-        run_stage(stage, std::false_type{}, k0);
-        run_stage(stage + 1, std::false_type{}, std::integral_constant<int, -1>{});
-    } else {
-        for (uint32_t stage = 0; stage < stages; ++stage) {
-            // The later stages' loads may still be on their way, and scales that were asked for
-            // with the last of them.
-            if (stage + STAGES - 1 > stages)
-                arrive(k0);
-            else if (kEvery > 1 && stage > 0 && (stage - 1) % kEvery == 0)
-                arrive(std::integral_constant<int, (STAGES - 2) * kLoads + kScaleLoads>{});
-            else
-                arrive(std::integral_constant<int, (STAGES - 2) * kLoads>{});
-            if (kEvery > 1 && stage % kEvery == 0) load_scales(stage / kEvery + 1);
-            if (stage + STAGES - 1 < stages) load_stage(stage + STAGES - 1, loading), loading = next(loading);
-            if (stage * WK + wk < steps) {
-                read_scales(stage);
-                take_scales();
-                read_half(reading, k0);
-                read_half(reading, k1);
-                multiply_half(k0, 0, NF * MF);
-                multiply_half(k1, 0, NF * MF);
-            }
-            reading = next(reading);
+        for (; stage + 1 < stages; ++stage) {
+            if (stage % 4 == 0) load_scales(stage / 4 + 1);
+            run_stage(stage, std::false_type{}, k0);
         }
+        run_stage(stage, std::false_type{}, std::integral_constant<int, -1>{});
     }
     __syncthreads();  // the last stage has been read
     if constexpr (WK > 1) {
@@ -473,8 +454,8 @@ int choose(const ProductArgs& a, hipStream_t stream) {
         if (enough(256, 256)) return launch<BITS, R, 256, 256, 2, 2, 1, 3>(a, stream);
         if (enough(128, 128)) return launch<BITS, R, 128, 128, 2, 2, 1, 3>(a, stream);
         if (enough(128, 64)) return launch<BITS, R, 128, 64, 2, 2, 1, 3>(a, stream);
-        if (enough(64, 64)) return launch<BITS, R, 64, 64, 2, 2, 2, 3>(a, stream);
-        if (enough(32, 64)) return launch<BITS, R, 32, 64, 1, 2, 4, 3>(a, stream);
+        if (enough(64, 64)) return launch<BITS, R, 64, 64, 1, 1, 4, 3>(a, stream);
+        if (enough(32, 64)) return launch<BITS, R, 32, 64, 1, 1, 4, 4>(a, stream);
         return launch<BITS, R, 32, 32, 1, 1, 4, 4>(a, stream);
     }
 }
