@@ -280,13 +280,13 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
         multiply_half(k1, 1, kProducts);
         order_fence();
     };
-    if (stages > 0) {
+    if (!kAlone || stages > 0) {
         load_scales(0);
 #pragma unroll
         for (uint32_t s = 0; s < STAGES - 1; ++s)
-            if (s < stages) load_stage(s, loading), loading = next(loading);
+            if (!kAlone || s < stages) load_stage(s, loading), loading = next(loading);
         constexpr std::integral_constant<int, (STAGES - 2) * kLoads> kSteady;
-        if (stages >= STAGES - 1)
+        if (!kAlone || stages >= STAGES - 1)
             arrive(kSteady);
         else
             arrive(k0);
@@ -304,9 +304,14 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
             if (stage % 4 == 0) load_scales(stage / 4 + 1);
             run_stage(stage, std::true_type{}, kSteady);
         }
-        for (; stage + 1 < stages; ++stage) {
-            if (stage % 4 == 0) load_scales(stage / 4 + 1);
-            run_stage(stage, std::false_type{}, k0);
+        if constexpr (kAlone) {
+            for (; stage + 1 < stages; ++stage) {
+                if (stage % 4 == 0) load_scales(stage / 4 + 1);
+                run_stage(stage, std::false_type{}, k0);
+            }
+        } else {  // two stages more: K has four at least
+            static_assert(STAGES == 3, "the last two stages");
+            run_stage(stage++, std::false_type{}, k0);
         }
         run_stage(stage, std::false_type{}, std::integral_constant<int, -1>{});
     }
