@@ -419,7 +419,7 @@ int mote_hip_cache_attention_q8_f16(const void* q, const void* cache, const void
  * the even code, held to +-6 or +-7.5.  A block of zeros has scale byte 0; one with an infinity or
  * NaN has 255 and zeros.  Writes the padding too.
  * dequantize: element x 2^(b - 127) rounded once to the output's type, to rows
- * `output_stride` apart; what lies between the rows is left as it is.
+ * `output_stride` apart; what lies between the rows is left as it is.  Neither works in place.
  * Status: 0; -1 for a null pointer, bits other than 4 or 6, features not a multiple of
  * 32 or above 2^24, a stride below features or above 2^40, more than 2^31 rows or 2^32 - 257 blocks
  * (padding included), values off the 16-byte grid, f16 or f32 off their alignment; the
@@ -438,9 +438,10 @@ int mote_hip_mx_dequantize_f32(const void* values, const void* scales, void* out
  * scale that is not a number shows as NaN in the outputs of its row.
  * Status: 0; -1 for a null pointer, input_bits other than 4 or 6, K not a multiple of
  * 32, K or N above 2^24, more than 2^30 rows, values off the 16-byte grid or scales off the 4-byte
- * one, an output off its alignment, more work than one launch holds (rows / 64 x N / 16 of
- * 2^23 - 1); the launch status.  rows == 0 or N == 0: 0 without a launch; K == 0 writes
- * zeros.  Output must not alias the inputs.  Nothing is allocated, and a call can be captured. */
+ * one, an output off its alignment, more work than one launch holds (2^36 outputs where K is
+ * at most 384, 2^40 else, each side counted in whole tiles of up to 256); the launch status.
+ * rows == 0 or N == 0: 0 without a launch; K == 0 writes zeros.  Output must not alias the inputs.
+ * Nothing is allocated, and a call can be captured. */
 int mote_hip_mx_linear_f16(const void* input_values, const void* input_scales, const void* weight_values,
                            const void* weight_scales, void* output, uint64_t rows, uint64_t output_features,
                            uint64_t input_features, int input_bits, void* stream);
@@ -463,7 +464,7 @@ int mote_hip_mx_linear_f32(const void* input_values, const void* input_scales, c
  * Status: 0; -1 for a null pointer (bias excepted), logits, bias, ids or weights off
  * their alignment, score or renormalize other than 0 or 1, group_best other than 1 or 2, a scale that is
  * not finite, more than 1024 experts, top above 64 or above the experts that the groups leave, groups that do not
- * divide the experts or top_groups not in 1 .. groups, more than 2^26 - 1 tokens
+ * divide the experts or top_groups not in 1 .. groups, more than 2^26 - 4 tokens
  * or 2^30 pairs; the launch status.  No token, expert or top: 0 without a launch. */
 int mote_hip_route_experts_f16(const void* logits, const void* bias, void* ids, void* weights, uint64_t tokens,
                                uint64_t experts, uint64_t top, int score, uint64_t groups, uint64_t top_groups,
@@ -476,7 +477,7 @@ int mote_hip_route_experts_f32(const void* logits, const void* bias, void* ids, 
  * top x t + j, in the order of their experts and within one of their numbers.  rows (int32
  * [tokens x top]): the pairs; expert e has rows offsets[e] up to offsets[e + 1] (int32
  * [experts + 1]).  A pair whose id is not in 0 .. experts - 1 has no row; the rows
- * past offsets[experts] are -1.
+ * past offsets[experts] are -1.  None of the arrays may overlap another.
  * Status: 0; -1 for a null pointer, int32 arrays off their alignment, more than 1024
  * experts, top above 64, 2^30 pairs or tokens; the launch status.  No expert: 0 without a launch. */
 int mote_hip_plan_experts(const void* ids, void* offsets, void* rows, uint64_t tokens, uint64_t top,
@@ -496,7 +497,8 @@ int mote_hip_plan_experts(const void* ids, void* offsets, void* rows, uint64_t t
  * plan must belong together.
  *
  * Offsets that run past the pairs are cut to them, and a row that names no pair reads
- * token 0 or is left out.  Nothing is allocated, and a call can be captured.
+ * token 0 or is left out.  Outputs and workspace must not alias inputs.  Nothing is allocated, and a
+ * call can be captured.
  * Status: 0; -1 for a null pointer (a workspace of which 0 bytes are needed excepted), operands as for
  * mx_linear, int32 or float arrays off their alignment, hidden or inner not a multiple of 32 or
  * above 2^24, more than 1024 experts, top above 64, 2^30 pairs or tokens, too small a

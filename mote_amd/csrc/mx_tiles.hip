@@ -91,6 +91,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     if (blockIdx.x >= units * columns) return;
     const Place place = place_of(blockIdx.x, units, columns);
     const Tile tile = tiles.at(a, place.unit);
+    if (tile.count == 0) return;  // (offsets of no plan)
     const uint32_t column = place.column * kColumns;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -309,7 +310,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
                 if (stage % 4 == 0) load_scales(stage / 4 + 1);
                 run_stage(stage, std::false_type{}, k0);
             }
-        } else {  // two stages more: K has four at least
+        } else {  // two stages more, K having four at least, in straight code (in a loop: 256 registers for 206)
             static_assert(STAGES == 3, "the last two stages");
             run_stage(stage++, std::false_type{}, k0);
         }

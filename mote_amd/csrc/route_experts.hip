@@ -23,7 +23,6 @@
 namespace mote::mx {
 namespace {
 
-
 struct RouteArgs {
     const void* logits;
     const float* bias;  // or null

@@ -19,8 +19,10 @@ class ExpertsMX:
 
     ``bits``: of the activations, 4 or 6.  ``score``, ``groups``, ``top_groups``,
     ``group_best``, ``renormalize`` and ``scale`` as for ``ops.route_experts_f32``.
-    All memory is taken here, for up to ``max_tokens`` tokens: ``forward`` allocates nothing,
-    does not wait, and can be captured.  Its calls share that memory, so they follow
+    Weights come by ``load``, or, already in 4 bits, to ``gate_up`` and ``down`` and their scales
+    (an expert's gate rows, its up rows, the next expert's; down rows likewise); what an expert
+    computes before is undefined.  All memory is taken here, for up to ``max_tokens`` tokens:
+    ``forward`` allocates nothing, does not wait, and can be captured.  Its calls share that memory, so they follow
     each other on one stream (or are ordered by the caller).
     """
 

@@ -13,6 +13,7 @@ import mx_oracle as mx
 from mote_amd import ops
 from mote_amd.device import DeviceBuffer
 from mote_amd.experts import ExpertsMX
+from mote_amd.hip_runtime import HipRuntime
 
 pytestmark = pytest.mark.gpu
 
@@ -20,7 +21,8 @@ sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(
 
 
 @pytest.mark.parametrize("bits,logits_f16", [(4, False), (6, True)])
-@pytest.mark.parametrize("tokens,top,experts,hidden,inner", [(1, 2, 4, 64, 32), (37, 3, 8, 288, 160), (260, 2, 4, 544, 96)])
+@pytest.mark.parametrize("tokens,top,experts,hidden,inner",
+                         [(1, 2, 4, 64, 32), (37, 3, 8, 288, 160), (260, 2, 4, 544, 96)])
 def test_steps(stream, tokens, top, experts, hidden, inner, bits, logits_f16):
     rng = np.random.default_rng(tokens + bits)
     bias = 0.1 * rng.standard_normal(experts)
@@ -70,6 +72,35 @@ def test_steps(stream, tokens, top, experts, hidden, inner, bits, logits_f16):
     got = y.download(np.float16).reshape(tokens, hidden)
     bound = 2.0 ** -11 * np.abs(total) + (inner / 32 + inner / 128 + top + 4) * 2.0 ** -23 * deep + 2.0 ** -25
     assert (np.abs(got - total) <= bound).all()
+    block.free()
+
+
+def test_two_graphs(stream):
+    """Calls of two sizes captured, replayed in turn with other inputs: each equal to the call made
+    at once, though they share the object's memory."""
+    tokens, top, experts, hidden, inner = (200, 3), 2, 8, 256, 96
+    rng = np.random.default_rng(9)
+    block = ExpertsMX(experts, top, hidden, inner, 200)
+    for e in range(experts):
+        block.load(e, *(rng.standard_normal(s).astype(np.float32) / np.sqrt(s[1])
+                        for s in ((inner, hidden), (inner, hidden), (hidden, inner))), stream)
+    x, logits, y = (DeviceBuffer(n) for n in (tokens[0] * hidden * 2, tokens[0] * experts * 4, tokens[0] * hidden * 2))
+    rt = HipRuntime()
+    graphs = [rt.capture(stream, lambda n=n: block.forward(x.ptr, logits.ptr, y.ptr, n, stream)) for n in tokens]
+    for i in range(6):
+        n = tokens[i % 2]
+        x.upload(rng.standard_normal((tokens[0], hidden)).astype(np.float16))
+        logits.upload(rng.standard_normal((tokens[0], experts)).astype(np.float32))
+        block.forward(x.ptr, logits.ptr, y.ptr, n, stream)
+        stream.synchronize()
+        want = y.download(np.uint16, count=n * hidden)
+        y.upload(np.full(tokens[0] * hidden, 0x7B7B, np.uint16))
+        rt.launch_graph(graphs[i % 2], stream)
+        stream.synchronize()
+        np.testing.assert_array_equal(y.download(np.uint16, count=n * hidden), want)
+        assert (y.download(np.uint16)[n * hidden:] == 0x7B7B).all()
+    for graph in graphs:
+        rt.destroy_graph(graph)
     block.free()
 
 
