@@ -16,9 +16,9 @@ namespace {
 // STEPS steps of K, the same for every column, and the waves' sums meet in LDS, in their order.
 //
 // A lane's operand is a 16-byte piece of a weights' row as it is stored, so nothing is
-// unpacked; what costs time beside the memory is the number of load instructions (14336 x 4096,
+// unpacked; what costs time beside the memory is the number of load instructions (one row, 14336 x 4096,
 // 31 MB that are read in 6.1 us at best: weights alone 6.9 us, with their scales a word at a
-// time and x at each step 11.5).  So scales are loaded four steps at a time, x once for all
+// time and x at each step 11.5, as here 8.2).  So scales are loaded four steps at a time, x once for all
 // of the workgroup's columns, and a step's weights for the next column as soon as they
 // have been multiplied.
 constexpr uint32_t kFewRows = 16;
@@ -178,8 +178,8 @@ __global__ __launch_bounds__(256) void combine_kernel(CombineArgs a) {
 }
 
 // Columns of a workgroup: more of them share the loads of x, but there have to be workgroups
-// enough (one row, 14336 x 4096: 10.3 us with one, 9.0 with two, 9.6 with four of 224
-// workgroups; 4096 x 4096, 256 columns: 4.2 with one, 5.2 with two).
+// enough (one row, 14336 x 4096: 10.5 us with one, 9.1 with two, 9.6 with four of 224
+// workgroups; 4096 x 4096, 256 columns: 5.6 with two, 8.2 with four).
 constexpr uint64_t kWorkgroups = 448, kMostColumns = 4;
 
 template <int BITS, Result R, int STEPS, int MOST_WAVES>
@@ -197,17 +197,31 @@ int launch_few(const ProductArgs& a, hipStream_t stream) {
     return static_cast<int>(hipGetLastError());
 }
 
-// Few rows up to 16, or 8 of an expert in the mean (32 experts of 2880 x 2880, gate/up: 2
-// rows each 45 us and 51 in tiles, 8 rows 63 and 66, 16 rows 88 and 83); where K is too long for the
-// waves of a workgroup, or too short for the tiles' four steps, the other kernel has them.
+// Few rows, where the tiles (mx_tiles.hip) would leave much of the chip without one, or work with few of their rows:
+// - a linear of up to 16 rows whose weights are few long rows (one row, 4096 x 14336 10.6 us, 13.3 in tiles;
+//   4096 x 4096 6.4 and 5.5, 1024 x 8192 6.5 and 6.1, 14336 x 4096 8.2 and 6.0, read from the memory-side cache);
+// - gate/up of less than 8 rows of an expert in the mean (32 experts of 2880 x 2880, 6 bits: a row each 41 us and
+//   45, 4 rows 63 and 70, 8 rows 74.5 and 73.4; 128 experts of 768 x 2048, 8 rows 54 and 46);
+// - down of up to 8, where there are few tiles (8 experts of 4096 x 14336, 4 tokens of two: 256 tiles, 28 us
+//   and 57; 64 experts of 4096 x 1408, 2 tokens of six: 384, 16.1 and 17.2; 128 of 2048 x 768, 4 of eight: 512, 14.8 and
+//   12.6);
+// - and K too short for the tiles' four steps, if it is not too long for a workgroup's waves.
+template <Result R>
+bool few_rows(const ProductArgs& a) {
+    const uint64_t columns = a.outputs, steps = a.kp / kStep;
+    if (steps < 4) return true;
+    if constexpr (R == Result::kGateUp) return a.rows < 8 * uint64_t{a.experts} && steps <= 64;
+    if constexpr (R == Result::kPairs)
+        return a.rows <= 8 * uint64_t{a.experts} && steps <= 128 &&
+               most_expert_tiles(a.rows, a.experts, 64) * ((columns + 127) / 128) < 512;
+    return a.rows <= kFewRows && columns <= 32 * 191 && steps > 64 && steps <= 128;
+}
+
 template <int BITS, Result R>
 int launch_bits(const ProductArgs& a, hipStream_t stream) {
-    constexpr bool kTwo = R == Result::kGateUp;  // twice the registers: no eight steps of K a wave
-    const uint32_t steps = a.kp / kStep;
-    const bool few = kOfExperts<R> ? a.rows <= 8 * uint64_t{a.experts} : a.rows <= kFewRows;
-    if (steps >= 4 && (!few || steps > (kTwo ? 64 : 128))) return launch_tiles(R, a, BITS, stream);
-    if constexpr (!kTwo) {
-        if (steps > 64) return launch_few<BITS, R, 8, 16>(a, stream);
+    if (!few_rows<R>(a)) return launch_tiles(R, a, BITS, stream);
+    if constexpr (R != Result::kGateUp) {  // (twice the registers: no eight steps of K a wave)
+        if (a.kp / kStep > 64) return launch_few<BITS, R, 8, 16>(a, stream);
     }
     return launch_few<BITS, R, 4, 16>(a, stream);
 }

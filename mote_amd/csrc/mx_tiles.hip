@@ -434,34 +434,43 @@ int launch(const ProductArgs& a, hipStream_t stream) {
     return static_cast<int>(hipGetLastError());
 }
 
-// A linear takes the largest tile of which there is one for three in four compute units: a
-// workgroup's time hardly depends on how many others run (4096 outputs of 4096, 6 bits: 256 rows
-// in 32, 64, 128 and 256 tiles of 256 x 256, 128 x 128, 128 x 64 and 64 x 64: 36, 19, 15 and 11 us;
-// 4096 rows in 256, 1024, 2048 and 4096 of them: 52, 77, 95 and 133 us).  With fewer than
-// the smallest tiles' 192, waves divide K.
+// A linear takes the largest tile, no taller than its rows need, of which there is one for three in
+// four compute units: a workgroup's time hardly depends on how many others run (4096 outputs
+// of 4096, 6 bits: 64 rows in 32, 64 and 256 tiles of 128 x 64, 64 x 64 and 32 x 32: 14.3, 10.4 and 6.8 us;
+// 256 rows in 64, 128 and 256 of 128 x 128, 128 x 64 and 64 x 64: 17.5, 14.6 and 12.0; 4096 rows in 256, 1024
+// and 2048 of 256 x 256, 128 x 128 and 128 x 64: 56, 76 and 95).  In the small ones waves divide K.
 constexpr uint64_t kEnough = 192;
 
 template <int BITS, Result R>
 int choose(const ProductArgs& a, hipStream_t stream) {
+    const auto enough = [&](uint32_t weight_rows, uint32_t rows) {
+        return row_tiles<R>(a, rows) * column_tiles<R>(a, weight_rows) >= kEnough;
+    };
     if constexpr (kOfExperts<R>) {
-        // An expert's rows seldom fill its last tile, so tiles follow the mean of the rows (32 experts of
-        // 2880 x 2880, gate/up: 32 rows each 97 and 87 us in tiles of 64 and 128 rows, 128 rows 151
-        // and 147, 256 rows 242 and 240 of 128 and 256; 128 experts of 768 x 2048, 16 rows 44 and 50, 64
-        // rows 58 and 67).
+        // An expert's rows seldom fill its last tile, so tiles follow the mean of the rows (gate/up, 6 bits, us;
+        // 32 experts of 2880 x 2880, and 128 of 768 x 2048):
+        //   rows       16          32        64         128   256         500
+        //   256 x 32    85    53  101    61
+        //   128 x 64    92    56   92    60  127    74  159  271   163  451
+        //   128 x 128                  104  106    72  146  204   144  367
+        //   256 x 256                                   154  199   143  290
+        // (4 bits: at 16 rows 78 and 51 in 128 x 64, 82 and 51 in 256 x 32.  Of 80 more products of 256 rows and
+        // more 256 x 256 was the faster in 60.)
         const uint64_t mean = a.rows / a.experts;
-        if (mean >= 256 && row_tiles<R>(a, 256) * column_tiles<R>(a, 256) >= kEnough)
-            return launch<BITS, R, 256, 256, 2, 2, 1, 3>(a, stream);
+        if (mean >= 256 && enough(256, 256)) return launch<BITS, R, 256, 256, 2, 2, 1, 3>(a, stream);
         if (mean >= 96) return launch<BITS, R, 128, 128, 2, 2, 1, 3>(a, stream);
+        if constexpr (R == Result::kGateUp && BITS == 6) {
+            if (mean < 24) return launch<BITS, R, 256, 32, 4, 1, 1, 3>(a, stream);
+        }
         return launch<BITS, R, 128, 64, 2, 2, 1, 3>(a, stream);
     } else {
-        const auto enough = [&](uint32_t weight_rows, uint32_t rows) {
-            return row_tiles<R>(a, rows) * column_tiles<R>(a, weight_rows) >= kEnough;
-        };
-        if (enough(256, 256)) return launch<BITS, R, 256, 256, 2, 2, 1, 3>(a, stream);
-        if (enough(128, 128)) return launch<BITS, R, 128, 128, 2, 2, 1, 3>(a, stream);
-        if (enough(128, 64)) return launch<BITS, R, 128, 64, 2, 2, 1, 3>(a, stream);
-        if (enough(64, 64)) return launch<BITS, R, 64, 64, 1, 1, 4, 3>(a, stream);
-        if (enough(32, 64)) return launch<BITS, R, 32, 64, 1, 1, 4, 4>(a, stream);
+        if (a.rows > 32) {
+            if (enough(256, 256)) return launch<BITS, R, 256, 256, 2, 2, 1, 3>(a, stream);
+            if (enough(128, 128)) return launch<BITS, R, 128, 128, 2, 2, 1, 3>(a, stream);
+            if (enough(128, 64)) return launch<BITS, R, 128, 64, 2, 2, 1, 3>(a, stream);
+            if (enough(64, 64)) return launch<BITS, R, 64, 64, 1, 1, 4, 3>(a, stream);
+        }
+        if (enough(64, 32)) return launch<BITS, R, 64, 32, 1, 1, 2, 4>(a, stream);
         return launch<BITS, R, 32, 32, 1, 1, 4, 4>(a, stream);
     }
 }

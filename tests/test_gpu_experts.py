@@ -228,6 +228,17 @@ def test_products(stream, tokens, top, experts, hidden, inner, bits):
     case.check_down(stream, rng, bits)
 
 
+@pytest.mark.parametrize("bits", [4, 6])
+@pytest.mark.parametrize("tokens,top,experts,hidden,inner", [
+    (60, 2, 8, 544, 416), (47, 4, 20, 1024, 160), (95, 1, 4, 512, 128), (96, 1, 4, 640, 96),  # 8 to 24 rows an expert
+    (30, 8, 60, 1120, 512)])                                                          # few, in many tiles
+def test_products_of_few_rows_each(stream, tokens, top, experts, hidden, inner, bits):
+    rng = np.random.default_rng(tokens + experts + hidden + bits)
+    case = Case(rng, tokens, top, experts, hidden, inner)
+    case.check_gate_up(stream, rng, bits)
+    case.check_down(stream, rng, bits)
+
+
 @pytest.mark.parametrize("hidden,inner", [(8192, 64), (8224, 32), (64, 8192), (32, 16384), (32, 16416)])
 def test_long_rows_of_few_tokens(stream, hidden, inner):
     rng = np.random.default_rng(hidden + inner)

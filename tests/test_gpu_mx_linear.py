@@ -61,6 +61,16 @@ def test_larger(stream, rows, n, k, bits):
     check(stream, rows, n, k, bits, rows % 2 == 0)
 
 
+@pytest.mark.parametrize("bits", [4, 6])
+@pytest.mark.parametrize("rows,n,k", [
+    (1, 12225, 512), (7, 12289, 2880), (32, 12300, 416), (31, 12777, 640),  # 64 x 32, K in two
+    (100, 3100, 1184), (200, 1790, 544), (257, 1400, 896), (33, 6111, 800),
+    (17, 200, 8320), (16, 6100, 8224), (16, 6113, 8224), (2, 64, 65536),    # long rows, few and more of them
+])
+def test_few_rows(stream, rows, n, k, bits):
+    check(stream, rows, n, k, bits, rows % 2 == 0)
+
+
 @pytest.mark.parametrize("rows", [1, 40, 300])
 def test_no_features_and_nothing(stream, rows):
     empty = np.zeros(16, np.uint8)
