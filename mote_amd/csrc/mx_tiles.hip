@@ -8,6 +8,12 @@
 // at piece ^ (row / 4 % 4), so 16 lanes that read the same piece of 16 rows touch every
 // bank once.  One barrier a stage: behind it, all waves' loads of the stage have
 // landed and the stage before is free to be loaded again.
+//
+// Large tiles are held by the loads' issue: with all compute units at work a unit takes 36 bytes a cycle in
+// pieces of 64 bytes (53 in pieces of 128), so the 34 KB of a step of 256 x 256 take some 950 cycles
+// in which waves wait to issue, beside 1024 of matrix instructions at most: 4096 x 14336 x 4096 in 4 bits
+// 154 us, matrix cores busy 39 % of the cycles, 3.1 PFLOP/s of the 6.2 that the instruction reaches
+// on registers alone.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

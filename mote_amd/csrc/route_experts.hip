@@ -11,7 +11,9 @@
 // then that of the formula, not of roundings, but for logits that differ by less than 2^-50.  A wave
 // has a token, expert 64 v + lane in its lanes' slots v; a choice is compared as the unsigned number
 // that orders like it, and the largest is found in the upper halves alone unless two
-// lanes share it.
+// lanes share it.  Bound by instructions: 4096 tokens of 256 experts in 8 groups, 8 of them, take 10.4 to 11.6 us
+// (their bytes 0.9), for the exponentials in 64 bits and a maximum over the lanes for each expert taken; one token
+// of 128 experts 3.9 us, a launch's chain.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -258,7 +260,8 @@ struct PlanArgs {
 // always the same.  A thread has four neighbouring pairs in each of up to kTurns turns, all
 // in its registers (so up to 32768 pairs are read once, with whole lines to a wave); a wave's own are bits of
 // ballots, and where they go is a prefix sum over turns and waves.  More pairs go by in rounds that are
-// counted first.
+// counted first.  Bound by the ids, which every workgroup reads from the L2 and compares: 32768 pairs of 256
+// experts 7.9 to 8.4 us, a token's eight of 128 experts 2.9.
 constexpr uint32_t kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64, kMostTurns = 8;
 
 // per: turns of a round, up to TURNS (one, where that is all: a single token's plan is bound by
