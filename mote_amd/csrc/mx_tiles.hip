@@ -9,11 +9,11 @@
 // bank once.  One barrier a stage: behind it, all waves' loads of the stage have
 // landed and the stage before is free to be loaded again.
 //
-// Large tiles are held by the loads' issue: with all compute units at work a unit takes 36 bytes a cycle in
-// pieces of 64 bytes (53 in pieces of 128), so the 34 KB of a step of 256 x 256 take some 950 cycles
-// in which waves wait to issue, beside 1024 of matrix instructions at most: 4096 x 14336 x 4096 in 4 bits
-// 154 us, matrix cores busy 39 % of the cycles, 3.1 PFLOP/s of the 6.2 that the instruction reaches
-// on registers alone.
+// What bounds large ones (4096 x 14336 x 4096 in 4 bits, 148 us, 3.2 PFLOP/s of the 6.2 that the instruction reaches on
+// registers alone; each part taken out in turn): the matrix instructions alone some 98 us, in four
+// rounds of 3.5 rounds' tiles; the results, which all compute units write at one time, 24; the loads 22, LDS
+// reads 13.  Stages of 256 elements, whose loads have pieces of 128 bytes (53 bytes a cycle and compute
+// unit in place of 36), were level (152 and 154 us) and slower for experts (130 and 122).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -45,19 +45,22 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 // The tile of workgroup `at`.  Workgroups go to the 8 XCDs in turn: each gets a run of
-// tiles, of kBand row tiles by all columns, columns outside, so that those it
-// computes at one time share rows of both operands in its L2.
-constexpr uint32_t kBand = 4;
+// tiles, of BAND row tiles by all columns, columns outside, so that those it
+// computes at one time share rows of both operands in its L2.  (Experts have bands of one, as the next
+// tile of rows is often another's: 5000 tokens' four of 32 experts of 2880 x 2880, down, 265 us, 284 in
+// bands of four.  Linears: 4096 x 28672 x 1024 141 us in bands of one, 136 of four, 131 of eight; 8192 x 4096 x 4096
+// 89, 87 and 94.)
 struct Place {
     uint32_t unit, column;
 };
+template <uint32_t BAND>
 __device__ __forceinline__ Place place_of(uint32_t at, uint32_t units, uint32_t columns) {
     const uint32_t total = units * columns;
     const uint32_t xcd = at % 8, each = total / 8, more = total % 8;
     const uint32_t t = xcd * each + min(xcd, more) + at / 8;
-    const uint32_t band = t / (kBand * columns), in_band = t - band * kBand * columns;
-    const uint32_t height = min(kBand, units - band * kBand);
-    return {band * kBand + in_band % height, in_band / height};
+    const uint32_t band = t / (BAND * columns), in_band = t - band * BAND * columns;
+    const uint32_t height = min(BAND, units - band * BAND);
+    return {band * BAND + in_band % height, in_band / height};
 }
 
 // WN x WM waves divide a tile, or WK waves divide K and add their sums at the end, in their order.
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     const Tiles<R, BM> tiles(a);
     const uint32_t units = tiles.total();
     if (blockIdx.x >= units * columns) return;
-    const Place place = place_of(blockIdx.x, units, columns);
+    const Place place = place_of<kOfExperts<R> ? 1 : 4>(blockIdx.x, units, columns);
     const Tile tile = tiles.at(a, place.unit);
     if (tile.count == 0) return;  // (offsets of no plan)
     const uint32_t column = place.column * kColumns;
@@ -358,6 +361,9 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
 
     // Results leave as whole rows: a wave turns 32 rows of up to 256 bytes at a time in LDS of
     // its own (rows 16 bytes apart more, so that 8 lanes writing 16 or 8 bytes touch all banks).
+    // Those of the largest tiles, tens of megabytes of all compute units at one time, go past the caches
+    // (256 experts' rows and more: down of 128 experts 331 -> 312 us, of 64 408 -> 374, 4096 x 14336 x 4096 151 -> 148).
+    constexpr bool kPast = BN * BM == 256 * 256;
     constexpr bool kHalf = R == Result::kGateUp || R == Result::kF16;
     constexpr int kSize = kHalf ? 2 : 4;
     constexpr int kOut = kGate ? NF / 2 : NF;                         // 32-column products of the wave
@@ -404,7 +410,10 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
                 }
                 uint8_t* const out = static_cast<uint8_t*>(a.output) + (to * a.outputs + n) * kSize;
                 if (n + kPer <= a.outputs) {
-                    *reinterpret_cast<u32x4_a2*>(out) = word;
+                    if constexpr (kPast)
+                        __builtin_nontemporal_store(static_cast<u32x4_a2>(word), reinterpret_cast<u32x4_a2*>(out));
+                    else
+                        *reinterpret_cast<u32x4_a2*>(out) = word;
                 } else {  // the last of a row that is no whole number of pieces
                     for (uint32_t i = 0; n + i < a.outputs; ++i) {
                         if constexpr (kHalf)
