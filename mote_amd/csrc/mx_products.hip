@@ -198,13 +198,14 @@ int launch_few(const ProductArgs& a, hipStream_t stream) {
 }
 
 // Few rows, where the tiles (mx_tiles.hip) would leave much of the chip without one, or work with few of their rows:
-// - a linear of up to 16 rows whose weights are few long rows (one row, 4096 x 14336 10.6 us, 13.3 in tiles;
-//   4096 x 4096 6.4 and 5.5, 1024 x 8192 6.5 and 6.1, 14336 x 4096 8.2 and 6.0, read from the memory-side cache);
+// - a linear of up to 16 rows whose weights are few long rows (one row, 4096 x 14336 10.5 us, 13.2 in tiles;
+//   4096 x 4096 5.8 and 5.1, 1024 x 8192 6.8 and 6.1; 14336 x 4096 9.4 in both, from the memory-side
+//   cache 8.2 and 6.0);
 // - gate/up of less than 8 rows of an expert in the mean (32 experts of 2880 x 2880, 6 bits: a row each 41 us and
-//   45, 4 rows 63 and 70, 8 rows 74.5 and 73.4; 128 experts of 768 x 2048, 8 rows 54 and 46);
-// - down of up to 8, where there are few tiles (8 experts of 4096 x 14336, 4 tokens of two: 256 tiles, 28 us
-//   and 57; 64 experts of 4096 x 1408, 2 tokens of six: 384, 16.1 and 17.2; 128 of 2048 x 768, 4 of eight: 512, 14.8 and
-//   12.6);
+//   44, 4 rows 63 and 66, 8 rows 74 and 71; 128 experts of 768 x 2048, 8 rows 54 and 45);
+// - down of up to 8, where there are few tiles (8 experts of 4096 x 14336, 4 tokens of two: 256 tiles, 30 us
+//   and 60; 64 experts of 4096 x 1408, 2 tokens of six: 384, 15.8 and 16.9; 128 of 2048 x 768, 4 of eight:
+//   512, 15.3 and 13.0);
 // - and K too short for the tiles' four steps, if it is not too long for a workgroup's waves.
 template <Result R>
 bool few_rows(const ProductArgs& a) {

@@ -362,7 +362,8 @@ __global__ __launch_bounds__(64 * WN * WM * WK) void tiles_kernel(ProductArgs a,
     // Results leave as whole rows: a wave turns 32 rows of up to 256 bytes at a time in LDS of
     // its own (rows 16 bytes apart more, so that 8 lanes writing 16 or 8 bytes touch all banks).
     // Those of the largest tiles, tens of megabytes of all compute units at one time, go past the caches
-    // (256 experts' rows and more: down of 128 experts 331 -> 312 us, of 64 408 -> 374, 4096 x 14336 x 4096 151 -> 148).
+    // (500 rows each, down of 128 experts of 2048 x 768 331 -> 312 us; 900 rows, 64 of 2048 x 1408 408 -> 374;
+    // 4096 x 14336 x 4096 151 -> 148).
     constexpr bool kPast = BN * BM == 256 * 256;
     constexpr bool kHalf = R == Result::kGateUp || R == Result::kF16;
     constexpr int kSize = kHalf ? 2 : 4;
@@ -452,8 +453,8 @@ int launch(const ProductArgs& a, hipStream_t stream) {
 // A linear takes the largest tile, no taller than its rows need, of which there is one for three in
 // four compute units: a workgroup's time hardly depends on how many others run (4096 outputs
 // of 4096, 6 bits: 64 rows in 32, 64 and 256 tiles of 128 x 64, 64 x 64 and 32 x 32: 14.3, 10.4 and 6.8 us;
-// 256 rows in 64, 128 and 256 of 128 x 128, 128 x 64 and 64 x 64: 17.5, 14.6 and 12.0; 4096 rows in 256, 1024
-// and 2048 of 256 x 256, 128 x 128 and 128 x 64: 56, 76 and 95).  In the small ones waves divide K.
+// 256 rows in 64, 128 and 256 of 128 x 128, 128 x 64 and 64 x 64: 17.8, 14.5 and 12.0; 4096 rows in 256, 1024
+// and 2048 of 256 x 256, 128 x 128 and 128 x 64: 50, 78 and 96).  In the small ones waves divide K.
 constexpr uint64_t kEnough = 192;
 
 template <int BITS, Result R>
@@ -464,18 +465,18 @@ int choose(const ProductArgs& a, hipStream_t stream) {
     if constexpr (kOfExperts<R>) {
         // An expert's rows seldom fill its last tile, so tiles follow the mean of the rows (gate/up, 6 bits, us;
         // 32 experts of 2880 x 2880, and 128 of 768 x 2048):
-        //   rows       16          32        64         128   256         500
-        //   256 x 32    85    53  101    61
-        //   128 x 64    92    56   92    60  127    74  159  271   163  451
-        //   128 x 128                  104  106    72  146  204   144  367
-        //   256 x 256                                   154  199   143  290
-        // (4 bits: at 16 rows 78 and 51 in 128 x 64, 82 and 51 in 256 x 32.  Of 80 more products of 256 rows and
-        // more 256 x 256 was the faster in 60.)
+        //   rows         8        16        32        64       128       256       500
+        //   256 x 32    71  45    85  53  102  61  136  82
+        //   128 x 64    74  48    80  54   91  59  121  74  165 106  272 170  488 288
+        //   128 x 128             81  60   92  66  104  73  134  92  201 143  355 236
+        //   256 x 256            101  74  104  77  114  94  140 104  183 137  274 197
+        // (4 bits, 8 rows: 75 and 45 in 256 x 32, 68 and 45 in 128 x 64; down, 64 rows: 75 and 62 in 128 x 64, 75 and
+        // 65 in 128 x 128.)
         const uint64_t mean = a.rows / a.experts;
         if (mean >= 256 && enough(256, 256)) return launch<BITS, R, 256, 256, 2, 2, 1, 3>(a, stream);
-        if (mean >= 96) return launch<BITS, R, 128, 128, 2, 2, 1, 3>(a, stream);
+        if (mean >= 64) return launch<BITS, R, 128, 128, 2, 2, 1, 3>(a, stream);
         if constexpr (R == Result::kGateUp && BITS == 6) {
-            if (mean < 24) return launch<BITS, R, 256, 32, 4, 1, 1, 3>(a, stream);
+            if (mean < 16) return launch<BITS, R, 256, 32, 4, 1, 1, 3>(a, stream);
         }
         return launch<BITS, R, 128, 64, 2, 2, 1, 3>(a, stream);
     } else {

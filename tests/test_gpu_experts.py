@@ -239,6 +239,17 @@ def test_products_of_few_rows_each(stream, tokens, top, experts, hidden, inner, 
     case.check_down(stream, rng, bits)
 
 
+@pytest.mark.parametrize("bits", [4, 6])
+@pytest.mark.parametrize("tokens,experts", [(150, 3), (190, 3), (130, 20), (700, 2), (1100, 3)])
+def test_one_expert_of_several_tiles(stream, tokens, experts, bits):
+    """More rows of one expert than the mean, by which the tiles are chosen, lets expect."""
+    rng = np.random.default_rng(tokens + bits)
+    ids = np.where(rng.random((tokens, 1)) < 0.95, 1, rng.integers(-1, experts, (tokens, 1))).astype(np.int32)
+    case = Case(rng, tokens, 1, experts, 544, 672, ids)
+    case.check_gate_up(stream, rng, bits)
+    case.check_down(stream, rng, bits)
+
+
 @pytest.mark.parametrize("hidden,inner", [(8192, 64), (8224, 32), (64, 8192), (32, 16384), (32, 16416)])
 def test_long_rows_of_few_tokens(stream, hidden, inner):
     rng = np.random.default_rng(hidden + inner)
