@@ -55,14 +55,33 @@ __device__ __forceinline__ uint32_t scale_of(uint32_t most) {
 }
 
 // The conversions of a whole block write their result in several passes while they still read, and the
-// compiler gives result and operand the same registers where it can: elements then came out
-// as others' bits.  So their operands are said to be in use a little longer.
-template <typename V>
-__device__ __forceinline__ void still_used(const V& v) {
+// compiler's own give result and operands the same registers where they can: elements then came out
+// as others' bits.  So they are written here, where the result can be said to be written early.  (The
+// compiler does not look into them for its wait states: two before and behind cover what a vector instruction needs
+// of another.)
 #ifdef __HIP_DEVICE_COMPILE__
-    asm volatile("" ::"v"(v));
+#define MOTE_CONVERT_BLOCK(instruction, result, ...) \
+    asm("s_nop 1\n\t" instruction "\n\ts_nop 1" : "=&v"(result) : __VA_ARGS__)
+#else
+#define MOTE_CONVERT_BLOCK(instruction, result, ...) (result = {})
 #endif
+__device__ __forceinline__ u32x6 to_six_bits(f16x32 v, float scale) {
+    u32x6 w;
+    MOTE_CONVERT_BLOCK("v_cvt_scalef32_pk32_fp6_f16 %0, %1, %2", w, "v"(v), "v"(scale));
+    return w;
 }
+// (The instruction takes its elements from the two in turn.)
+__device__ __forceinline__ u32x6 to_six_bits(f32x16 even, f32x16 odd, float scale) {
+    u32x6 w;
+    MOTE_CONVERT_BLOCK("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3", w, "v"(even), "v"(odd), "v"(scale));
+    return w;
+}
+__device__ __forceinline__ f32x32 from_six_bits(u32x6 codes) {
+    f32x32 v;
+    MOTE_CONVERT_BLOCK("v_cvt_scalef32_pk32_f32_fp6 %0, %1, 1.0", v, "v"(codes));
+    return v;
+}
+#undef MOTE_CONVERT_BLOCK
 
 template <int BITS>
 __device__ __forceinline__ Block<BITS> convert(const _Float16 (&x)[32], float scale) {
@@ -82,9 +101,7 @@ __device__ __forceinline__ Block<BITS> convert(const _Float16 (&x)[32], float sc
         f16x32 v;
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[i] = x[i];
-        const u32x6 w = __builtin_amdgcn_cvt_scalef32_pk32_fp6_f16(v, scale);
-        still_used(v);
-        still_used(scale);
+        const u32x6 w = to_six_bits(v, scale);
         b.low = u32x4{w[0], w[1], w[2], w[3]};
         b.high = u32x2{w[4], w[5]};
     }
@@ -105,16 +122,13 @@ __device__ __forceinline__ Block<BITS> convert(const float (&x)[32], float scale
             b.low[i] = word;
         }
     } else {
-        f32x16 even, odd;  // the instruction takes its elements from the two in turn
+        f32x16 even, odd;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             even[i] = x[2 * i];
             odd[i] = x[2 * i + 1];
         }
-        const u32x6 w = __builtin_amdgcn_cvt_scalef32_2xpk16_fp6_f32(even, odd, scale);
-        still_used(even);
-        still_used(odd);
-        still_used(scale);
+        const u32x6 w = to_six_bits(even, odd, scale);
         b.low = u32x4{w[0], w[1], w[2], w[3]};
         b.high = u32x2{w[4], w[5]};
     }
@@ -204,8 +218,7 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(RowArgs a) {
             }
         } else {
             const u32x6 codes = {b.low.x, b.low.y, b.low.z, b.low.w, b.high.x, b.high.y};
-            const f32x32 w = __builtin_amdgcn_cvt_scalef32_pk32_f32_fp6(codes, 1.0f);
-            still_used(codes);
+            const f32x32 w = from_six_bits(codes);
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = w[i];
         }
