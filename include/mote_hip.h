@@ -453,14 +453,17 @@ int mote_hip_mx_linear_f32(const void* input_values, const void* input_scales, c
 /* [new] No counterpart in the reference.  The `top` experts of each token: logits
  * [tokens, experts] -> ids (int32) and weights (float), [tokens, top] each, the best first.
  * score 0: softmax over the experts; 1: sigmoid.  The choice is by score + bias[expert]
- * (float, NULL: none), the lowest index first among equals; the bias is not in the weights.
+ * (float), by the logit where bias is NULL, for both scores grow with it; equal choices go by the logit,
+ * then the lowest index first; the bias is not in the weights.
  * With top_groups < groups the experts are `groups` runs of experts / groups; a group's
  * worth is the sum of its group_best (1 or 2) best choices, as many as it has, and only the experts of
  * the top_groups best groups are chosen.  weights = scale x score, divided by the chosen
  * scores' sum with renormalize = 1 (0 where that is 0).  An expert whose logit, or whose score +
  * bias, is infinite or NaN takes no part (a logit that is, not in the softmax either);
  * where fewer than `top` are left the ids are -1 and the weights 0, so a row of
- * -infinity is a token without experts.  Scores are held in 64 bits.
+ * -infinity is a token without experts.  Scores are held in 64 bits: choices of different biases, and
+ * worths, that differ by less than 2^-50 (of the larger, or of 1) can come in either order; a score under 2^-1022,
+ * of a softmax's logit 708 below the largest or a sigmoid's below -708, can be 0 in the weights and in the worth of two.
  * Status: 0; -1 for a null pointer (bias excepted), logits, bias, ids or weights off
  * their alignment, score or renormalize other than 0 or 1, group_best other than 1 or 2, a scale that is
  * not finite, more than 1024 experts, top above 64 or above the experts that the groups leave, groups that do not

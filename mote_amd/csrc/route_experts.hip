@@ -7,11 +7,17 @@
 // one or two choices and only the experts of the best groups stay.  The `top`
 // largest choices are taken, the lowest index first among equals.
 //
-// The choice is a comparison, so scores, choices and worths are held in 64 bits: it is
-// then that of the formula, not of roundings, but for logits that differ by less than 2^-50.  A wave
-// has a token, expert 64 v + lane in its lanes' slots v; a choice is compared as the unsigned number
+// The choice is a comparison, and 64 bits do not tell all scores apart: sigmoids of 37 and
+// more are 1, softmaxes of 746 under the largest 0.  Both scores grow with the logit, so without a
+// bias the logits are compared, and equal choices by their logits (scores of different logits and biases never
+// add up to the very same number).  Worths of two choices that are equal where it matters, between the last group that stays
+// and the first that does not, are told apart by what 64 bits dropped (rest_of); the whole token is then
+// done again, slowly: 4096 tokens of 256 logits that are all equal, in 8 groups, take 29 us.  What can still come in
+// either order are choices of different biases, and worths, less than 2^-50 apart.
+//
+// A wave has a token, expert 64 v + lane in its lanes' slots v; a choice is compared as the unsigned number
 // that orders like it, and the largest is found in the upper halves alone unless two
-// lanes share it.  Bound by instructions: 4096 tokens of 256 experts in 8 groups, 8 of them, take 10.4 to 11.6 us
+// lanes share it.  Bound by instructions: 4096 tokens of 256 experts in 8 groups, 8 of them, take 9.3 us in a row
 // (their bytes 0.9), for the exponentials in 64 bits and a maximum over the lanes for each expert taken; one token
 // of 128 experts 3.9 us, a launch's chain.
 #include <hip/hip_runtime.h>
@@ -21,6 +27,7 @@
 #include <cstdint>
 
 #include "mx_products.hpp"
+#include "tile_ops.hpp"
 
 namespace mote::mx {
 namespace {
@@ -49,11 +56,13 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     v = max_dpp<0x143, 0xC>(v);  // row_bcast:31 into rows 2 and 3
     return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
 }
+__device__ __forceinline__ uint64_t lane_value(uint64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
 __device__ __forceinline__ double lane_value(double v, int lane) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane);
-    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+    return __builtin_bit_cast(double, lane_value(__builtin_bit_cast(uint64_t, v), lane));
 }
 template <int Ctrl, int RowMask = 0xF>
 __device__ __forceinline__ double add_dpp64(double v) {
@@ -71,13 +80,6 @@ __device__ __forceinline__ double wave_sum64(double v) {
     v = add_dpp64<0x143, 0xC>(v);
     return lane_value(v, 63);
 }
-// The largest of finite numbers and -infinity.
-__device__ __forceinline__ float wave_max_float(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const uint32_t most = wave_max(b >> 31 ? ~b : b | 0x80000000u);
-    return __builtin_bit_cast(float, most >> 31 ? most & 0x7FFFFFFFu : ~most);
-}
-
 // Orders as the number does, above 0; 0 is for what takes no part.
 __device__ __forceinline__ uint64_t order_of(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);  // -0 as 0
@@ -86,7 +88,76 @@ __device__ __forceinline__ uint64_t order_of(double v) {
 __device__ __forceinline__ double value_of(uint64_t order) {
     return __builtin_bit_cast(double, order >> 63 ? order & ~(uint64_t{1} << 63) : ~order);
 }
+__device__ __forceinline__ uint32_t order_of(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
+    return b >> 31 ? ~b : b | 0x80000000u;
+}
+// The largest of finite numbers and -infinity.
+__device__ __forceinline__ float wave_max_float(float v) {
+    const uint32_t most = wave_max(order_of(v));
+    return __builtin_bit_cast(float, most >> 31 ? most & 0x7FFFFFFFu : ~most);
+}
 __device__ __forceinline__ bool finite(double v) { return __builtin_isfinite(v); }
+
+// Of a logit that is finite, or -infinity for one that takes no part: all in the upper half.
+__device__ __forceinline__ uint64_t logit_choice(float x) {
+    return x != -__builtin_inff() ? static_cast<uint64_t>(order_of(x)) << 32 : 0;
+}
+
+// What tells groups of one worth apart, compared as they stand: the logit, where one choice is
+// the worth.  Of two, the parts of their scores that 64 bits drop: a sigmoid is kept as its distance
+// from 0 or 1, the nearer, their sum as its distance from the worth, and what that sum drops; softmaxes, which
+// may all be 0, as the logarithm of their sum (but for the row's own sum) and the lower logit.
+struct Rest {
+    uint64_t first, second;
+};
+template <typename T>
+__device__ Rest rest_of(const RouteArgs& a, const T* logits, const uint64_t* choices, uint64_t worth, uint32_t group) {
+    uint64_t choice[2] = {};
+    float x[2] = {-__builtin_inff(), -__builtin_inff()};
+    double bias[2] = {};
+    for (uint32_t e = group * a.size; e < (group + 1) * a.size; ++e) {
+        const uint64_t c = choices[e];
+        const float logit = static_cast<float>(logits[e]);
+        const double b = a.bias != nullptr ? static_cast<double>(a.bias[e]) : 0.0;
+        const bool best = c > choice[0] || (c == choice[0] && logit > x[0]);
+        if (c != 0 && best) choice[1] = choice[0], x[1] = x[0], bias[1] = bias[0];
+        if (c != 0 && (best || c > choice[1] || (c == choice[1] && logit > x[1])))
+            choice[best ? 0 : 1] = c, x[best ? 0 : 1] = logit, bias[best ? 0 : 1] = b;
+    }
+    if (a.best == 1 || a.size == 1) return {order_of(static_cast<double>(x[0])), 0};
+    // (With a bias the second may have the larger logit.)
+    const double most = fmax(x[0], x[1]), least = fmin(x[0], x[1]);
+    const double power = floor(most * 0x1.71547652b82fep0);  // log2 e
+    double t[2] = {a.sigmoid ? -fabs(static_cast<double>(x[0])) : least - most,
+                   a.sigmoid ? -fabs(static_cast<double>(x[1])) : fma(power, -0x1.62e42fefa39efp-1, most)};  // ln 2
+#pragma nounroll
+    for (int i = 0; i < 2; ++i) {
+        const double e = exp(t[0]);
+        t[0] = t[1], t[1] = e;
+    }
+    if (!a.sigmoid) {
+        const double size = (1.0 + t[0]) * t[1];
+        return {order_of(size < 2.0 ? power + (size - 1.0) : power + size * 0.5), order_of(least)};
+    }
+    double whole = bias[0] + bias[1], distance[2] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (choice[i] == 0) continue;
+        const double far = t[i] / (1.0 + t[i]);
+        whole += x[i] > 0.0f ? 1.0 : 0.0;
+        distance[i] = x[i] > 0.0f ? -far : far;
+    }
+    const double sum = distance[0] + distance[1], of_second = sum - distance[0];
+    const double dropped = distance[0] - (sum - of_second) + (distance[1] - of_second);
+    return {order_of(whole - value_of(worth) + sum), order_of(dropped)};
+}
+
+// Between a wave's writes to LDS and its other lanes' reads there.
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 
 // SLOTS: experts of a lane.  GROUPED: LDS holds the choices and the groups' worths.
 template <typename T, int SLOTS, bool GROUPED>
@@ -99,45 +170,54 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
     if (token >= a.tokens) return;
     const T* logits = static_cast<const T*>(a.logits) + static_cast<uint64_t>(token) * a.experts;
     float x[SLOTS];
-#pragma unroll
-    for (int v = 0; v < SLOTS; ++v) {
-        const uint32_t e = v * 64 + lane;
-        x[v] = e < a.experts ? static_cast<float>(logits[e]) : -__builtin_inff();
-        if (!__builtin_isfinite(x[v])) x[v] = -__builtin_inff();
-    }
     double score[SLOTS];
-    if (a.sigmoid) {
-#pragma unroll
-        for (int v = 0; v < SLOTS; ++v) score[v] = 1.0 / (1.0 + exp(-static_cast<double>(x[v])));
-    } else {
-        float most = x[0];
-#pragma unroll
-        for (int v = 1; v < SLOTS; ++v) most = fmaxf(most, x[v]);
-        most = wave_max_float(most);
-        double sum = 0.0;
+    uint64_t choice[SLOTS];
+    // Without a bias the logits are compared, and so are groups whose worth is one choice.
+    const bool by_score = a.bias != nullptr || (GROUPED && a.best == 2 && a.size > 1);
+    const auto find_scores = [&] {
 #pragma unroll
         for (int v = 0; v < SLOTS; ++v) {
-            const bool there = x[v] != -__builtin_inff();
-            score[v] = there ? exp(static_cast<double>(x[v]) - static_cast<double>(most)) : 0.0;
-            sum += score[v];
+            const uint32_t e = v * 64 + lane;
+            x[v] = e < a.experts ? static_cast<float>(logits[e]) : -__builtin_inff();
+            if (!__builtin_isfinite(x[v])) x[v] = -__builtin_inff();
         }
-        const double part = 1.0 / wave_sum64(sum);  // of no expert: unused
+        if (a.sigmoid) {
 #pragma unroll
-        for (int v = 0; v < SLOTS; ++v) score[v] *= part;
-    }
-    uint64_t choice[SLOTS];
+            for (int v = 0; v < SLOTS; ++v) score[v] = 1.0 / (1.0 + exp(-static_cast<double>(x[v])));
+        } else {
+            float most = x[0];
 #pragma unroll
-    for (int v = 0; v < SLOTS; ++v) {
-        const uint32_t e = v * 64 + lane;
-        double c = score[v];
-        if (a.bias != nullptr && e < a.experts) c += static_cast<double>(a.bias[e]);
-        choice[v] = x[v] != -__builtin_inff() && finite(c) ? order_of(c) : 0;
-    }
+            for (int v = 1; v < SLOTS; ++v) most = fmaxf(most, x[v]);
+            most = wave_max_float(most);
+            double sum = 0.0;
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) {
+                const bool there = x[v] != -__builtin_inff();
+                score[v] = there ? exp(static_cast<double>(x[v]) - static_cast<double>(most)) : 0.0;
+                sum += score[v];
+            }
+            const double part = 1.0 / wave_sum64(sum);  // of no expert: unused
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) score[v] *= part;
+        }
+        if (by_score) {
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) {
+                const uint32_t e = v * 64 + lane;
+                double c = score[v];
+                if (a.bias != nullptr && e < a.experts) c += static_cast<double>(a.bias[e]);
+                choice[v] = x[v] != -__builtin_inff() && finite(c) ? order_of(c) : 0;
+            }
+        } else {
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) choice[v] = logit_choice(x[v]);
+        }
+    };
+    find_scores();
     if constexpr (GROUPED) {
 #pragma unroll
         for (int v = 0; v < SLOTS; ++v) choices[wave][v * 64 + lane] = choice[v];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
         // `part` lanes share a group: its choices in turn, then their bests across the lanes.
         uint32_t part = 1;
         while (part * 2 * a.groups <= 64) part *= 2;
@@ -156,23 +236,27 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
                 second = max(max(second, d), min(first, c));
                 first = max(first, c);
             }
-            double worth = first ? value_of(first) : 0.0;
-            if (a.best == 2 && second) worth += value_of(second);
-            if (g < a.groups && lane % part == 0) worths[wave][g] = first ? order_of(worth) : 0;
+            if (a.best == 2 && second != 0) first = order_of(value_of(first) + value_of(second));
+            if (g < a.groups && lane % part == 0) worths[wave][g] = first;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        wave_fence();
         // Groups that fewer than top_groups others come before stay.
         const float part_of = 1.0f / static_cast<float>(a.size);  // e / size: e + 1/2 is 2^-11 away from the next
+        uint64_t last_in = 0, first_out = 0;  // worths
+        const auto note_border = [&](uint32_t before, uint64_t worth) {
+            const uint64_t in = __builtin_amdgcn_ballot_w64(before == a.top_groups - 1);
+            const uint64_t out = __builtin_amdgcn_ballot_w64(before == a.top_groups);
+            if (in != 0) last_in = lane_value(worth, __builtin_ctzll(in));
+            if (out != 0) first_out = lane_value(worth, __builtin_ctzll(out));
+        };
         if (a.groups <= 64) {
             const uint64_t worth = lane < a.groups ? worths[wave][lane] : 0;
             uint32_t before = 0;
             for (uint32_t g = 0; g < a.groups; ++g) {
-                const uint64_t other =
-                    static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(worth >> 32, g))) << 32 |
-                    static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(worth), g));
+                const uint64_t other = lane_value(worth, g);
                 before += other > worth || (other == worth && g < lane) ? 1 : 0;
             }
+            note_border(before, worth);
             const uint64_t kept = __builtin_amdgcn_ballot_w64(before < a.top_groups);
 #pragma unroll
             for (int v = 0; v < SLOTS; ++v) {
@@ -189,9 +273,48 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
                     const uint64_t other = worths[wave][g];
                     before += other > worth || (other == worth && g < mine) ? 1 : 0;
                 }
+                note_border(before, worth);
                 if (before >= a.top_groups) choice[v] = 0;
             }
         }
+        if (by_score && last_in == first_out && last_in != 0) {
+            // What tells equal worths apart, over choices that have been read.  Then all once more: to
+            // keep scores and choices meanwhile takes registers that halve the waves at work (16384 tokens of 256
+            // experts 28 us, 25 as here, whether there are such worths or not).
+            uint64_t* const rests = choices[wave];
+            const uint32_t each = min(a.size, 2u), last = each - 1;
+            for (uint32_t first_group = 0; first_group < a.groups; first_group += 64) {
+                const uint32_t g = first_group + lane;
+                Rest rest{};
+                if (g < a.groups && worths[wave][g] != 0) rest = rest_of(a, logits, rests, worths[wave][g], g);
+                wave_fence();
+                if (g < a.groups) {
+                    rests[g * each] = rest.first;
+                    if (each == 2) rests[g * 2 + 1] = rest.second;
+                }
+                wave_fence();
+            }
+            memory_fence();
+            find_scores();
+#pragma unroll
+            for (int v = 0; v < SLOTS; ++v) {
+                const uint32_t mine = min((v * 64 + lane) / a.size, a.groups - 1);
+                const uint64_t worth = worths[wave][mine], first = rests[mine * each], second = rests[mine * each + last];
+                uint32_t before = 0;
+                for (uint32_t g = 0; g < a.groups; ++g) {
+                    const uint64_t w = worths[wave][g], f = rests[g * each], s = rests[g * each + last];
+                    const bool level = w == worth && f == first;
+                    before += w > worth || (w == worth && f > first) || (level && (s > second || (s == second && g < mine)))
+                                  ? 1
+                                  : 0;
+                }
+                if (before >= a.top_groups) choice[v] = 0;
+            }
+        }
+    }
+    if (GROUPED && by_score && a.bias == nullptr) {
+#pragma unroll
+        for (int v = 0; v < SLOTS; ++v) choice[v] = choice[v] != 0 ? logit_choice(x[v]) : 0;
     }
     // The largest, `top` times; lane j keeps the j-th.  The upper halves decide unless two are equal.
     int32_t id = -1;
@@ -222,6 +345,21 @@ __global__ __launch_bounds__(256) void route_kernel(RouteArgs a) {
             for (int v = SLOTS - 1; v >= 0; --v) {
                 holders[v] = __builtin_amdgcn_ballot_w64(high[v] == most && static_cast<uint32_t>(choice[v]) == low);
                 slot = holders[v] ? v : slot;
+            }
+            if (a.bias != nullptr) {  // equal sums: the larger logit (read again: few rows come here)
+                uint32_t order[SLOTS], largest = 0;
+#pragma unroll
+                for (int v = 0; v < SLOTS; ++v) {
+                    const bool holds = holders[v] >> lane & 1;
+                    order[v] = holds ? order_of(static_cast<float>(logits[v * 64 + lane])) : 0;
+                    largest = max(largest, order[v]);
+                }
+                largest = wave_max(largest);
+#pragma unroll
+                for (int v = SLOTS - 1; v >= 0; --v) {
+                    holders[v] = __builtin_amdgcn_ballot_w64(order[v] == largest);
+                    slot = holders[v] ? v : slot;
+                }
             }
         }
         int winner = 0;
