@@ -31,8 +31,16 @@ class ExpertsMX:
                  renormalize: bool = True, scale: float = 1.0) -> None:
         if experts < 1 or not 1 <= top <= experts or max_tokens < 1:
             raise ValueError("an expert, a choice of no more than there are, and a token at least")
-        if hidden < 32 or inner < 32 or hidden % 32 or inner % 32:
-            raise ValueError("hidden and inner elements are multiples of 32")
+        if experts > 1024 or top > 64 or max_tokens > (1 << 26) - 4 or max_tokens * top > 1 << 30:
+            raise ValueError("up to 1024 experts, 64 of a token, 2^26 - 4 tokens and 2^30 choices")
+        if any(n < 32 or n % 32 or n > 1 << 24 for n in (hidden, inner)):
+            raise ValueError("hidden and inner elements are multiples of 32, up to 2^24")
+        if score not in (ops.SOFTMAX, ops.SIGMOID) or group_best not in (1, 2) or not abs(scale) <= np.finfo(np.float32).max:
+            raise ValueError("scores of softmax or sigmoid, groups by one or two choices, a finite scale")
+        if groups < 1 or experts % groups or not 1 <= top_groups <= groups:
+            raise ValueError("groups of as many experts each, and one of them at least")
+        if top > top_groups * (experts // groups):
+            raise ValueError("no more choices than the groups leave experts")
         if bits not in (4, 6):
             raise ValueError("activations of 4 or 6 bits")
         if bias is not None and np.shape(bias) != (experts,):
