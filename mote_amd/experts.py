@@ -10,6 +10,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import ops
+from ._ffi import check, lib
 from .device import DeviceBuffer
 
 
@@ -84,7 +85,7 @@ class ExpertsMX:
             held.append(DeviceBuffer.from_array(a))
             ops.mx_quantize_f32(held[-1].ptr, values.ptr + first * ops.mx_value_bytes(features, 4),
                                 scales.ptr + first * ops.mx_scale_bytes(features), rows, features, 4, stream)
-        stream.synchronize()
+        check(lib().mote_hip_stream_synchronize(ops._s(stream)), "synchronize stream")
 
     def forward(self, x: int, logits: int, y: int, tokens: int, stream, logits_f16: bool = False, stride=None) -> None:
         """y [tokens, hidden] (f16) of x (f16, rows `stride` elements apart) and router logits

@@ -47,3 +47,28 @@ def test_refusals_before_any_memory(buffers, change):
     with pytest.raises(ValueError):
         experts.ExpertsMX(**{**GOOD, **change})
     assert buffers.taken == 0
+
+
+@pytest.mark.parametrize("by_handle", [False, True])
+def test_load_waits_for_a_stream_or_its_handle(buffers, monkeypatch, by_handle):
+    events = []
+    monkeypatch.setattr(experts.ops, "mx_quantize_f32", lambda *a: events.append(("quantize", ops._s(a[-1]))))
+
+    class Library:
+        @staticmethod
+        def mote_hip_stream_synchronize(handle):
+            events.append(("wait", handle))
+            return 0
+
+    monkeypatch.setattr(experts, "lib", Library, raising=False)
+
+    class Stream:
+        handle = 0x77
+
+        def synchronize(self):
+            events.append(("wait", self.handle))
+
+    layer = experts.ExpertsMX(**GOOD)
+    gate = np.zeros((96, 64), np.float32)
+    layer.load(3, gate, gate, np.zeros((64, 96), np.float32), Stream.handle if by_handle else Stream())
+    assert events == [("quantize", 0x77)] * 3 + [("wait", 0x77)]
