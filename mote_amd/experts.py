@@ -36,7 +36,7 @@ class ExpertsMX:
             raise ValueError("up to 1024 experts, 64 of a token, 2^26 - 4 tokens and 2^30 choices")
         if any(n < 32 or n % 32 or n > 1 << 24 for n in (hidden, inner)):
             raise ValueError("hidden and inner elements are multiples of 32, up to 2^24")
-        if score not in (ops.SOFTMAX, ops.SIGMOID) or group_best not in (1, 2) or not abs(scale) <= np.finfo(np.float32).max:
+        if score not in (ops.SOFTMAX, ops.SIGMOID) or group_best not in (1, 2) or not abs(scale) <= 3.4028234663852886e38:
             raise ValueError("scores of softmax or sigmoid, groups by one or two choices, a finite scale")
         if groups < 1 or experts % groups or not 1 <= top_groups <= groups:
             raise ValueError("groups of as many experts each, and one of them at least")
