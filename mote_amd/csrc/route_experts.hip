@@ -17,9 +17,9 @@
 //
 // A wave has a token, expert 64 v + lane in its lanes' slots v; a choice is compared as the unsigned number
 // that orders like it, and the largest is found in the upper halves alone unless two
-// lanes share it.  Bound by instructions: 4096 tokens of 256 experts in 8 groups, 8 of them, take 9.3 us in a row
-// (their bytes 0.9), for the exponentials in 64 bits and a maximum over the lanes for each expert taken; one token
-// of 128 experts 3.9 us, a launch's chain.
+// lanes share it.  Bound by instructions: 4096 tokens of 256 experts in 8 groups, 8 of them, take 9.3 us one after
+// another (their bytes 0.7), for the exponentials in 64 bits and a maximum over the lanes for each expert taken; one token
+// of 128 experts 4.0 us, a launch's chain.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -126,11 +126,13 @@ __device__ Rest rest_of(const RouteArgs& a, const T* logits, const uint64_t* cho
             choice[best ? 0 : 1] = c, x[best ? 0 : 1] = logit, bias[best ? 0 : 1] = b;
     }
     if (a.best == 1 || a.size == 1) return {order_of(static_cast<double>(x[0])), 0};
-    // (With a bias the second may have the larger logit.)
+    // (With a bias the second may have the larger logit.)  e^most as 2^power e^left; what is left of logits so large
+    // that it cannot be known is held to where it has to be, under ln 2, which is here in two parts.
     const double most = fmax(x[0], x[1]), least = fmin(x[0], x[1]);
     const double power = floor(most * 0x1.71547652b82fep0);  // log2 e
+    const double left = fma(power, -0x1.abc9e3b39803fp-56, fma(power, -0x1.62e42fefa39efp-1, most));
     double t[2] = {a.sigmoid ? -fabs(static_cast<double>(x[0])) : least - most,
-                   a.sigmoid ? -fabs(static_cast<double>(x[1])) : fma(power, -0x1.62e42fefa39efp-1, most)};  // ln 2
+                   a.sigmoid ? -fabs(static_cast<double>(x[1])) : fmin(fmax(left, 0.0), 0x1.62e42fefa39efp-1)};
 #pragma nounroll
     for (int i = 0; i < 2; ++i) {
         const double e = exp(t[0]);

@@ -181,3 +181,30 @@ def test_far_groups_of_two_best(stream, experts, groups, top_groups, top, score,
     want = largest_first(logits, top, np.repeat(kept, size, 1))
     check(stream, logits, want, score, bias=None if bias is None else np.full(experts, bias), groups=groups,
           top_groups=top_groups, group_best=2)
+
+
+@pytest.mark.parametrize("bias", [None, 0.0])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("top_groups", [2, 4, 6, 9])
+def test_softmax_groups_of_any_size(stream, top_groups, dtype, bias):
+    """Groups of two best that all underflow, down to the type's lowest value: their best logits lie more
+    than log 2 apart, so they and then the second ones decide."""
+    rng = np.random.default_rng(top_groups)
+    lowest = float(np.finfo(dtype).min)
+    far = [-2000, -2001, -5000.5, -30000, lowest / 2, lowest]
+    if dtype == np.float32:
+        far += [-1e5, -1e7, -3e9, -1e15, -2.0 ** 60, -1e20, -1e30]
+    logits = np.empty((40, 16, 4), dtype)
+    for row in logits:
+        best = rng.choice(far, 16).astype(dtype)
+        row[:] = lowest
+        row[np.arange(16), rng.integers(0, 4, 16)] = best
+        row[rng.integers(0, 16)] = 0
+    ordered = np.sort(logits.astype(np.float64), 2)[:, :, ::-1]
+    kept = np.zeros((40, 16))
+    for row, k in zip(ordered, kept):
+        k[sorted(range(16), key=lambda g: (-row[g, 0], -row[g, 1]))[:top_groups]] = 1
+    logits = logits.reshape(40, 64)
+    want = largest_first(logits, 7, np.repeat(kept, 4, 1))
+    check(stream, logits, want, ops.SOFTMAX, bias=None if bias is None else np.zeros(64), groups=16,
+          top_groups=top_groups, group_best=2)
