@@ -16,11 +16,11 @@ namespace {
 // STEPS steps of K, the same for every column, and the waves' sums meet in LDS, in their order.
 //
 // A lane's operand is a 16-byte piece of a weights' row as it is stored, so nothing is
-// unpacked; what costs time beside the memory is the number of load instructions (one row, 14336 x 4096,
-// 31 MB that are read in 6.1 us at best: weights alone 6.9 us, with their scales a word at a
-// time and x at each step 11.5, as here 8.2).  So scales are loaded four steps at a time, x once for all
-// of the workgroup's columns, and a step's weights for the next column as soon as they
-// have been multiplied.
+// unpacked; what costs time beside the memory is the number of load instructions (one row, 14336 x 4096, which
+// the tiles take by now, 31 MB in the memory-side cache, 5.0 us at the rate of reads alone: weights alone 6.9 us, with
+// their scales a word at a time and x at each step 11.5, as here 8.2).  So scales are loaded four steps at a
+// time, x once for all of the workgroup's columns, and a step's weights for the next column as
+// soon as they have been multiplied.
 constexpr uint32_t kFewRows = 16;
 
 template <typename F, int... I>
@@ -206,7 +206,11 @@ int launch_few(const ProductArgs& a, hipStream_t stream) {
 // - down of up to 8, where there are few tiles (8 experts of 4096 x 14336, 4 tokens of two: 256 tiles, 30 us
 //   and 60; 64 experts of 4096 x 1408, 2 tokens of six: 384, 15.8 and 16.9; 128 of 2048 x 768, 4 of eight:
 //   512, 15.3 and 13.0);
-// - and K too short for the tiles' four steps, if it is not too long for a workgroup's waves.
+// - and K too short for the tiles' four steps, for any number of rows.  That is right but slow where there are
+//   many: every 16 rows read the weights again, and results leave 2 or 4 bytes a lane (K 128, 256 and 384 here,
+//   and 512 in tiles: 4096 x 4096 outputs 45, 65, 57 and 12 us; 8192 x 14336, 6 bits, 318, 451, 436 and 80; gate/up of
+//   4096 tokens' four of 32 experts of 2880 181, 277, 254 and 91; down of 4096 tokens' eight of 128 experts to 2048
+//   268, 333, 335 and 151; 16 x 4096 4.7, 4.8, 4.9 and 4.5).
 template <Result R>
 bool few_rows(const ProductArgs& a) {
     const uint64_t columns = a.outputs, steps = a.kp / kStep;
@@ -215,7 +219,7 @@ bool few_rows(const ProductArgs& a) {
     if constexpr (R == Result::kPairs)
         return a.rows <= 8 * uint64_t{a.experts} && steps <= 128 &&
                most_expert_tiles(a.rows, a.experts, 64) * ((columns + 127) / 128) < 512;
-    return a.rows <= kFewRows && columns <= 32 * 191 && steps > 64 && steps <= 128;
+    return a.rows <= kFewRows && (columns + 31) / 32 < kEnoughTiles && steps > 64 && steps <= 128;
 }
 
 template <int BITS, Result R>

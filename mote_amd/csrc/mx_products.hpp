@@ -29,6 +29,9 @@ struct ProductArgs {
     uint32_t experts, top;
 };
 
+// Tiles that keep the chip busy: one for three in four compute units.
+constexpr uint64_t kEnoughTiles = 192;
+
 // Products of many rows (mx_tiles.hip).
 int launch_tiles(Result result, const ProductArgs& a, int bits, hipStream_t stream);
 

@@ -8,8 +8,8 @@
 //
 // A thread has a block: 64 or 128 bytes in, one conversion of the whole block (or one a
 // pair), 16 and 8 bytes and a scale out, each contiguous over a wave.  Bound by the bytes: 4000 x 14336
-// of f16 to 6 bits 25 us and back 25, 160 MB each, 6.4 TB/s (some of it from the memory-side
-// cache); 64 x 4096 2.7 and 2.9 us, a launch's chain.
+// of f16 to 6 bits 25 to 26 us and back 25, 160 MB each, 6.2 to 6.4 TB/s (some of it from the
+// memory-side cache); 64 x 4096 2.7 and 2.9 us, a launch's chain.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

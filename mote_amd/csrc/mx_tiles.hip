@@ -6,11 +6,12 @@
 // scales.  A wave multiplies 32 x 32 x 64 (half the time of 16 x 16 x 128 a
 // product), reading operands as the instruction takes them.  A row's 16-byte pieces lie
 // at piece ^ (row / 4 % 4), so 16 lanes that read the same piece of 16 rows touch every
-// bank once.  One barrier a stage: behind it, all waves' loads of the stage have
-// landed and the stage before is free to be loaded again.
+// bank once; but lanes l and l + 32 read neighbouring pieces, and those two of 8 rows fall on 8 of the 16 places,
+// two on each: 35 to 40 % of the LDS cycles are conflicts.  One barrier a stage: behind it, all waves' loads of
+// the stage have landed and the stage before is free to be loaded again.
 //
-// What bounds large ones (4096 x 14336 x 4096 in 4 bits, 148 us, 3.2 PFLOP/s of the 6.2 that the instruction reaches on
-// registers alone; each part taken out in turn): the matrix instructions alone some 98 us, in four
+// What bounds large ones (4096 x 14336 x 4096 in 4 bits, 142 to 151 us from card to card, 3.2 to 3.4 PFLOP/s of the 6.2
+// that the instruction reaches on registers alone; each part taken out in turn): the matrix instructions alone some 98 us, in four
 // rounds of 3.5 rounds' tiles; the results, which all compute units write at one time, 24; the loads 22, LDS
 // reads 13.  Stages of 256 elements, whose loads have pieces of 128 bytes (53 bytes a cycle and compute
 // unit in place of 36), were level (152 and 154 us) and slower for experts (130 and 122).
@@ -455,12 +456,10 @@ int launch(const ProductArgs& a, hipStream_t stream) {
 // of 4096, 6 bits: 64 rows in 32, 64 and 256 tiles of 128 x 64, 64 x 64 and 32 x 32: 14.3, 10.4 and 6.8 us;
 // 256 rows in 64, 128 and 256 of 128 x 128, 128 x 64 and 64 x 64: 17.8, 14.5 and 12.0; 4096 rows in 256, 1024
 // and 2048 of 256 x 256, 128 x 128 and 128 x 64: 50, 78 and 96).  In the small ones waves divide K.
-constexpr uint64_t kEnough = 192;
-
 template <int BITS, Result R>
 int choose(const ProductArgs& a, hipStream_t stream) {
     const auto enough = [&](uint32_t weight_rows, uint32_t rows) {
-        return row_tiles<R>(a, rows) * column_tiles<R>(a, weight_rows) >= kEnough;
+        return row_tiles<R>(a, rows) * column_tiles<R>(a, weight_rows) >= kEnoughTiles;
     };
     if constexpr (kOfExperts<R>) {
         // An expert's rows seldom fill its last tile, so tiles follow the mean of the rows (gate/up, 6 bits, us;
